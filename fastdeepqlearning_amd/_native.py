@@ -86,6 +86,34 @@ class EpisodeVmapSpec(C.Structure):
                 ("K", C.c_int32), ("n_step", C.c_int32), ("gamma", C.c_float), ("reward_fn", RewardFn)]
 
 
+class CausalConv(C.Structure):
+    _fields_ = [(k, C.c_int32) for k in ("size", "dtype", "T", "R", "D", "K", "silu")] + [
+        ("x", C.c_void_p), ("x_st", C.c_int64), ("x_sr", C.c_int64), ("weight", C.c_void_p), ("bias", C.c_void_p),
+        ("reset", C.c_void_p), ("reset_st", C.c_int64), ("reset_sr", C.c_int64), ("state_in", C.c_void_p), ("state_in_sr", C.c_int64),
+        ("y", C.c_void_p), ("state_out", C.c_void_p), ("dy", C.c_void_p), ("dy_st", C.c_int64), ("dy_sr", C.c_int64),
+        ("dstate_out", C.c_void_p), ("dx", C.c_void_p), ("dstate_in", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class Scan(C.Structure):
+    _fields_ = [(k, C.c_int32) for k in ("size", "dtype", "T", "R", "D", "N", "G", "dt_softplus")] + [
+        ("x", C.c_void_p), ("dt", C.c_void_p), ("z", C.c_void_p)] + [
+        (k, C.c_int64) for k in ("x_st", "x_sr", "dt_st", "dt_sr", "z_st", "z_sr")] + [("B", C.c_void_p), ("C", C.c_void_p)] + [
+        (k, C.c_int64) for k in ("B_st", "B_sr", "B_sg", "C_st", "C_sr", "C_sg")] + [
+        (k, C.c_void_p) for k in ("A", "skip", "dt_bias", "reset")] + [("reset_st", C.c_int64), ("reset_sr", C.c_int64),
+        ("state_in", C.c_void_p), ("state_in_sr", C.c_int64), ("y", C.c_void_p), ("state_out", C.c_void_p), ("checkpoints", C.c_void_p),
+        ("dy", C.c_void_p), ("dy_st", C.c_int64), ("dy_sr", C.c_int64)] + [
+        (k, C.c_void_p) for k in ("dstate_out", "dx", "ddt", "dz", "dB", "dC", "dA", "dskip", "ddt_bias", "dstate_in", "workspace")] + [
+        ("workspace_bytes", C.c_int64)]
+
+
+class Gated(C.Structure):
+    _fields_ = [("size", C.c_int32), ("dtype", C.c_int32), ("M", C.c_int64), ("D", C.c_int32), ("F", C.c_int32), ("act", C.c_int32),
+                ("x", C.c_void_p), ("x_sr", C.c_int64)] + [
+        (k, C.c_void_p) for k in ("w_gate", "w_up", "b_gate", "b_up", "y", "pre", "dy")] + [("dy_sr", C.c_int64)] + [
+        (k, C.c_void_p) for k in ("dx", "dw_gate", "dw_up", "db_gate", "db_up", "workspace")] + [("workspace_bytes", C.c_int64)]
+
+
 # Every symbol include/fdql.h declares, with its ctypes signature (restype, argtypes).
 _vp, _i32, _i64, _u64, _f32 = C.c_void_p, C.c_int32, C.c_int64, C.c_uint64, C.c_float
 SIGNATURES = {
@@ -140,6 +168,16 @@ SIGNATURES = {
                                  _vp]),
     "fdql_agent_stats": (C.c_int, [_vp, C.POINTER(AgentStats)]),
     "fdql_agent_profile_update": (_i32, [_vp, C.POINTER(Batch), _vp, _vp, _u64, C.POINTER(KernelTime), _i32, _vp]),
+    "fdql_causal_conv": (C.c_int, [C.POINTER(CausalConv), _vp]),
+    "fdql_causal_conv_workspace_bytes": (_i64, [C.POINTER(CausalConv)]),
+    "fdql_causal_conv_backward": (C.c_int, [C.POINTER(CausalConv), _vp]),
+    "fdql_scan": (C.c_int, [C.POINTER(Scan), _vp]),
+    "fdql_scan_checkpoint_floats": (_i64, [C.POINTER(Scan)]),
+    "fdql_scan_workspace_bytes": (_i64, [C.POINTER(Scan), _i32]),
+    "fdql_scan_backward": (C.c_int, [C.POINTER(Scan), _vp]),
+    "fdql_gated": (C.c_int, [C.POINTER(Gated), _vp]),
+    "fdql_gated_workspace_bytes": (_i64, [C.POINTER(Gated), _i32]),
+    "fdql_gated_backward": (C.c_int, [C.POINTER(Gated), _vp]),
     "fdql_debug_set_gemm_dense_shape": (C.c_int, [_i32]),
     "fdql_test_gemm": (C.c_int, [_vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _i32, _i32, _i32, _i32, _i32, _vp, _i32,
                                  _i32, _vp]),

@@ -1,0 +1,168 @@
+// Entry points of the sequence operators: argument checks, empty shapes, launches.
+#include "seq.h"
+
+using namespace fdql;
+
+namespace {
+
+constexpr int64_t MAX_THREADS = 0xffffffffll;      // threads of a launch
+
+__global__ __launch_bounds__(256) void k_seq_zero(float *p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0.f;
+}
+__global__ __launch_bounds__(256) void k_seq_zero16(uint16_t *p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
+}
+// dst [R, per] dense = src (row stride sr) or zeros
+__global__ __launch_bounds__(256) void k_seq_copy_rows(const float *src, int64_t sr, float *dst, int64_t R, int64_t per) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < R * per; i += (int64_t)gridDim.x * 256) dst[i] = src ? src[i / per * sr + i % per] : 0.f;
+}
+dim3 grid_for(int64_t n) { return dim3((unsigned)(n < 256 * 1024 ? (n + 255) / 256 : 1024)); }
+
+int zero(void *p, int64_t n, int32_t dtype, hipStream_t s) {   // a kernel, not a memset: the call may be captured
+  if (!p || n <= 0) return FDQL_OK;
+  if (dtype == FDQL_F32) hipLaunchKernelGGL(k_seq_zero, grid_for(n), dim3(256), 0, s, (float *)p, n);
+  else hipLaunchKernelGGL(k_seq_zero16, grid_for(n), dim3(256), 0, s, (uint16_t *)p, n);
+  FDQL_HIP(hipGetLastError());
+  return FDQL_OK;
+}
+int copy_rows(const float *src, int64_t sr, float *dst, int64_t R, int64_t per, hipStream_t s) {
+  if (!dst || R * per == 0) return FDQL_OK;
+  hipLaunchKernelGGL(k_seq_copy_rows, grid_for(R * per), dim3(256), 0, s, src, sr, dst, R, per);
+  FDQL_HIP(hipGetLastError());
+  return FDQL_OK;
+}
+
+bool type_ok(int32_t t) { return t == FDQL_F32 || t == FDQL_BF16 || t == FDQL_F16; }
+
+int check_conv(const fdql_causal_conv_t *p) {
+  FDQL_REQUIRE(p && p->size == (int32_t)sizeof(*p), "causal_conv: struct size %d, this library has %d", p ? p->size : 0, (int)sizeof(*p));
+  FDQL_REQUIRE(type_ok(p->dtype), "causal_conv: dtype %d (float32, bf16 or fp16)", p->dtype);
+  FDQL_REQUIRE(p->T >= 0 && p->R >= 0 && p->D >= 1, "causal_conv: T %d, R %d, D %d", p->T, p->R, p->D);
+  FDQL_REQUIRE(p->K >= 2 && p->K <= 4, "causal_conv: %d taps (2 to 4)", p->K);
+  FDQL_REQUIRE(((int64_t)p->D + 63) / 64 * p->R * ((p->T + 7ll) / 8 + 1) * 64 < MAX_THREADS, "causal_conv: T %d x R %d x D %d is more than one launch", p->T, p->R, p->D);
+  return FDQL_OK;
+}
+int check_scan(const fdql_scan_t *p) {
+  FDQL_REQUIRE(p && p->size == (int32_t)sizeof(*p), "scan: struct size %d, this library has %d", p ? p->size : 0, (int)sizeof(*p));
+  FDQL_REQUIRE(type_ok(p->dtype), "scan: dtype %d (float32, bf16 or fp16)", p->dtype);
+  FDQL_REQUIRE(p->T >= 0 && p->R >= 0 && p->D >= 1, "scan: T %d, R %d, D %d", p->T, p->R, p->D);
+  FDQL_REQUIRE(p->N >= 1 && p->N <= 64, "scan: %d states (1 to 64)", p->N);
+  FDQL_REQUIRE(p->G >= 1 && p->D % p->G == 0, "scan: %d groups do not divide %d channels", p->G, p->D);
+  // at most 2048 + rows x tiles waves, finish kernels of 1024 threads per 16 channels and state
+  FDQL_REQUIRE(((int64_t)p->R * p->G * ((p->D / p->G + 15) / 16) + 4096) * 64 * 16 < MAX_THREADS, "scan: R %d x D %d is more than one launch", p->R, p->D);
+  return FDQL_OK;
+}
+int check_gated(const fdql_gated_t *p) {
+  FDQL_REQUIRE(p && p->size == (int32_t)sizeof(*p), "gated: struct size %d, this library has %d", p ? p->size : 0, (int)sizeof(*p));
+  FDQL_REQUIRE(type_ok(p->dtype), "gated: dtype %d (float32, bf16 or fp16)", p->dtype);
+  FDQL_REQUIRE(p->M >= 0 && p->D >= 1 && p->F >= 1, "gated: M %lld, D %d, F %d", (long long)p->M, p->D, p->F);
+  FDQL_REQUIRE(p->act >= FDQL_ACT_SILU && p->act <= FDQL_ACT_SIGMOID, "gated: activation %d", p->act);
+  FDQL_REQUIRE(p->M <= 128ll * 65535 && (p->M / 64 + 1) * ((int64_t)(p->F > p->D ? p->F : p->D) / 64 + 1) * 256 < MAX_THREADS,
+               "gated: M %lld x (D %d, F %d) is more than one launch", (long long)p->M, p->D, p->F);
+  FDQL_REQUIRE(((int64_t)p->F / 128 + 1) * (p->D / 128 + 1) * 256 * 2 < MAX_THREADS / 16, "gated: weights %d x %d are more than one launch", p->F, p->D);
+  return FDQL_OK;
+}
+int check_workspace(const char *what, const void *ws, int64_t have, int64_t need) {
+  FDQL_REQUIRE(need <= 0 || (ws && have >= need && ((uintptr_t)ws & 15) == 0), "%s: workspace of %lld bytes (16-byte aligned), %lld are needed", what, (long long)have,
+               (long long)need);
+  return FDQL_OK;
+}
+#define FDQL_TRY(call)              \
+  do {                              \
+    const int _rc = (call);         \
+    if (_rc != FDQL_OK) return _rc; \
+  } while (0)
+
+}  // namespace
+
+extern "C" int fdql_causal_conv(const fdql_causal_conv_t *p, void *stream) {
+  FDQL_TRY(check_conv(p));
+  if (p->R == 0) return FDQL_OK;
+  FDQL_REQUIRE(p->weight && (p->T == 0 || (p->x && p->y)), "causal_conv: x, weight and y are needed");
+  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1 && p->state_in_sr == (int64_t)(p->K - 1) * p->D),
+               "causal_conv: the state is updated in place only in a single step over dense rows");
+  FDQL_HIP(seqconv_fwd_launch(*p, (hipStream_t)stream));
+  return FDQL_OK;
+}
+extern "C" int64_t fdql_causal_conv_workspace_bytes(const fdql_causal_conv_t *p) {
+  if (check_conv(p) != FDQL_OK) return FDQL_EINVAL;
+  return seqconv_workspace_bytes(*p);
+}
+extern "C" int fdql_causal_conv_backward(const fdql_causal_conv_t *p, void *stream) {
+  hipStream_t s = (hipStream_t)stream;
+  FDQL_TRY(check_conv(p));
+  if (p->R == 0) {
+    FDQL_TRY(zero(p->dweight, (int64_t)p->D * p->K, FDQL_F32, s));
+    return zero(p->dbias, p->D, FDQL_F32, s);
+  }
+  FDQL_REQUIRE(p->weight && (p->T == 0 || (p->x && p->dy)), "causal_conv backward: x, weight and dy are needed");
+  FDQL_TRY(check_workspace("causal_conv backward", p->workspace, p->workspace_bytes, seqconv_workspace_bytes(*p)));
+  FDQL_HIP(seqconv_bwd_launch(*p, s));
+  return FDQL_OK;
+}
+
+extern "C" int fdql_scan(const fdql_scan_t *p, void *stream) {
+  hipStream_t s = (hipStream_t)stream;
+  FDQL_TRY(check_scan(p));
+  if (p->R == 0) return FDQL_OK;
+  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1 && !p->checkpoints && p->state_in_sr == (int64_t)p->D * p->N),
+               "scan: the state is updated in place only in a single step over dense rows");
+  if (p->T == 0) return copy_rows(p->state_in, p->state_in_sr, p->state_out, p->R, (int64_t)p->D * p->N, s);
+  FDQL_REQUIRE(p->x && p->dt && p->A && p->B && p->C && p->y, "scan: x, dt, A, B, C and y are needed");
+  FDQL_TRY(check_workspace("scan", p->workspace, p->workspace_bytes, scan_workspace_bytes(*p, false)));
+  FDQL_HIP(scan_fwd_launch(*p, s));
+  return FDQL_OK;
+}
+extern "C" int64_t fdql_scan_checkpoint_floats(const fdql_scan_t *p) {
+  if (check_scan(p) != FDQL_OK) return FDQL_EINVAL;
+  return scan_checkpoint_floats(*p);
+}
+extern "C" int64_t fdql_scan_workspace_bytes(const fdql_scan_t *p, int32_t backward) {
+  if (check_scan(p) != FDQL_OK) return FDQL_EINVAL;
+  return scan_workspace_bytes(*p, backward != 0);
+}
+extern "C" int fdql_scan_backward(const fdql_scan_t *p, void *stream) {
+  hipStream_t s = (hipStream_t)stream;
+  FDQL_TRY(check_scan(p));
+  if (p->R == 0 || p->T == 0) {
+    FDQL_TRY(zero(p->dA, (int64_t)p->D * p->N, FDQL_F32, s));
+    FDQL_TRY(zero(p->dskip, p->D, FDQL_F32, s));
+    FDQL_TRY(zero(p->ddt_bias, p->D, FDQL_F32, s));
+    return copy_rows(p->dstate_out, (int64_t)p->D * p->N, p->dstate_in, p->R, (int64_t)p->D * p->N, s);
+  }
+  FDQL_REQUIRE(p->x && p->dt && p->A && p->B && p->C && p->dy, "scan backward: x, dt, A, B, C and dy are needed");
+  FDQL_REQUIRE(p->checkpoints, "scan backward: the forward call's checkpoints are needed");
+  FDQL_REQUIRE(p->dx && p->ddt && p->dA && p->dB && p->dC, "scan backward: dx, ddt, dA, dB and dC are needed");
+  FDQL_TRY(check_workspace("scan backward", p->workspace, p->workspace_bytes, scan_workspace_bytes(*p, true)));
+  FDQL_HIP(scan_bwd_launch(*p, s));
+  return FDQL_OK;
+}
+
+extern "C" int fdql_gated(const fdql_gated_t *p, void *stream) {
+  FDQL_TRY(check_gated(p));
+  if (p->M == 0) return FDQL_OK;
+  FDQL_REQUIRE(p->x && p->w_gate && p->w_up && p->y, "gated: x, both weights and y are needed");
+  FDQL_REQUIRE(!p->b_gate == !p->b_up, "gated: both biases or neither");
+  FDQL_HIP(gated_fwd_launch(*p, (hipStream_t)stream));
+  return FDQL_OK;
+}
+extern "C" int64_t fdql_gated_workspace_bytes(const fdql_gated_t *p, int32_t backward) {
+  if (check_gated(p) != FDQL_OK) return FDQL_EINVAL;
+  return gated_workspace_bytes(*p, backward != 0);
+}
+extern "C" int fdql_gated_backward(const fdql_gated_t *p, void *stream) {
+  hipStream_t s = (hipStream_t)stream;
+  FDQL_TRY(check_gated(p));
+  FDQL_REQUIRE(!p->dw_gate == !p->dw_up && !p->db_gate == !p->db_up, "gated backward: the gradients of the gate and up sides come together");
+  if (p->M == 0) {
+    FDQL_TRY(zero(p->dw_gate, (int64_t)p->F * p->D, p->dtype, s));
+    FDQL_TRY(zero(p->dw_up, (int64_t)p->F * p->D, p->dtype, s));
+    FDQL_TRY(zero(p->db_gate, p->F, p->dtype, s));
+    return zero(p->db_up, p->F, p->dtype, s);
+  }
+  FDQL_REQUIRE(p->x && p->w_gate && p->w_up && p->dy && p->pre, "gated backward: x, both weights, dy and the forward call's pre are needed");
+  FDQL_TRY(check_workspace("gated backward", p->workspace, p->workspace_bytes, gated_workspace_bytes(*p, true)));
+  FDQL_HIP(gated_bwd_launch(*p, s));
+  return FDQL_OK;
+}

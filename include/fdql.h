@@ -412,6 +412,116 @@ int32_t fdql_agent_profile_update(fdql_agent_t *agent, const fdql_batch_t *batch
                                   int32_t cap, void *stream);
 
 /* ------------------------------------------------------------------------------------ */
+/* Sequence operators: a recurrent block over replay windows                             */
+/* ------------------------------------------------------------------------------------ */
+/* The reference's only learned operator over the time axis is nn.GRU (franQ/Agent/components/encoder.py:40-42, 78-94).  These
+ * three are a design of this build: the short causal convolution, the selective state-space scan and the gated linear unit of
+ * a recurrent block, for training on [T, rows, *] windows, for prompts and for one acting step (T = 1).
+ *
+ * Common to all: `size` is sizeof the struct (checked); dtype is FDQL_F32, FDQL_BF16 or FDQL_F16 and is the type of every
+ * void * tensor; float * tensors are float32 whatever dtype is, and all sums and states are kept in float32.  Activations are
+ * time-major with a dense last dimension and any element strides _st (time) and _sr (row), zero included; outputs and
+ * gradients are dense [T, R, D] unless a stride is named.  No alignment beyond the element's is needed.  reset (or NULL) is one byte per
+ * step and row, nonzero where a new sequence begins: whatever came before that step is dropped (selected away, so that a NaN
+ * there does not pass).  T or R of 0 is allowed.  Outputs must not overlap inputs except where a comment allows it.
+ * workspace: device scratch of at least the *_workspace_bytes() of the same struct (its pointers are not read by that call),
+ * 16-byte aligned, private to the call until it has run on its stream.  Calls are asynchronous on `stream`, allocate
+ * nothing, may be captured into a graph, and give the same bits for the same inputs.  Unsupported arguments: FDQL_EINVAL. */
+#define FDQL_BF16 2
+#define FDQL_F16 3
+
+/* y_t = f(bias + sum_{j<K} weight[:, K-1-j] * x_{t-j}), f = SiLU or identity, channel by channel; x_{t-j} counts as zero when a
+ * reset lies in (t-j, t].  Inputs before step 0 come from state_in [R, K-1, D] (row stride state_in_sr, oldest first; NULL: zeros); state_out
+ * [R, K-1, D] (or NULL) receives the last K-1 inputs (zeros for those before the last reset).  state_out may be state_in when T == 1.
+ * Backward: dy [T, R, D] (strides dy_st, dy_sr) and dstate_out (or NULL) -> dx, dweight [D, K], dbias [D], dstate_in (each or NULL).                  */
+typedef struct {
+  int32_t size, dtype;
+  int32_t T, R, D, K;                 /* K: 2..4 taps                                          */
+  int32_t silu;
+  const void *x;
+  int64_t x_st, x_sr;
+  const float *weight, *bias;         /* [D, K], [D] or NULL                                    */
+  const uint8_t *reset;
+  int64_t reset_st, reset_sr;
+  const void *state_in;
+  int64_t state_in_sr;
+  void *y, *state_out;                /* forward                                                */
+  const void *dy;                     /* backward                                               */
+  int64_t dy_st, dy_sr;
+  const void *dstate_out;             /* [R, K-1, D] dense                                      */
+  void *dx, *dstate_in;
+  float *dweight, *dbias;
+  void *workspace;                    /* backward only                                          */
+  int64_t workspace_bytes;
+} fdql_causal_conv_t;
+int fdql_causal_conv(const fdql_causal_conv_t *p, void *stream);
+int64_t fdql_causal_conv_workspace_bytes(const fdql_causal_conv_t *p);
+int fdql_causal_conv_backward(const fdql_causal_conv_t *p, void *stream);
+
+/* Per row and channel d of group g = d / (D / G), with state h [N]:
+ *   delta = softplus(dt_t + dt_bias)   (dt_t + dt_bias itself without dt_softplus)
+ *   h     = exp(delta * A[d]) * h + delta * x_t * B_t[g]      (the first term dropped at a reset)
+ *   y_t   = (C_t[g] . h + skip[d] * x_t) * SiLU(z_t)          (factors that are NULL left out)
+ * state_in [R, D, N] (row stride state_in_sr, NULL: zeros), state_out [R, D, N] dense (or NULL; may be state_in when T == 1).
+ * checkpoints: fdql_scan_checkpoint_floats() floats that the forward call fills for the backward call of the same inputs (NULL
+ * when there is none).  Backward: dy (strides dy_st, dy_sr) and dstate_out (or NULL) -> every gradient; those of optional inputs that are NULL may be NULL,
+ * dstate_in always.                                                                                              */
+typedef struct {
+  int32_t size, dtype;
+  int32_t T, R, D, N, G;              /* N: 1..64 states, G groups (G divides D)                */
+  int32_t dt_softplus;
+  const void *x, *dt, *z;             /* z: or NULL                                             */
+  int64_t x_st, x_sr, dt_st, dt_sr, z_st, z_sr;
+  const void *B, *C;                  /* [T, R, G, N], last dimension dense                     */
+  int64_t B_st, B_sr, B_sg, C_st, C_sr, C_sg;
+  const float *A;                     /* [D, N]                                                 */
+  const float *skip, *dt_bias;        /* [D] or NULL                                            */
+  const uint8_t *reset;
+  int64_t reset_st, reset_sr;
+  const float *state_in;
+  int64_t state_in_sr;
+  void *y;                            /* forward                                                */
+  float *state_out;
+  float *checkpoints;
+  const void *dy;                     /* backward                                               */
+  int64_t dy_st, dy_sr;
+  const float *dstate_out;            /* [R, D, N] dense                                        */
+  void *dx, *ddt, *dz, *dB, *dC;
+  float *dA, *dskip, *ddt_bias, *dstate_in;
+  void *workspace;
+  int64_t workspace_bytes;
+} fdql_scan_t;
+int fdql_scan(const fdql_scan_t *p, void *stream);
+int64_t fdql_scan_checkpoint_floats(const fdql_scan_t *p);
+int64_t fdql_scan_workspace_bytes(const fdql_scan_t *p, int32_t backward);
+int fdql_scan_backward(const fdql_scan_t *p, void *stream);
+
+/* y = f(x Wg^T + bg) * (x Wu^T + bu), f = SiLU, GELU (the erf form) or sigmoid; x [M, D] (row stride x_sr), weights [F, D] dense, y [M, F] dense.
+ * pre: [2, M, F] float32 (or NULL) that the forward call fills with both products for the backward call.
+ * Backward: dy [M, F] (row stride dy_sr) -> dx [M, D], dw_gate, dw_up [F, D], db_gate, db_up [F] (each or NULL), all of the type dtype.            */
+#define FDQL_ACT_SILU 0
+#define FDQL_ACT_GELU 1
+#define FDQL_ACT_SIGMOID 2
+typedef struct {
+  int32_t size, dtype;
+  int64_t M;
+  int32_t D, F, act;
+  const void *x;
+  int64_t x_sr;
+  const void *w_gate, *w_up, *b_gate, *b_up;   /* biases: both or neither                       */
+  void *y;
+  float *pre;
+  const void *dy;
+  int64_t dy_sr;
+  void *dx, *dw_gate, *dw_up, *db_gate, *db_up;
+  void *workspace;
+  int64_t workspace_bytes;
+} fdql_gated_t;
+int fdql_gated(const fdql_gated_t *p, void *stream);
+int64_t fdql_gated_workspace_bytes(const fdql_gated_t *p, int32_t backward);
+int fdql_gated_backward(const fdql_gated_t *p, void *stream);
+
+/* ------------------------------------------------------------------------------------ */
 /* Test hook: the grouped MFMA GEMM on its own (C = A * op(B) + bias, fp32)               */
 int fdql_test_gemm(const float *A, int32_t lda, int32_t a_kc, const float *B, int32_t ldb, int32_t b_kc,
                    const float *bias, float *C, int32_t ldc, int32_t M, int32_t N, int32_t K,

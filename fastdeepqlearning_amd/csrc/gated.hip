@@ -7,17 +7,17 @@
 // their column sums; then dx = dg Wg + du Wu is one product over 2 F, and dWg = dg^T x, dWu = du^T x are one launch with the rows
 // split over workgroups where the weights alone leave the card idle (float32 slabs, added in order).
 //
-// Tiles: BM x 128 per workgroup of four waves, K in slices of 128 bytes; LDS rows are one slice long, 16-byte chunk c of row n lies at
-// c ^ swz(n), and both operands are kept contraction-contiguous: an operand that lies the other way in memory is transposed in
-// registers on its way to LDS (16-byte rows of k against 4 columns: byte permutes for 16-bit types, renaming for float).  So one inner loop
-// serves all three products: v_mfma_f32_32x32x16 (bf16, fp16) or four v_mfma_f32_32x32x2 (float) per pair of 16-byte fragments; which k
-// a lane half holds is the same on both sides and does not matter.  Slices are double-buffered, the next one in flight in registers.
+// k_gated_mma serves all three products: tiles of BM x BN, slices of the contraction in an LDS ring filled by LDS-DMA (see there).  Tensors whose
+// rows are not 16-byte aligned take k_gated_any: the same tiles with element loads through registers.  Matrix instructions:
+// v_mfma_f32_32x32x16 (bf16, fp16) or four v_mfma_f32_32x32x2 (float) per pair of 16-byte fragments; which k a lane half holds is the same on
+// both sides and does not matter.
 //
 // Few rows (M <= 32) are bound by the weights' bytes and by latency: k_gated_rows gives 16 outputs to a workgroup, splits K over its
 // four waves and reads fragments straight from memory.
 #include "seq.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fdql {
 namespace {
@@ -27,8 +27,6 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
-
-constexpr int BN = 128;
 
 enum Mode { FWD, DX, DW };
 
@@ -108,12 +106,12 @@ __device__ __forceinline__ v4i row_chunk(const T *row, int64_t k, int64_t K) {
   }
 }
 
-// A K slice of `rows` LDS rows on its way: NCH 16-byte chunks per thread.
+// A slice of LDS rows on its way through registers: NCH 16-byte chunks per thread.
 template <int NCH>
 struct Flight { v4i c[NCH]; };
 
-// rows_ptr(n) -> first element of operand row n or nullptr (zeros)
-template <typename T, bool VEC, int NCH, typename F>
+// row_ptr(n) -> first element of operand row n or nullptr (zeros)
+template <typename T, int NCH, typename F>
 __device__ __forceinline__ void fetch_rows(Flight<NCH> &f, F row_ptr, int64_t k0, int64_t K) {
   constexpr int E = 16 / sizeof(T);
 #pragma unroll
@@ -121,7 +119,7 @@ __device__ __forceinline__ void fetch_rows(Flight<NCH> &f, F row_ptr, int64_t k0
     const int n = (threadIdx.x >> 3) + 32 * i, c = threadIdx.x & 7;
     const T *row = row_ptr(n);
     v4i z = {0, 0, 0, 0};
-    f.c[i] = row ? row_chunk<T, VEC>(row, k0 + c * E, K) : z;
+    f.c[i] = row ? row_chunk<T, false>(row, k0 + c * E, K) : z;
   }
 }
 template <int NCH>
@@ -133,41 +131,26 @@ __device__ __forceinline__ void put_rows(const Flight<NCH> &f, char *lds) {
   }
 }
 
-// The other orientation: memory is [k][column] with row length ld; thread = 4 columns x E rows of k, transposed in registers to four chunks.
-template <typename T, bool VEC>
-__device__ __forceinline__ void fetch_cols(Flight<4> &f, const T *base, int64_t ld, int64_t k0, int64_t K, int64_t col0, int64_t cols) {
+// The other orientation: memory is [k][column] with row length ld; thread = NJ columns x E rows of k, transposed in registers.
+template <typename T, int NJ>
+__device__ __forceinline__ void fetch_cols(Flight<NJ> &f, const T *base, int64_t ld, int64_t k0, int64_t K, int64_t col0, int64_t cols) {
   constexpr int E = 16 / sizeof(T);
-  typedef T vec4 __attribute__((ext_vector_type(4)));
-  const int64_t col = col0 + (threadIdx.x & 31) * 4;
+  typedef T vec __attribute__((ext_vector_type(E)));
+  const int64_t col = col0 + (threadIdx.x & 31) * NJ;
   const int64_t k = k0 + (threadIdx.x >> 5) * E;
-  vec4 r[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) r[e][j] = T(0.f);
-    if (k + e < K) {
-      if constexpr (VEC) {
-        if (col < cols) r[e] = *reinterpret_cast<const vec4 *>(base + (k + e) * ld + col);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (col + j < cols) r[e][j] = base[(k + e) * ld + col + j];
-      }
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    typedef T vec __attribute__((ext_vector_type(E)));
+  for (int j = 0; j < NJ; ++j) {
     vec v;
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = r[e][j];
+    for (int e = 0; e < E; ++e) v[e] = k + e < K && col + j < cols ? base[(k + e) * ld + col + j] : T(0.f);
     f.c[j] = __builtin_bit_cast(v4i, v);
   }
 }
-__device__ __forceinline__ void put_cols(const Flight<4> &f, char *lds) {
+template <int NJ>
+__device__ __forceinline__ void put_cols(const Flight<NJ> &f, char *lds) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int n = (threadIdx.x & 31) * 4 + j, c = threadIdx.x >> 5;
+  for (int j = 0; j < NJ; ++j) {
+    const int n = (threadIdx.x & 31) * NJ + j, c = threadIdx.x >> 5;
     *reinterpret_cast<v4i *>(lds + n * 128 + ((c ^ swz(n)) << 4)) = f.c[j];
   }
 }
@@ -182,34 +165,92 @@ __device__ __forceinline__ void tile_of(int bid, int tiles_m, int tiles_n, int &
   tn = in / h;
 }
 
-template <typename T, int MODE, int BM, bool VEC>
-__global__ __launch_bounds__(256, 2) void k_gated_tile(Args a) {
-  constexpr int BK = 128 / sizeof(T), MT = BM / 64, NT = 2, NCA = BM / 32;
+// A wave's accumulators: rows wm of two, 64 columns wn.  Register r of a 32 x 32 tile: row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32.
+// WHOLE: the tile lies inside the matrix.  An address is a running scalar part and one 32-bit offset per lane (rows are at most 2^24 long).
+template <typename T, int MODE, int MT, int BM, bool WHOLE>
+__device__ __forceinline__ void store_part(const Args &a, const v16f (&acc)[MT][2], int64_t m0, int64_t n0, int64_t f0, int wm, int wn, int which, int ks) {
+  const fdql_gated_t &p = a.p;
+  const int lane = threadIdx.x & 63;
+  const int64_t ld = MODE == FWD ? p.F : p.D, rows = MODE == DW ? p.F : p.M, top = m0 + wm * (BM / 2);
+  const unsigned at = (unsigned)(lane >> 5) * 4u * (unsigned)ld + (lane & 31);
+  const int left = (int)min(rows - top, (int64_t)BM) - 4 * (lane >> 5);           // rows of this lane's that are there
+  float bg = 0.f, bu = 0.f;
+  if (MODE == FWD && p.b_gate && f0 + wn * 32 + (lane & 31) < p.F) {
+    bg = to_f(reinterpret_cast<const T *>(p.b_gate)[f0 + wn * 32 + (lane & 31)]);
+    bu = to_f(reinterpret_cast<const T *>(p.b_up)[f0 + wn * 32 + (lane & 31)]);
+  }
+  T *out = reinterpret_cast<T *>(MODE == FWD ? p.y : MODE == DX ? p.dx : which ? p.dw_up : p.dw_gate);
+  float *slab = MODE == DW ? a.slab + ((int64_t)ks * 2 + which) * rows * ld : nullptr;
+#pragma unroll
+  for (int j = 0; j < (MODE == FWD ? 1 : 2); ++j) {
+    const int64_t c0 = MODE == FWD ? f0 + wn * 32 : n0 + wn * 64 + j * 32;
+    const bool col = WHOLE || c0 + (lane & 31) < ld;
+    int64_t o = top * ld + c0;
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = i * 32 + 8 * (r / 4) + r % 4;
+        if (WHOLE || (col && row < left)) {
+          if constexpr (MODE == FWD) {
+            const float g = acc[i][0][r] + bg, u = acc[i][1][r] + bu;
+            (out + o)[at] = from_f<T>(act_f(p.act, g) * u);
+            if (p.pre) {
+              (p.pre + o)[at] = g;
+              (p.pre + p.M * ld + o)[at] = u;
+            }
+          } else if (MODE == DW && a.ksplit > 1) {
+            (slab + o)[at] = acc[i][j][r];
+          } else {
+            (out + o)[at] = from_f<T>(acc[i][j][r]);
+          }
+        }
+        o += r % 4 == 3 ? 5 * ld : ld;
+        asm volatile("" : "+s"(o));         // (64 precomputed row addresses would spill)
+      }
+  }
+}
+template <typename T, int MODE, int MT, int BM, int BN>
+__device__ __forceinline__ void store_tile(const Args &a, const v16f (&acc)[MT][2], int64_t m0, int64_t n0, int64_t f0, int wm, int wn, int which, int ks) {
+  const int64_t rows = MODE == DW ? a.p.F : a.p.M, cols = MODE == FWD ? a.p.F : a.p.D, c1 = MODE == FWD ? f0 + BN / 2 : n0 + BN;
+  if (m0 + BM <= rows && c1 <= cols) store_part<T, MODE, MT, BM, true>(a, acc, m0, n0, f0, wm, wn, which, ks);
+  else store_part<T, MODE, MT, BM, false>(a, acc, m0, n0, f0, wm, wn, which, ks);
+}
+
+template <int MT>
+__device__ __forceinline__ void clear(v16f (&acc)[MT][2]) {
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+}
+
+// 64 x 128 tiles for any alignment: slices of 128 bytes through registers into two LDS buffers, operands that lie across the contraction
+// transposed on the way.
+template <typename T, int MODE>
+__global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
+  constexpr int BM = 64, BN = 128, BK = 128 / sizeof(T);
   __shared__ __align__(16) char lds[2][(BM + BN) * 128];
   const fdql_gated_t &p = a.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
   int tm, tn;
   tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
-  const int64_t M = p.M, D = p.D, F = p.F, m0 = (int64_t)tm * BM;
+  const int64_t M = p.M, D = p.D, F = p.F, m0 = (int64_t)tm * BM, f0 = (int64_t)tn * (BN / 2), n0 = (int64_t)tn * BN;
   const int which = MODE == DW ? blockIdx.y : 0, ks = MODE == DW ? blockIdx.z : 0;
   const T *x = reinterpret_cast<const T *>(p.x), *wg = reinterpret_cast<const T *>(p.w_gate), *wu = reinterpret_cast<const T *>(p.w_up);
   const T *dd = reinterpret_cast<const T *>(a.d);
-  const int64_t f0 = (int64_t)tn * (BN / 2), n0 = (int64_t)tn * BN;
+  const int64_t kbeg = MODE == DW ? (int64_t)ks * a.kper : 0, kend = MODE == FWD ? D : MODE == DX ? F : min(M, kbeg + a.kper);
+  const int half = (int)((kend - kbeg + BK - 1) / BK), steps = MODE == DX ? 2 * half : half;     // DX: the gate's pass, then the up side's
 
-  int64_t kbeg = 0, kend;                          // contraction range in elements; DX runs over both halves one after the other
-  int steps;
-  if (MODE == FWD) kend = D, steps = (int)((D + BK - 1) / BK);
-  else if (MODE == DX) kend = F, steps = 2 * (int)((F + BK - 1) / BK);
-  else kbeg = (int64_t)ks * a.kper, kend = min(M, kbeg + a.kper), steps = kend > kbeg ? (int)((kend - kbeg + BK - 1) / BK) : 0;
-  const int half = steps / 2;
-
-  Flight<NCA> fa;
+  Flight<2> fa;
   Flight<4> fb;
   const auto fetch = [&](int step) {
     if constexpr (MODE == FWD) {
       const int64_t k0 = (int64_t)step * BK;
-      fetch_rows<T, VEC>(fa, [&](int n) { return m0 + n < M ? x + (m0 + n) * p.x_sr : (const T *)nullptr; }, k0, D);
-      fetch_rows<T, VEC>(fb, [&](int n) {          // 32 gate rows, 32 up rows per wave column
+      fetch_rows<T>(fa, [&](int n) { return m0 + n < M ? x + (m0 + n) * p.x_sr : (const T *)nullptr; }, k0, D);
+      fetch_rows<T>(fb, [&](int n) {               // 32 gate rows, 32 up rows per wave column
         const int64_t f = f0 + (n >> 6) * 32 + (n & 31);
         return f < F ? (n & 32 ? wu : wg) + f * D : (const T *)nullptr;
       }, k0, D);
@@ -217,91 +258,234 @@ __global__ __launch_bounds__(256, 2) void k_gated_tile(Args a) {
       const int up = step >= half;
       const int64_t k0 = (int64_t)(step - up * half) * BK;
       const T *src = dd + up * M * a.Fp;
-      fetch_rows<T, true>(fa, [&](int n) { return m0 + n < M ? src + (m0 + n) * a.Fp : (const T *)nullptr; }, k0, a.Fp);
-      fetch_cols<T, VEC>(fb, up ? wu : wg, D, k0, F, n0, D);
+      fetch_rows<T>(fa, [&](int n) { return m0 + n < M ? src + (m0 + n) * a.Fp : (const T *)nullptr; }, k0, F);
+      fetch_cols<T>(fb, up ? wu : wg, D, k0, F, n0, D);
     } else {
       const int64_t k0 = kbeg + (int64_t)step * BK;
-      fetch_cols<T, true>(reinterpret_cast<Flight<4> &>(fa), dd + which * M * a.Fp, a.Fp, k0, kend, m0, a.Fp);
-      fetch_cols<T, VEC>(fb, x, p.x_sr, k0, kend, n0, D);
+      fetch_cols<T>(fa, dd + which * M * a.Fp, a.Fp, k0, kend, m0, F);
+      fetch_cols<T>(fb, x, p.x_sr, k0, kend, n0, D);
     }
   };
   const auto put = [&](int buf) {
-    if constexpr (MODE == DW) put_cols(reinterpret_cast<const Flight<4> &>(fa), lds[buf]);
+    if constexpr (MODE == DW) put_cols(fa, lds[buf]);
     else put_rows(fa, lds[buf]);
     if constexpr (MODE == FWD) put_rows(fb, lds[buf] + BM * 128);
     else put_cols(fb, lds[buf] + BM * 128);
   };
-
-  v16f acc[MT][NT];
-#pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-
+  v16f acc[1][2];
+  clear(acc);
   if (steps > 0) {
     fetch(0);
     put(0);
   }
   __syncthreads();
   for (int step = 0; step < steps; ++step) {
-    const int buf = step & 1;
+    const int buf = step & 1, n = lane & 31;
     if (step + 1 < steps) fetch(step + 1);
-    const char *la = lds[buf] + (wm * (BM / 2) + (lane & 31)) * 128, *lb = lds[buf] + (BM + wn * 64 + (lane & 31)) * 128;
+    const char *la = lds[buf] + (wm * 32 + n) * 128, *lb = lds[buf] + (BM + wn * 64 + n) * 128;
 #pragma unroll
     for (int kk = 0; kk < 4; ++kk) {
       const int c = 2 * kk + (lane >> 5);
-      v4i ra[MT], rb[NT];
+      const v4i ra = *reinterpret_cast<const v4i *>(la + ((c ^ swz(wm * 32 + n)) << 4));
 #pragma unroll
-      for (int i = 0; i < MT; ++i) ra[i] = *reinterpret_cast<const v4i *>(la + i * 32 * 128 + ((c ^ swz(wm * (BM / 2) + i * 32 + (lane & 31))) << 4));
-#pragma unroll
-      for (int j = 0; j < NT; ++j) rb[j] = *reinterpret_cast<const v4i *>(lb + j * 32 * 128 + ((c ^ swz(wn * 64 + j * 32 + (lane & 31))) << 4));
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) Mma<T>::mma32(acc[i][j], ra[i], rb[j]);
+      for (int j = 0; j < 2; ++j) Mma<T>::mma32(acc[0][j], ra, *reinterpret_cast<const v4i *>(lb + j * 32 * 128 + ((c ^ swz(wn * 64 + j * 32 + n)) << 4)));
     }
     if (step + 1 < steps) put(buf ^ 1);
     __syncthreads();
   }
+  store_tile<T, MODE, 1, BM, BN>(a, acc, m0, n0, f0, wm, wn, which, ks);
+}
 
-  // register r of a 32 x 32 tile: row 8 (r / 4) + 4 (lane / 32) + r % 4, column lane % 32
-  const int64_t rows = MODE == DW ? F : M;
+// ---------------------------------------------------------------------------------------------------- rows of whole 16-byte chunks
+// BM x BN tiles, two waves along the rows and BN / 64 along the columns.  LDS holds a ring of NBUF slices of KS along the contraction, filled by
+// LDS-DMA (16 bytes per lane straight from memory, no registers in between): while one slice is multiplied the next ones are on their way, with
+// one counted wait and one barrier per slice; a wave's requests go out in pieces between its products.  An operand whose rows run along the
+// contraction lies in LDS as [row][slice] and is read 16 bytes at a time; one that runs across it lies as [k][column]: 16-bit types read it with
+// ds_read_b64_tr_b16, which hands every lane four consecutive k of its column, float one value at a time (v_mfma_f32_32x32x2 wants no more).
+// The DMA writes lanes in order, so the swizzles against bank conflicts are applied to the addresses that lanes read from memory.  Chunks past
+// an edge come from a block of zeros.
+// Shapes: 256 x 256 (KS 32, 4 slices) and 128 x 256 (KS 64, 3 slices) with one workgroup per CU for 16-bit types and many tiles; 64 x 128 for
+// few tiles and for float, whose matrix instructions take so long that the ring needs only two slices and three workgroups share a CU.
+__device__ const v4i g_zeros = {0, 0, 0, 0};
+
+template <typename T, int BM, int BN>
+struct Ring {
+  static constexpr int KS = sizeof(T) == 4 ? 32 : BM == 256 ? 32 : 64, NBUF = sizeof(T) == 4 ? 2 : BM == 256 ? 4 : 3;
+  static constexpr int ABYTES = BM * KS * (int)sizeof(T), BBYTES = BN * KS * (int)sizeof(T), BYTES = NBUF * (ABYTES + BBYTES);
+};
+
+template <int RB>     // [row][RB bytes]: row and chunk of LDS byte `o`; sixteen rows that are read together use sixteen different 16-byte places of 256
+struct RowTile {
+  static __device__ __forceinline__ int turn(int n) { return RB == 128 ? swz(n) : n >> 2 & 3; }
+  static __device__ __forceinline__ int row(int o) { return o / RB; }
+  static __device__ __forceinline__ int chunk(int o) { return (o / 16 % (RB / 16)) ^ turn(row(o)); }
+  static __device__ __forceinline__ int at(int n, int c) { return n * RB + ((c ^ turn(n)) << 4); }
+};
+template <typename T, int COLS>   // [k][COLS]: groups of 32 columns change places with k so that the rows one instruction reads lie in different banks
+struct ColTile {
+  static constexpr int RB = COLS * (int)sizeof(T), GC = 32 * (int)sizeof(T) / 16, GROUPS = COLS / 32;      // chunks of a group
+  static __device__ __forceinline__ int turn(int k) {
+    if (sizeof(T) == 4) return k >> 2 & 1;                             // lane halves read k and k + 4
+    return COLS == 64 ? k >> 1 & 1 : ((k & 3) | (k >> 1 & 4)) & (GROUPS - 1);      // four k, and four more eight further
+  }
+  static __device__ __forceinline__ int row(int o) { return o / RB; }
+  static __device__ __forceinline__ int chunk(int o) { return (o / 16 % (RB / 16)) ^ (turn(row(o)) * GC); }
+};
+__device__ __forceinline__ unsigned lds_addr(const char *p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char *)p; }
+// LDS-DMA of 16 bytes per lane, lane l to lds + 16 l.  Written out because the compiler, which knows the builtin, would wait for every DMA in
+// flight in front of each transposing read; nothing comes back into a register, the kernel counts its own waits, and nothing else in it uses M0.
+__device__ __forceinline__ void dma16(const void *src, unsigned lds) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory");
+}
+typedef short v4s __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ int2 tr_read(const char *p) {
+  return __builtin_bit_cast(int2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)p));
+}
+
+template <typename T, int MODE, int BM, int BN>
+__global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
+  typedef Ring<T, BM, BN> R;
+  constexpr int KS = R::KS, NBUF = R::NBUF, ABYTES = R::ABYTES, BBYTES = R::BBYTES, E = 16 / sizeof(T), RB = KS * sizeof(T), WAVES = BN / 32;
+  constexpr int MT = BM / 64, NT = 2, NA = ABYTES / (WAVES * 1024), NB = BBYTES / (WAVES * 1024), KSTEPS = RB / 32;
+  typedef RowTile<RB> Rows;
+  typedef ColTile<T, BM> ACols;
+  typedef ColTile<T, BN> BCols;
+  extern __shared__ __align__(16) char lds[];
+  const fdql_gated_t &p = a.p;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave / (WAVES / 2), wn = wave % (WAVES / 2);
+  int tm, tn;
+  tile_of(blockIdx.x, a.tiles_m, a.tiles_n, tm, tn);
+  const int64_t M = p.M, D = p.D, F = p.F, m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN, f0 = (int64_t)tn * (BN / 2);
+  const int which = MODE == DW ? blockIdx.y : 0, ks = MODE == DW ? blockIdx.z : 0;
+  const T *x = reinterpret_cast<const T *>(p.x), *wg = reinterpret_cast<const T *>(p.w_gate), *wu = reinterpret_cast<const T *>(p.w_up);
+  const T *dd = reinterpret_cast<const T *>(a.d) + which * M * a.Fp;
+  // contraction [kbeg, K) of one pass; DX makes two, gate and up
+  const int64_t kbeg = MODE == DW ? (int64_t)ks * a.kper : 0, K = MODE == FWD ? D : MODE == DX ? a.Fp : min(M, kbeg + a.kper);
+  const int half = (int)((K - kbeg + KS - 1) / KS), steps = MODE == DX ? 2 * half : half;
+
+  // where this lane's chunks come from: an element offset from the operand's start for slice 0, and the chunk's place in the contraction
+  int64_t oa[NA], ob[NB];
+  int ka[NA], kb[NB];
+  bool ina[NA], inb[NB];
 #pragma unroll
-  for (int i = 0; i < MT; ++i) {
-    if constexpr (MODE == FWD) {
-      const int64_t f = f0 + wn * 32 + (lane & 31);
-      const float bg = p.b_gate && f < F ? to_f(reinterpret_cast<const T *>(p.b_gate)[f]) : 0.f;
-      const float bu = p.b_up && f < F ? to_f(reinterpret_cast<const T *>(p.b_up)[f]) : 0.f;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int64_t m = m0 + wm * (BM / 2) + i * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-        if (m < M && f < F) {
-          const float g = acc[i][0][r] + bg, u = acc[i][1][r] + bu;
-          reinterpret_cast<T *>(p.y)[m * F + f] = from_f<T>(act_f(p.act, g) * u);
-          if (p.pre) {
-            p.pre[m * F + f] = g;
-            p.pre[(M + m) * F + f] = u;
-          }
-        }
-      }
+  for (int q = 0; q < NA; ++q) {
+    const int o = (wave * NA + q) * 1024 + lane * 16;
+    if (MODE == DW) {
+      ka[q] = ACols::row(o);
+      const int64_t c = m0 + ACols::chunk(o) * E;
+      ina[q] = c < a.Fp;
+      oa[q] = (int64_t)ka[q] * a.Fp + c;
     } else {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int64_t n = n0 + wn * 64 + j * 32 + (lane & 31);
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int64_t m = m0 + wm * (BM / 2) + i * 32 + 8 * (r / 4) + 4 * (lane >> 5) + r % 4;
-          if (m < rows && n < D) {
-            if (MODE == DX) reinterpret_cast<T *>(p.dx)[m * D + n] = from_f<T>(acc[i][j][r]);
-            else if (a.ksplit > 1) a.slab[(((int64_t)ks * 2 + which) * F + m) * D + n] = acc[i][j][r];
-            else reinterpret_cast<T *>(which ? p.dw_up : p.dw_gate)[m * D + n] = from_f<T>(acc[i][j][r]);
-          }
-        }
-      }
+      ka[q] = Rows::chunk(o) * E;
+      const int64_t r = m0 + Rows::row(o);
+      ina[q] = r < M;
+      oa[q] = r * (MODE == FWD ? p.x_sr : a.Fp) + ka[q];
     }
   }
+#pragma unroll
+  for (int q = 0; q < NB; ++q) {
+    const int o = (wave * NB + q) * 1024 + lane * 16;
+    if (MODE == FWD) {                              // LDS row n: 32 gate rows, then 32 up rows for every wave column
+      const int n = Rows::row(o);
+      kb[q] = Rows::chunk(o) * E;
+      const int64_t f = f0 + (n >> 6) * 32 + (n & 31);
+      inb[q] = f < F;
+      ob[q] = f * D + kb[q];
+    } else {
+      kb[q] = BCols::row(o);
+      const int64_t c = n0 + BCols::chunk(o) * E;
+      inb[q] = c < D;
+      ob[q] = (int64_t)kb[q] * (MODE == DX ? D : p.x_sr) + c;
+    }
+  }
+  // piece `piece` of `pieces` of a slice's DMA (a wave is held up while its requests are taken: in one go, with the other waves', that left the
+  // matrix unit idle for a quarter of a step)
+  const auto fetch = [&](int step, int buf, int piece, int pieces) {
+    const int up = MODE == DX && step >= half;
+    const int64_t k0 = kbeg + (int64_t)(step - up * half) * KS;
+    const unsigned la = lds_addr(lds) + buf * (ABYTES + BBYTES) + wave * NA * 1024, lb = lds_addr(lds) + buf * (ABYTES + BBYTES) + ABYTES + wave * NB * 1024;
+    const T *pa = MODE == FWD ? x + k0 : MODE == DX ? dd + up * M * a.Fp + k0 : dd + k0 * a.Fp;
+    const int64_t kx = k0 * (MODE == DX ? D : p.x_sr);
+#pragma unroll
+    for (int q = 0; q < NA + NB; ++q) {
+      if (q * pieces / (NA + NB) != piece) continue;
+      if (q < NA) {
+        const int i = q < NA ? q : 0;
+        dma16(ina[i] && k0 + ka[i] < K ? (const void *)(pa + oa[i]) : (const void *)&g_zeros, la + i * 1024);
+      } else {
+        const int i = q < NA ? 0 : q - NA;
+        const T *pb = MODE == FWD ? ((wave * NB + i) * (1024 / RB) & 32 ? wu : wg) + k0 : MODE == DX ? (up ? wu : wg) + kx : x + kx;
+        dma16(inb[i] && k0 + kb[i] < (MODE == DX ? F : K) ? (const void *)(pb + ob[i]) : (const void *)&g_zeros, lb + i * 1024);
+      }
+    }
+  };
+
+  // where this lane reads its fragments: [row][slice] tiles at row lane % 32, chunk 2 kk + lane / 32; [k][column] tiles at the k and columns
+  // that the transposing read collects from it, or that it multiplies itself
+  const int tr_k = (lane >> 5) * (sizeof(T) == 4 ? 4 : 8) + (sizeof(T) == 4 ? 0 : lane >> 2 & 3);
+  const int tr_c = sizeof(T) == 4 ? lane & 31 : (lane >> 4 & 1) * 16 + (lane & 3) * 4;
+  int at_a[MT], at_b[NT];                           // byte offsets of the wave's 32-row / 32-column blocks, kk = 0
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+    at_a[i] = MODE == DW ? tr_k * ACols::RB + ((wm * MT + i) ^ ACols::turn(tr_k)) * (32 * (int)sizeof(T)) + tr_c * (int)sizeof(T) : 0;
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+    at_b[j] = MODE != FWD ? tr_k * BCols::RB + ((wn * 2 + j) ^ BCols::turn(tr_k)) * (32 * (int)sizeof(T)) + tr_c * (int)sizeof(T) : 0;
+  const auto row_frag = [&](const char *t, int r0, int kk) { return *reinterpret_cast<const v4i *>(t + Rows::at(r0 + (lane & 31), 2 * kk + (lane >> 5))); };
+  const auto col_frag = [&](const char *t, int kk, int rb) {
+    if constexpr (sizeof(T) == 4) {
+      v4i v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const int *>(t + (kk * 8 + e) * rb);
+      return v;
+    } else {
+      const int2 lo = tr_read(t + kk * 16 * rb), hi = tr_read(t + (kk * 16 + 4) * rb);
+      return v4i{lo.x, lo.y, hi.x, hi.y};
+    }
+  };
+
+  v16f acc[MT][NT];
+  clear(acc);
+  // (s_barrier by itself: __syncthreads would wait for every DMA in flight.  A wave's LDS reads are done when it arrives: their products are issued)
+  int issued = 0;
+  for (; issued < min(NBUF - 1, steps); ++issued) fetch(issued, issued, 0, 1);
+  if (issued == NBUF - 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((NBUF - 2) * (NA + NB)) : "memory");
+  else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  int buf = 0;
+  for (int step = 0; step < steps; ++step) {
+    const bool more = step + NBUF - 1 < steps;
+    const char *ta = lds + buf * (ABYTES + BBYTES), *tb = ta + ABYTES;
+    // the next fragments are on their way while these are multiplied
+    v4i ra[2][MT], rb[2][NT];
+    const auto frags = [&](int kk) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if constexpr (MODE == FWD) rb[kk & 1][j] = row_frag(tb, wn * 64 + j * 32, kk);
+        else rb[kk & 1][j] = col_frag(tb + at_b[j], kk, BCols::RB);
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        if constexpr (MODE == DW) ra[kk & 1][i] = col_frag(ta + at_a[i], kk, ACols::RB);
+        else ra[kk & 1][i] = row_frag(ta, wm * (BM / 2) + i * 32, kk);
+      }
+    };
+    frags(0);
+#pragma unroll
+    for (int kk = 0; kk < KSTEPS; ++kk) {
+      if (kk + 1 < KSTEPS) frags(kk + 1);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) Mma<T>::mma32(acc[i][j], ra[kk & 1][i], rb[kk & 1][j]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (more) fetch(step + NBUF - 1, buf ? buf - 1 : NBUF - 1, kk, KSTEPS);   // into the slice that the last step was done with
+    }
+    if (more) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((NBUF - 2) * (NA + NB)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+    buf = buf == NBUF - 1 ? 0 : buf + 1;
+  }
+  store_tile<T, MODE, MT, BM, BN>(a, acc, m0, n0, f0, wm, wn, which, ks);
 }
 
 // M <= 32 rows: 16 outputs per workgroup, K split over its four waves.  MFMA 16x16: the outputs are the A side, the rows the B side, so
@@ -412,36 +596,95 @@ __global__ __launch_bounds__(256) void k_gated_grad(Args a) {
   a.colsum[((int64_t)blockIdx.y * 2 + 1) * F + f] = su;
 }
 
-// out[i] = sum over n parts, `stride` floats apart; blockIdx.y picks the gate's or the up side's.
+// Weight gradients from the row slices' slabs (blockIdx.z 0) and bias gradients from the row blocks' column sums (1), both sides (blockIdx.y):
+// 64 neighbouring values per workgroup, the parts dealt to its four waves.
 template <typename T>
-__global__ __launch_bounds__(256) void k_gated_sum(const float *part, int64_t n, int64_t stride, int64_t count, void *gate, void *up) {
-  T *out = reinterpret_cast<T *>(blockIdx.y ? up : gate);
-  if (!out) return;
-  const float *src = part + blockIdx.y * count;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+__global__ __launch_bounds__(256) void k_gated_sum(Args a, int64_t rblocks) {
+  __shared__ float red[3][64];
+  const bool bias = blockIdx.z;
+  const int64_t count = bias ? a.p.F : (int64_t)a.p.F * a.p.D, n = bias ? rblocks : a.ksplit;
+  T *out = reinterpret_cast<T *>(bias ? (blockIdx.y ? a.p.db_up : a.p.db_gate) : (blockIdx.y ? a.p.dw_up : a.p.dw_gate));
+  if (!out || (!bias && a.ksplit == 1)) return;
+  const float *src = (bias ? a.colsum : a.slab) + blockIdx.y * count;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  for (int64_t i0 = (int64_t)blockIdx.x * 64; i0 < count; i0 += (int64_t)gridDim.x * 64) {
+    const int64_t i = min(i0 + lane, count - 1);
     float v = 0.f;
-    for (int64_t k = 0; k < n; ++k) v += src[k * stride + i];
-    out[i] = from_f<T>(v);
+#pragma unroll 8
+    for (int64_t k = wave; k < n; k += 4) v += src[k * 2 * count + i];
+    if (wave) red[wave - 1][lane] = v;
+    __syncthreads();
+    if (wave == 0 && i0 + lane < count) out[i] = from_f<T>(v + red[0][lane] + red[1][lane] + red[2][lane]);
+    __syncthreads();
   }
 }
 
+// Tile shape of a product: rows x columns of tiles, and for the weight gradients the slices of the rows that fill the card.
+struct Shape {
+  int bm, bn;
+  int64_t tiles_m, tiles_n;
+};
+constexpr int CUS = 256;
+Shape shape_of(bool wide, int64_t rows, int64_t cols, int tile_of_256, int copies) {     // tile_of_256: columns that a 256-wide tile covers
+  const auto tiles = [&](int bm, int bn) { return (rows + bm - 1) / bm * ((cols + tile_of_256 * bn / 256 - 1) / (tile_of_256 * bn / 256)); };
+  Shape s = {64, 128, 0, 0};
+  if (wide && tiles(128, 256) * copies >= 192) {
+    // one workgroup per CU: the tile that needs fewer row-steps of the card, the larger one where they need the same
+    s.bn = 256;
+    s.bm = (tiles(256, 256) * copies + CUS - 1) / CUS * 2 <= (tiles(128, 256) * copies + CUS - 1) / CUS ? 256 : 128;
+  }
+  s.tiles_m = (rows + s.bm - 1) / s.bm;
+  s.tiles_n = (cols + tile_of_256 * s.bn / 256 - 1) / (tile_of_256 * s.bn / 256);
+  return s;
+}
+
 struct Plan {
-  int Fp, bk, ksplit, kper;
+  int Fp, ksplit, kper;
   int64_t rblocks;
 };
 Plan plan_of(const fdql_gated_t &p) {
   Plan q;
   q.Fp = (p.F + 7) / 8 * 8;
-  q.bk = p.dtype == FDQL_F32 ? 32 : 64;
   q.rblocks = (p.M + RB - 1) / RB;
-  const int64_t tiles = 2ll * ((p.F + 127) / 128) * ((p.D + BN - 1) / BN), slices = std::max<int64_t>(1, (p.M + q.bk - 1) / q.bk);
-  int64_t ks = std::max<int64_t>(1, std::min<int64_t>(512 / tiles, slices / 8));
-  q.kper = (int)((slices + ks - 1) / ks * q.bk);
+  // rows split for the 64 x 128 tiles of the weight gradients (larger tiles are chosen where there are enough of them): three workgroups
+  // per CU, at least 256 rows each
+  const int64_t tiles = 2ll * ((p.F + 63) / 64) * ((p.D + 127) / 128);
+  const int64_t ks = std::max<int64_t>(1, std::min<int64_t>(3 * CUS / tiles, p.M / 256));
+  q.kper = (int)(((p.M + ks - 1) / ks + 63) / 64 * 64);
+  q.kper = std::max(q.kper, 64);
   q.ksplit = (int)std::max<int64_t>(1, (p.M + q.kper - 1) / q.kper);
   return q;
 }
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 bool al16(const void *q) { return ((uintptr_t)q & 15) == 0; }
+
+template <typename T, int MODE, int BM, int BN>
+hipError_t launch_mma(const Args &a, dim3 grid, hipStream_t s) {
+  constexpr int bytes = Ring<T, BM, BN>::BYTES;
+  const hipError_t e = hipFuncSetAttribute((const void *)k_gated_mma<T, MODE, BM, BN>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((k_gated_mma<T, MODE, BM, BN>), grid, dim3(BN * 2), bytes, s, a);
+  return hipGetLastError();
+}
+// rows x cols of the product's result; aligned: every operand row is made of whole 16-byte chunks
+template <typename T, int MODE>
+hipError_t product(Args a, int64_t rows, int64_t cols, bool aligned, hipStream_t s) {
+  const int copies = MODE == DW ? 2 : 1;
+  const Shape q = shape_of(sizeof(T) == 2 && aligned, rows, cols, MODE == FWD ? 128 : 256, copies);
+  a.tiles_m = (int)q.tiles_m;
+  a.tiles_n = (int)q.tiles_n;
+  if (MODE == DW && q.bn == 256) a.ksplit = 1, a.kper = (int)((a.p.M + 63) / 64 * 64);
+  const dim3 grid((unsigned)(q.tiles_m * q.tiles_n), copies, MODE == DW ? (unsigned)a.ksplit : 1);
+  if (!aligned) {
+    hipLaunchKernelGGL((k_gated_any<T, MODE>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (q.bm == 256) return launch_mma<T, MODE, 256, 256>(a, grid, s);
+    if (q.bm == 128) return launch_mma<T, MODE, 128, 256>(a, grid, s);
+  }
+  return launch_mma<T, MODE, 64, 128>(a, grid, s);
+}
 
 template <typename T>
 hipError_t fwd(const fdql_gated_t &p, hipStream_t s) {
@@ -449,28 +692,16 @@ hipError_t fwd(const fdql_gated_t &p, hipStream_t s) {
   a.p = p;
   constexpr int E = 16 / sizeof(T);
   const bool vec = p.D % E == 0 && p.x_sr % E == 0 && al16(p.x) && al16(p.w_gate) && al16(p.w_up);
-  if (p.M <= 32) {
-    const dim3 grid((unsigned)((p.F + 15) / 16));
-    if (vec) hipLaunchKernelGGL((k_gated_rows<T, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_gated_rows<T, false>), grid, dim3(256), 0, s, a);
-    return hipGetLastError();
-  }
-  a.tiles_n = (p.F + BN / 2 - 1) / (BN / 2);
-  const bool small = (p.M + 127) / 128 * a.tiles_n < 512;
-  a.tiles_m = (int)(small ? (p.M + 63) / 64 : (p.M + 127) / 128);
-  const dim3 grid((unsigned)(a.tiles_m * a.tiles_n));
-  if (small) {
-    if (vec) hipLaunchKernelGGL((k_gated_tile<T, FWD, 64, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_gated_tile<T, FWD, 64, false>), grid, dim3(256), 0, s, a);
-  } else {
-    if (vec) hipLaunchKernelGGL((k_gated_tile<T, FWD, 128, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_gated_tile<T, FWD, 128, false>), grid, dim3(256), 0, s, a);
-  }
+  if (p.M > 32) return product<T, FWD>(a, p.M, p.F, vec, s);
+  const dim3 grid((unsigned)((p.F + 15) / 16));
+  if (vec) hipLaunchKernelGGL((k_gated_rows<T, true>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((k_gated_rows<T, false>), grid, dim3(256), 0, s, a);
   return hipGetLastError();
 }
 
 template <typename T>
 hipError_t bwd(const fdql_gated_t &p, hipStream_t s) {
+  constexpr int E = 16 / sizeof(T);
   const Plan q = plan_of(p);
   Args a = {};
   a.p = p;
@@ -484,37 +715,18 @@ hipError_t bwd(const fdql_gated_t &p, hipStream_t s) {
   a.ksplit = q.ksplit;
   a.kper = q.kper;
   hipLaunchKernelGGL((k_gated_grad<T>), dim3((unsigned)((q.Fp + 63) / 64), (unsigned)q.rblocks), dim3(256), 0, s, a);
-  // a column group of 4 must not straddle a row's end and must lie on its own size in memory
-  const auto ok = [](const void *v) { return ((uintptr_t)v & (4 * sizeof(T) - 1)) == 0; };
-  a.tiles_n = (p.D + BN - 1) / BN;
-  if (p.dx) {
-    const bool vec = p.D % 4 == 0 && ok(p.w_gate) && ok(p.w_up);
-    const bool small = (p.M + 127) / 128 * a.tiles_n < 512;
-    a.tiles_m = (int)(small ? (p.M + 63) / 64 : (p.M + 127) / 128);
-    const dim3 grid((unsigned)(a.tiles_m * a.tiles_n));
-    if (small) {
-      if (vec) hipLaunchKernelGGL((k_gated_tile<T, DX, 64, true>), grid, dim3(256), 0, s, a);
-      else hipLaunchKernelGGL((k_gated_tile<T, DX, 64, false>), grid, dim3(256), 0, s, a);
-    } else {
-      if (vec) hipLaunchKernelGGL((k_gated_tile<T, DX, 128, true>), grid, dim3(256), 0, s, a);
-      else hipLaunchKernelGGL((k_gated_tile<T, DX, 128, false>), grid, dim3(256), 0, s, a);
-    }
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess && p.dx) e = product<T, DX>(a, p.M, p.D, p.D % E == 0 && al16(p.w_gate) && al16(p.w_up), s);
+  const bool w = p.dw_gate && p.dw_up, vec = p.D % E == 0 && p.x_sr % E == 0 && al16(p.x);
+  if (w && shape_of(sizeof(T) == 2 && vec, p.F, p.D, 256, 2).bn == 256) a.ksplit = 1;
+  if (e == hipSuccess && w) e = product<T, DW>(a, p.F, p.D, vec, s);
+  const bool sum_w = w && a.ksplit > 1;
+  if (e == hipSuccess && (sum_w || p.db_gate || p.db_up)) {
+    const int64_t n = sum_w ? (int64_t)p.F * p.D : p.F;
+    hipLaunchKernelGGL((k_gated_sum<T>), dim3((unsigned)std::min<int64_t>((n + 63) / 64, 4096), 2, 2), dim3(256), 0, s, a, q.rblocks);
+    e = hipGetLastError();
   }
-  if (p.dw_gate && p.dw_up) {
-    const bool vec = p.D % 4 == 0 && p.x_sr % 4 == 0 && ok(p.x);
-    a.tiles_m = (p.F + 127) / 128;
-    const dim3 grid((unsigned)(a.tiles_m * a.tiles_n), 2, (unsigned)q.ksplit);
-    if (vec) hipLaunchKernelGGL((k_gated_tile<T, DW, 128, true>), grid, dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((k_gated_tile<T, DW, 128, false>), grid, dim3(256), 0, s, a);
-    if (q.ksplit > 1) {
-      const int64_t n = (int64_t)p.F * p.D;
-      hipLaunchKernelGGL((k_gated_sum<T>), dim3((unsigned)std::min<int64_t>((n + 255) / 256, 4096), 2), dim3(256), 0, s, a.slab, (int64_t)q.ksplit, 2 * n, n,
-                         p.dw_gate, p.dw_up);
-    }
-  }
-  if (p.db_gate || p.db_up)
-    hipLaunchKernelGGL((k_gated_sum<T>), dim3((unsigned)((p.F + 255) / 256), 2), dim3(256), 0, s, a.colsum, q.rblocks, 2ll * p.F, (int64_t)p.F, p.db_gate, p.db_up);
-  return hipGetLastError();
+  return e;
 }
 
 }  // namespace

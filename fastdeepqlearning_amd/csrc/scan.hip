@@ -14,18 +14,23 @@
 // them in order, and the main kernel runs every segment from its true start.  Backward does the same from the right.
 //
 // Backward.  The forward pass keeps the state in front of every TS steps (checkpoints, N floats per channel and tile).  The
-// backward kernel rebuilds a tile's states from it, four states at a time (decays and states of TS steps then stay in registers), and
-// walks the tile in reverse with g_t = carry + C_t dy_t, carry <- e^(delta A) g_t.  dB and dC sum over channels: 8 values per step and
-// part go through a butterfly over the wave that halves the values at each step (permlane swaps, then DPP), then over the
-// workgroup's waves in LDS, then over workgroups in a slab that k_scan_bc_finish adds up.  No atomics: results repeat bit by bit.
+// backward kernel rebuilds a tile's states from it, two states of a lane at a time (decays and states of TS steps then stay in registers), and
+// walks the tile in reverse with g_t = carry + C_t dy_t, carry <- e^(delta A) g_t.  dB and dC sum over channels, 4 values per step, lane and
+// pass: permlane swaps halve the values while they add (v_permlane32_swap exchanges half of one register's lanes with half of another's),
+// two DPP rotations finish - a channel's parts are neighbouring lanes so that these steps need no selects; then the workgroup's waves meet in
+// LDS, the workgroups in a slab that k_scan_bc_finish adds up.  No atomics: results repeat bit by bit.  (One-hot v_mfma_f32_16x16x4 products
+// for these sums measured slower, 190 us against 126 at 50 x 256 x 512 x 16: float32 matrix instructions and vector arithmetic do not overlap.)
 #include "seq.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fdql {
 namespace {
 
 constexpr int TS = 8;             // steps per tile
+constexpr int S = 4, CW = 64 / S; // lanes that share a channel, channels of a wave
+constexpr int OWN = TS / S;       // steps of a tile whose state-independent work a lane does
 constexpr int WPB = 4;            // waves per workgroup
 
 struct Args {
@@ -57,164 +62,245 @@ __device__ __forceinline__ void wave_lds_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// x + the same lane's value in the other states' lanes (S lanes CW apart hold parts of one channel's sum)
-template <int S>
-__device__ __forceinline__ float sum_parts(float v) {
-  if constexpr (S >= 4) v += __shfl_xor(v, 16);
-  if constexpr (S >= 2) v += __shfl_xor(v, 32);
-  return v;
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+// Nothing is read or computed ahead across this point: unrolled code would otherwise fetch every tile row into registers first, and spill.
+__device__ __forceinline__ void pass_edge() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
 }
 
+// The value is computed by here (an accumulation put off to the end would keep every one of its terms in a register).
+__device__ __forceinline__ void settle(float &v) { asm volatile("" : "+v"(v)); }
+
+// A lane's view of a [T, R, D] tensor: one channel of one row from its part's step on (part s of a tile does the steps S q + s).
 template <typename T>
-struct Col {                      // one lane's column of a [T, R, D] tensor
-  const T *base;
+struct Col {
+  const T *at0;
   int64_t st;
-  __device__ __forceinline__ float at(int t) const { return to_f(base[t * st]); }
+  __device__ __forceinline__ T at(int t, int q) const { return at0[(int64_t)(t + q * S) * st]; }   // (scalar but for the last addition)
 };
 template <typename T>
-__device__ __forceinline__ Col<T> column(const void *p, int64_t st, int64_t sr, int r, int d) {
-  return {reinterpret_cast<const T *>(p) + (int64_t)r * sr + d, st};
+__device__ __forceinline__ Col<T> col_of(const void *p, int64_t st, int64_t sr, int r, int s, int d) {
+  return {reinterpret_cast<const T *>(p) + (int64_t)r * sr + s * st + d, st};
 }
 
-// bit i: a reset at step t + i (i < nt)
-__device__ __forceinline__ unsigned reset_bits(const fdql_scan_t &p, int r, int t, int nt, int lane) {
-  if (!p.reset) return 0u;
-  const bool on = lane < nt && p.reset[(int64_t)(t + lane) * p.reset_st + (int64_t)r * p.reset_sr] != 0;
-  return (unsigned)__ballot(on);
-}
-
-// The tile's B or C rows, widened to float and padded with zeros to NP states, spread over `nthreads` threads.
-template <typename T, int NP>
-__device__ __forceinline__ void stage_rows(const void *src, int64_t st, int64_t sr, int64_t sg, const fdql_scan_t &p, int r, int g, int t, int nt,
-                                           float *dst, int tid, int nthreads) {
-  const T *b = reinterpret_cast<const T *>(src) + (int64_t)r * sr + (int64_t)g * sg;
-  for (int i = tid; i < TS * NP; i += nthreads) {
-    const int k = i / NP, n = i % NP;
-    dst[i] = (k < nt && n < p.N) ? to_f(b[(int64_t)(t + k) * st + n]) : 0.f;
-  }
-}
-
-template <int NL, int S>
+template <int NL>
 __device__ __forceinline__ int64_t lane_slot(const Args &a, int64_t block, const Unit &w) {   // first float of a wave's [NL][64] block
   return (((block * a.p.R + w.r) * a.p.G + w.g) * a.tpg + w.tile) * (NL * 64);
 }
 
+// A tile's B or C rows on their way to LDS, one wave's work: element lane + 64 q is (step, state) = (/ NP, % NP), zeros behind state N.
+template <typename T, int NP>
+struct Rows {
+  static constexpr int Q = TS * NP / 64, KQ = 64 / NP;     // elements per lane, steps that 64 of them span
+  static_assert(64 % NP == 0, "a row must not straddle the lanes");
+  const T *base;
+  int64_t st;
+  int k;
+  bool on;
+  T v[Q];
+  __device__ __forceinline__ Rows(const void *p, int64_t st_, int64_t sr, int64_t sg, const Unit &w, int N, int lane)
+      : base(reinterpret_cast<const T *>(p) + (int64_t)w.r * sr + (int64_t)w.g * sg + (lane / NP) * st_ + min(lane % NP, N - 1)), st(st_), k(lane / NP),
+        on(lane % NP < N) {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) v[q] = T(0.f);
+  }
+  __device__ __forceinline__ void load(int t, int t1) {
+#pragma unroll
+    for (int q = 0; q < Q; ++q)
+      if (on && t + q * KQ + k < t1) v[q] = base[(int64_t)(t + q * KQ) * st];
+  }
+  __device__ __forceinline__ void put(float *dst, int lane) const {
+#pragma unroll
+    for (int q = 0; q < Q; ++q) dst[lane + 64 * q] = to_f(v[q]);
+  }
+};
+
+// lanes with BIT clear end with the sum (over lanes BIT apart) of a, the others with that of b: v_permlane32_swap / v_permlane16_swap
+// exchange half of one register's lanes with half of another's; inside a quad the same takes two selects and a DPP add.
+__device__ __forceinline__ float dpp_xor2(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4e, 0xf, 0xf, true)); }
+__device__ __forceinline__ float dpp_xor1(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xb1, 0xf, 0xf, true)); }
+template <int N>
+__device__ __forceinline__ float dpp_ror(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, true)); }
+template <int BIT>
+__device__ __forceinline__ float fold(float a, float b, int lane) {
+  if constexpr (BIT == 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  } else if constexpr (BIT == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  } else {
+    const bool up = lane & BIT;
+    const float keep = up ? b : a, give = up ? a : b;
+    return keep + (BIT == 2 ? dpp_xor2(give) : dpp_xor1(give));
+  }
+}
+// One value per step of a tile, in parts over the S lanes of a channel: lane part s ends with the sums of its own steps S q + s.
+__device__ __forceinline__ void own_sums(const float v[TS], float out[OWN], int lane) {
+#pragma unroll
+  for (int q = 0; q < OWN; ++q) out[q] = fold<1>(fold<2>(v[4 * q], v[4 * q + 2], lane), fold<2>(v[4 * q + 1], v[4 * q + 3], lane), lane);
+}
+
 // ---------------------------------------------------------------------------------------------------------------- forward
-template <typename T, int NL, int S>
+// CARRY: a segment's state at its end from a zero start and the sum of its steps, for segments [0, nseg - 1); no outputs.
+// The S lanes of a channel share the work of a step that does not depend on the state (loads, softplus, gate, store): part s takes the
+// steps S q + s of a tile and hands delta and delta x to the others through LDS.
+template <typename T, int NL, bool CARRY>
 __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
-  constexpr int CW = 64 / S, NP = NL * S;
-  __shared__ float lds[WPB][2][TS * NP];
+  constexpr int NP = NL * S, VW = NL < 4 ? NL : 4;         // VW: states read from LDS at once
+  typedef float vec __attribute__((ext_vector_type(VW)));
+  __shared__ __align__(16) float lds[WPB][CARRY ? 1 : 2][TS * NP];
+  __shared__ __align__(8) float2 lds_d[WPB][TS][CW];
   const fdql_scan_t &p = a.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int u = blockIdx.x * WPB + wave;
-  if (u >= a.nseg * p.R * p.G * a.tpg) return;
+  if (u >= (a.nseg - CARRY) * p.R * p.G * a.tpg) return;
   const Unit w = unit_of(a, u);
-  const int c = lane % CW, s = lane / CW;
+  const int c = lane / S, s = lane % S;
   const int dc = w.tile * CW + c, d = w.g * a.Dg + min(dc, a.Dg - 1);
   const bool live = dc < a.Dg;
   const int t0 = w.seg * a.seglen, t1 = min(p.T, t0 + a.seglen);
-  float *lB = lds[wave][0], *lC = lds[wave][1];
+  float *lB = lds[wave][0], *lC = lds[wave][CARRY ? 0 : 1];
 
-  const Col<T> X = column<T>(p.x, p.x_st, p.x_sr, w.r, d), DT = column<T>(p.dt, p.dt_st, p.dt_sr, w.r, d),
-               Z = column<T>(p.z ? p.z : p.x, p.z ? p.z_st : p.x_st, p.z ? p.z_sr : p.x_sr, w.r, d);
+  const Col<T> X = col_of<T>(p.x, p.x_st, p.x_sr, w.r, s, d), DT = col_of<T>(p.dt, p.dt_st, p.dt_sr, w.r, s, d),
+               Z = col_of<T>(p.z ? p.z : p.x, p.z ? p.z_st : p.x_st, p.z ? p.z_sr : p.x_sr, w.r, s, d);
   const float bias = p.dt_bias ? p.dt_bias[d] : 0.f, skip = p.skip ? p.skip[d] : 0.f;
-  float h[NL], A[NL];
+  float h[NL], A[NL], sum = 0.f;
+  int any = 0;
 #pragma unroll
   for (int j = 0; j < NL; ++j) {
     const int n = s * NL + j;
     A[j] = n < p.N ? p.A[(int64_t)d * p.N + n] * LOG2E : 0.f;
-    if (a.nseg > 1) h[j] = a.seg_h[lane_slot<NL, S>(a, w.seg, w) + j * 64 + lane];
+    if (CARRY) h[j] = 0.f;
+    else if (a.nseg > 1) h[j] = a.seg_h[lane_slot<NL>(a, w.seg, w) + j * 64 + lane];
     else h[j] = p.state_in && n < p.N ? p.state_in[(int64_t)w.r * p.state_in_sr + (int64_t)d * p.N + n] : 0.f;
   }
-  T *yp = reinterpret_cast<T *>(p.y) + (int64_t)w.r * p.D + d;
   const int64_t y_st = (int64_t)p.R * p.D;
+  T *yp = reinterpret_cast<T *>(p.y) + (int64_t)w.r * p.D + s * y_st + d;
 
-  float xn[TS], dn[TS], zn[TS];
+  // the next tile, in flight while this one is computed
+  T xn[OWN] = {}, dn[OWN] = {}, zn[OWN] = {};
+  Rows<T, NP> Bn(p.B, p.B_st, p.B_sr, p.B_sg, w, p.N, lane), Cn(p.C, p.C_st, p.C_sr, p.C_sg, w, p.N, lane);
+  uint8_t rn = 0;
+  const uint8_t *rp = p.reset ? p.reset + (int64_t)w.r * p.reset_sr + (lane % TS) * p.reset_st : nullptr;
+  const auto fetch = [&](int t) {
 #pragma unroll
-  for (int i = 0; i < TS; ++i) {
-    const int t = min(t0 + i, t1 - 1);
-    xn[i] = X.at(t); dn[i] = DT.at(t); zn[i] = Z.at(t);
-  }
+    for (int q = 0; q < OWN; ++q) {
+      if (t + q * S + s < t1) {
+        xn[q] = X.at(t, q);
+        dn[q] = DT.at(t, q);
+        if (!CARRY) zn[q] = Z.at(t, q);
+      }
+    }
+    Bn.load(t, t1);
+    if (!CARRY) Cn.load(t, t1);
+    if (rp && t + lane % TS < t1) rn = rp[t * p.reset_st];
+  };
+  fetch(t0);
   for (int t = t0; t < t1; t += TS) {
     const int nt = min(TS, t1 - t);
-    stage_rows<T, NP>(p.B, p.B_st, p.B_sr, p.B_sg, p, w.r, w.g, t, nt, lB, lane, 64);
-    stage_rows<T, NP>(p.C, p.C_st, p.C_sr, p.C_sg, p, w.r, w.g, t, nt, lC, lane, 64);
-    const unsigned rst = reset_bits(p, w.r, t, nt, lane);
-    if (p.checkpoints) {
-      float *ck = p.checkpoints + lane_slot<NL, S>(a, t / TS, w) + lane;
+    const unsigned rst = (unsigned)__ballot(lane < nt && rn != 0);
+    any |= rst != 0;
+    Bn.put(lB, lane);
+    if (!CARRY) Cn.put(lC, lane);
+    float x[OWN], del[OWN], z[OWN];
+#pragma unroll
+    for (int q = 0; q < OWN; ++q) {
+      x[q] = to_f(xn[q]);
+      del[q] = to_f(dn[q]) + bias;
+      if (!CARRY) z[q] = to_f(zn[q]);
+    }
+    if (t + TS < t1) fetch(t + TS);
+    if (!CARRY && p.checkpoints) {
+      float *ck = p.checkpoints + lane_slot<NL>(a, t / TS, w) + lane;
 #pragma unroll
       for (int j = 0; j < NL; ++j) ck[j * 64] = h[j];
     }
-    float x[TS], del[TS], z[TS];
 #pragma unroll
-    for (int i = 0; i < TS; ++i) {
-      x[i] = xn[i];
-      z[i] = zn[i];
-      del[i] = dn[i] + bias;
-    }
-    if (t + TS < t1) {
-#pragma unroll
-      for (int i = 0; i < TS; ++i) {
-        const int tn = min(t + TS + i, t1 - 1);
-        xn[i] = X.at(tn); dn[i] = DT.at(tn); zn[i] = Z.at(tn);
-      }
-    }
-    if (p.dt_softplus) {
-#pragma unroll
-      for (int i = 0; i < TS; ++i) del[i] = softplus_f(del[i]);
+    for (int q = 0; q < OWN; ++q) {
+      if (p.dt_softplus) del[q] = softplus_f(del[q]);
+      lds_d[wave][q * S + s][c] = make_float2(del[q], del[q] * x[q]);
     }
     wave_lds_fence();
+    float acc[TS];
+    const auto tile = [&](auto whole) {              // whole: eight steps without a reset
 #pragma unroll
-    for (int i = 0; i < TS; ++i) {
-      if (i < nt) {
-        if (rst >> i & 1) {
+      for (int i = 0; i < TS; ++i) {
+        if (i % 2 == 0) pass_edge();
+        acc[i] = 0.f;
+        if (decltype(whole)::value || i < nt) {
+          const float2 v = lds_d[wave][i][c];
+          const float dl = v.x, dx = v.y;
+          if (CARRY) sum += dl;
+          if (!decltype(whole)::value && (rst >> i & 1)) {
 #pragma unroll
-          for (int j = 0; j < NL; ++j) h[j] = 0.f;
+            for (int j = 0; j < NL; ++j) h[j] = 0.f;
+          }
+#pragma unroll
+          for (int j4 = 0; j4 < NL; j4 += VW) {
+            const vec B = *reinterpret_cast<const vec *>(lB + i * NP + s * NL + j4);
+            vec C = {};
+            if (!CARRY) C = *reinterpret_cast<const vec *>(lC + i * NP + s * NL + j4);
+#pragma unroll
+            for (int j = 0; j < VW; ++j) {
+              h[j4 + j] = fmaf(__builtin_amdgcn_exp2f(dl * A[j4 + j]), h[j4 + j], dx * B[j]);
+              if (!CARRY) acc[i] = fmaf(h[j4 + j], C[j], acc[i]);
+            }
+          }
+          if (!CARRY) settle(acc[i]);
         }
-        const float dx = del[i] * x[i];
-        float acc = 0.f;
+      }
+    };
+    if (rst == 0 && nt == TS) tile(std::true_type());
+    else tile(std::false_type());
+    if (!CARRY) {
+      float own[OWN];
+      own_sums(acc, own, lane);
 #pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          const float e = __builtin_amdgcn_exp2f(del[i] * A[j]);
-          h[j] = fmaf(e, h[j], dx * lB[i * NP + s * NL + j]);
-          acc = fmaf(h[j], lC[i * NP + s * NL + j], acc);
-        }
-        acc = sum_parts<S>(acc);
-        float y = fmaf(skip, x[i], acc);
-        if (p.z) y *= z[i] * sigmoid_f(z[i]);
-        if (live && s == 0) yp[(int64_t)(t + i) * y_st] = from_f<T>(y);
+      for (int q = 0; q < OWN; ++q) {
+        const int i = q * S + s;
+        float y = fmaf(skip, x[q], own[q]);
+        if (p.z) y *= z[q] * sigmoid_f(z[q]);
+        if (live && i < nt) yp[(int64_t)(t + q * S) * y_st] = from_f<T>(y);
       }
     }
     wave_lds_fence();
   }
-  if (p.state_out && t1 == p.T && live) {
+  if (CARRY) {
+    const int64_t o = lane_slot<NL>(a, w.seg, w);
+#pragma unroll
+    for (int j = 0; j < NL; ++j) a.seg_h[o + j * 64 + lane] = live ? h[j] : 0.f;
+    a.seg_d[o / NL + lane] = sum;
+    if (lane == 0 && w.tile == 0 && w.g == 0) a.seg_f[(int64_t)w.seg * p.R + w.r] = any;
+  } else if (p.state_out && t1 == p.T && live) {
 #pragma unroll
     for (int j = 0; j < NL; ++j)
       if (s * NL + j < p.N) p.state_out[((int64_t)w.r * p.D + d) * p.N + s * NL + j] = h[j];
   }
 }
 
-// A segment's contribution to its neighbour.  Forward (REV = 0): the state at its end from a zero start, segments [0, nseg - 1).
-// Backward (REV = 1): the carry at its start from a zero carry, segments [1, nseg).
-template <typename T, int NL, int S, int REV>
-__global__ __launch_bounds__(WPB * 64) void k_scan_carry(Args a) {
-  constexpr int CW = 64 / S, NP = NL * S;
-  __shared__ float lds[WPB][TS * NP];
+// The backward pass's segments: the carry at a segment's start from a zero carry at its end, for segments [1, nseg).
+template <typename T, int NL>
+__global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
+  constexpr int NP = NL * S, VW = NL < 4 ? NL : 4;
+  typedef float vec __attribute__((ext_vector_type(VW)));
+  __shared__ __align__(16) float lds[WPB][TS * NP];
+  __shared__ __align__(8) float2 lds_d[WPB][TS][CW];
   const fdql_scan_t &p = a.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int u = blockIdx.x * WPB + wave;
   if (u >= (a.nseg - 1) * p.R * p.G * a.tpg) return;
   Unit w = unit_of(a, u);
-  if (REV) w.seg += 1;
-  const int c = lane % CW, s = lane / CW;
+  w.seg += 1;
+  const int c = lane / S, s = lane % S;
   const int dc = w.tile * CW + c, d = w.g * a.Dg + min(dc, a.Dg - 1);
   const bool live = dc < a.Dg;
   const int t0 = w.seg * a.seglen, t1 = min(p.T, t0 + a.seglen);
-  float *lds_w = lds[wave];
-  const Col<T> DT = column<T>(p.dt, p.dt_st, p.dt_sr, w.r, d),
-               V = REV ? column<T>(p.dy, p.dy_st, p.dy_sr, w.r, d) : column<T>(p.x, p.x_st, p.x_sr, w.r, d);
-  const bool gate = REV && p.z;
-  const Col<T> Z = gate ? column<T>(p.z, p.z_st, p.z_sr, w.r, d) : DT;
+  float *lC = lds[wave];
+  const Col<T> DT = col_of<T>(p.dt, p.dt_st, p.dt_sr, w.r, s, d), DY = col_of<T>(p.dy, p.dy_st, p.dy_sr, w.r, s, d),
+               Z = p.z ? col_of<T>(p.z, p.z_st, p.z_sr, w.r, s, d) : DY;
   const float bias = p.dt_bias ? p.dt_bias[d] : 0.f;
   float h[NL], A[NL], sum = 0.f;
   int any = 0;
@@ -223,52 +309,68 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry(Args a) {
     h[j] = 0.f;
     A[j] = s * NL + j < p.N ? p.A[(int64_t)d * p.N + s * NL + j] * LOG2E : 0.f;
   }
-  const int nt_all = t1 - t0, tiles = (nt_all + TS - 1) / TS;
-  for (int k = 0; k < tiles; ++k) {
-    const int t = t0 + (REV ? tiles - 1 - k : k) * TS, nt = min(TS, t1 - t);
-    if (REV) stage_rows<T, NP>(p.C, p.C_st, p.C_sr, p.C_sg, p, w.r, w.g, t, nt, lds_w, lane, 64);
-    else stage_rows<T, NP>(p.B, p.B_st, p.B_sr, p.B_sg, p, w.r, w.g, t, nt, lds_w, lane, 64);
-    const unsigned rst = reset_bits(p, w.r, t, nt, lane);
+  T yn[OWN] = {}, dn[OWN] = {}, zn[OWN] = {};
+  Rows<T, NP> Cn(p.C, p.C_st, p.C_sr, p.C_sg, w, p.N, lane);
+  uint8_t rn = 0;
+  const uint8_t *rp = p.reset ? p.reset + (int64_t)w.r * p.reset_sr + (lane % TS) * p.reset_st : nullptr;
+  const auto fetch = [&](int t) {
+#pragma unroll
+    for (int q = 0; q < OWN; ++q) {
+      if (t + q * S + s < t1) {
+        yn[q] = DY.at(t, q);
+        dn[q] = DT.at(t, q);
+        zn[q] = Z.at(t, q);
+      }
+    }
+    Cn.load(t, t1);
+    if (rp && t + lane % TS < t1) rn = rp[t * p.reset_st];
+  };
+  const int last = t0 + (t1 - t0 - 1) / TS * TS;
+  fetch(last);
+  for (int t = last; t >= t0; t -= TS) {
+    const int nt = min(TS, t1 - t);
+    const unsigned rst = (unsigned)__ballot(lane < nt && rn != 0);
     any |= rst != 0;
-    float v[TS], del[TS];
+    Cn.put(lC, lane);
+    float v[OWN], del[OWN];
 #pragma unroll
-    for (int i = 0; i < TS; ++i) {
-      const int ti = min(t + i, t1 - 1);
-      del[i] = DT.at(ti) + bias;
-      v[i] = V.at(ti);
-      if (gate) {
-        const float z = Z.at(ti);
-        v[i] *= z * sigmoid_f(z);
+    for (int q = 0; q < OWN; ++q) {
+      v[q] = to_f(yn[q]);
+      if (p.z) {
+        const float z = to_f(zn[q]);
+        v[q] *= z * sigmoid_f(z);
       }
-      if (p.dt_softplus) del[i] = softplus_f(del[i]);
+      del[q] = to_f(dn[q]) + bias;
+      if (p.dt_softplus) del[q] = softplus_f(del[q]);
+      lds_d[wave][q * S + s][c] = make_float2(del[q], v[q]);
     }
+    if (t > t0) fetch(t - TS);
     wave_lds_fence();
+    const auto tile = [&](auto whole) {
 #pragma unroll
-    for (int ii = 0; ii < TS; ++ii) {
-      const int i = REV ? TS - 1 - ii : ii;
-      if (i < nt) {
-        const bool cut = rst >> i & 1;
-        sum += del[i];
-        const float f = REV ? v[i] : del[i] * v[i];
-        if (!REV && cut) {
+      for (int i = TS - 1; i >= 0; --i) {
+        if (decltype(whole)::value || i < nt) {
+          const float2 q = lds_d[wave][i][c];
+          const float dl = q.x, dy = q.y;
+          sum += dl;
+          const bool cut = !decltype(whole)::value && (rst >> i & 1);
 #pragma unroll
-          for (int j = 0; j < NL; ++j) h[j] = 0.f;
-        }
+          for (int j4 = 0; j4 < NL; j4 += VW) {
+            const vec C = *reinterpret_cast<const vec *>(lC + i * NP + s * NL + j4);
 #pragma unroll
-        for (int j = 0; j < NL; ++j) {
-          const float e = __builtin_amdgcn_exp2f(del[i] * A[j]);
-          if (REV) h[j] = e * fmaf(f, lds_w[i * NP + s * NL + j], h[j]);
-          else h[j] = fmaf(e, h[j], f * lds_w[i * NP + s * NL + j]);
-        }
-        if (REV && cut) {
-#pragma unroll
-          for (int j = 0; j < NL; ++j) h[j] = 0.f;
+            for (int j = 0; j < VW; ++j) {
+              const float g = __builtin_amdgcn_exp2f(dl * A[j4 + j]) * fmaf(dy, C[j], h[j4 + j]);
+              h[j4 + j] = cut ? 0.f : g;
+            }
+          }
         }
       }
-    }
+    };
+    if (rst == 0 && nt == TS) tile(std::true_type());
+    else tile(std::false_type());
     wave_lds_fence();
   }
-  const int64_t o = lane_slot<NL, S>(a, w.seg, w);
+  const int64_t o = lane_slot<NL>(a, w.seg, w);
 #pragma unroll
   for (int j = 0; j < NL; ++j) a.seg_h[o + j * 64 + lane] = live ? h[j] : 0.f;
   a.seg_d[o / NL + lane] = sum;
@@ -276,9 +378,8 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry(Args a) {
 }
 
 // seg_h becomes the state every segment starts from (REV = 0) / the carry that enters every segment from the right (REV = 1).
-template <int NL, int S, int REV>
+template <int NL, int REV>
 __global__ __launch_bounds__(256) void k_scan_combine(Args a) {
-  constexpr int CW = 64 / S;
   const fdql_scan_t &p = a.p;
   const int64_t per = (int64_t)p.R * p.G * a.tpg * NL * 64;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -286,7 +387,7 @@ __global__ __launch_bounds__(256) void k_scan_combine(Args a) {
   const int lane = (int)(i & 63), j = (int)(i / 64 % NL);
   const int64_t blk = i / (64 * NL);
   const int tile = (int)(blk % a.tpg), g = (int)(blk / a.tpg % p.G), r = (int)(blk / a.tpg / p.G);
-  const int dc = tile * CW + lane % CW, n = lane / CW * NL + j;
+  const int dc = tile * CW + lane / S, n = lane % S * NL + j;
   const bool live = dc < a.Dg && n < p.N;
   const int d = g * a.Dg + min(dc, a.Dg - 1);
   const float A = live ? p.A[(int64_t)d * p.N + n] * LOG2E : 0.f;
@@ -310,51 +411,12 @@ __global__ __launch_bounds__(256) void k_scan_combine(Args a) {
 }
 
 // --------------------------------------------------------------------------------------------------------------- backward
-// v_permlane32_swap / v_permlane16_swap exchange half of one register's lanes with half of another's, so a swap and an add leave
-// in each half the sum over both of ONE of two values; inside a row of 16 the same takes two selects and a DPP add.
-__device__ __forceinline__ float dpp_ror8(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x128, 0xf, 0xf, true)); }
-__device__ __forceinline__ float dpp_half_mirror(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x141, 0xf, 0xf, true)); }
-__device__ __forceinline__ float dpp_xor2(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x4e, 0xf, 0xf, true)); }
-__device__ __forceinline__ float dpp_xor1(float v) { return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0xb1, 0xf, 0xf, true)); }
-
-// lanes with BIT clear end with the sum (over lanes BIT apart) of a, the others with that of b
-template <int BIT>
-__device__ __forceinline__ float fold(float a, float b, int lane) {
-  if constexpr (BIT == 32) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  } else if constexpr (BIT == 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
-    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  } else {
-    const bool up = lane & BIT;
-    const float keep = up ? b : a, give = up ? a : b;
-    if constexpr (BIT == 8) return keep + dpp_ror8(give);
-    else if constexpr (BIT == 4) return keep + dpp_half_mirror(give);
-    else return keep + dpp_xor2(give);
-  }
-}
-// Sums of eight values over the CW consecutive lanes of a part; value k = 4 b2 + 2 b1 + b0 ends (complete) in the lanes whose bits
-// CW/2, CW/4, CW/8 are b2, b1, b0.
-template <int CW>
-__device__ __forceinline__ float sum8(const float v[8], int lane) {
-  float u[4], q[2], o;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) u[i] = fold<CW / 2>(v[i], v[i + 4], lane);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) q[i] = fold<CW / 4>(u[i], u[i + 2], lane);
-  o = fold<CW / 8>(q[0], q[1], lane);
-  if constexpr (CW >= 64) o += dpp_half_mirror(o);
-  if constexpr (CW >= 32) o += dpp_xor2(o);
-  o += dpp_xor1(o);
-  return o;
-}
-
-template <typename T, int NL, int S>
+template <typename T, int NL>
 __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
-  constexpr int CW = 64 / S, NP = NL * S, PARTS = NL / 4;
-  __shared__ float lB[TS * NP], lC[TS * NP];
-  __shared__ float red[WPB][TS][2][NP];
+  constexpr int NP = NL * S;
+  __shared__ __align__(16) float lB[2][TS * NP], lC[2][TS * NP];
+  __shared__ __align__(16) v4f lds_d[WPB][TS][CW];     // delta, delta x, gated dy of every step
+  __shared__ __align__(8) float red[2][WPB][TS * 2 * NP];                       // [step][dB, dC][state]
   const fdql_scan_t &p = a.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nthreads = blockDim.x;
   int u = blockIdx.x;
@@ -367,135 +429,182 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
   const int active = min(a.wpw, a.tpg - wgt * a.wpw);
   const bool idle = w.tile >= a.tpg;            // a wave past the group's channels still takes part in staging and barriers
   if (idle) w.tile = a.tpg - 1;
-  const int c = lane % CW, s = lane / CW;
+  const int c = lane / S, s = lane % S;
   const int dc = w.tile * CW + c, d = w.g * a.Dg + min(dc, a.Dg - 1);
   const bool live = !idle && dc < a.Dg;
   const int t0 = w.seg * a.seglen, t1 = min(p.T, t0 + a.seglen);
 
-  const Col<T> X = column<T>(p.x, p.x_st, p.x_sr, w.r, d), DT = column<T>(p.dt, p.dt_st, p.dt_sr, w.r, d),
-               DY = column<T>(p.dy, p.dy_st, p.dy_sr, w.r, d), Z = p.z ? column<T>(p.z, p.z_st, p.z_sr, w.r, d) : X;
+  const Col<T> X = col_of<T>(p.x, p.x_st, p.x_sr, w.r, s, d), DT = col_of<T>(p.dt, p.dt_st, p.dt_sr, w.r, s, d),
+               DY = col_of<T>(p.dy, p.dy_st, p.dy_sr, w.r, s, d), Z = p.z ? col_of<T>(p.z, p.z_st, p.z_sr, w.r, s, d) : X;
   const float bias = p.dt_bias ? p.dt_bias[d] : 0.f, skip = p.skip ? p.skip[d] : 0.f;
   float A[NL], carry[NL], dA[NL], dskip = 0.f, dbias = 0.f;
 #pragma unroll
   for (int j = 0; j < NL; ++j) {
     const int n = s * NL + j;
-    A[j] = n < p.N ? p.A[(int64_t)d * p.N + n] : 0.f;
+    A[j] = n < p.N ? p.A[(int64_t)d * p.N + n] * LOG2E : 0.f;
     dA[j] = 0.f;
-    if (a.nseg > 1) carry[j] = a.seg_h[lane_slot<NL, S>(a, w.seg, w) + j * 64 + lane];
+    if (a.nseg > 1) carry[j] = a.seg_h[lane_slot<NL>(a, w.seg, w) + j * 64 + lane];
     else carry[j] = live && p.dstate_out && n < p.N ? p.dstate_out[((int64_t)w.r * p.D + d) * p.N + n] : 0.f;
   }
-  const int64_t o_st = (int64_t)p.R * p.D, o0 = (int64_t)w.r * p.D + d;
-  const int tiles = (t1 - t0 + TS - 1) / TS;
-  for (int k = tiles - 1; k >= 0; --k) {
-    const int t = t0 + k * TS, nt = min(TS, t1 - t);
-    stage_rows<T, NP>(p.B, p.B_st, p.B_sr, p.B_sg, p, w.r, w.g, t, nt, lB, threadIdx.x, nthreads);
-    stage_rows<T, NP>(p.C, p.C_st, p.C_sr, p.C_sg, p, w.r, w.g, t, nt, lC, threadIdx.x, nthreads);
-    const unsigned rst = reset_bits(p, w.r, t, nt, lane);
-    float x[TS], del[TS], dy[TS], yc[TS], dd[TS], gx[TS];
+  const int64_t o_st = (int64_t)p.R * p.D, o0 = (int64_t)w.r * p.D + s * o_st + d;
+  const int last = t0 + (t1 - t0 - 1) / TS * TS;
+  const int64_t slab_st = (int64_t)p.R * p.G * p.N, slab_0 = (int64_t)wgt * p.T * slab_st + ((int64_t)w.r * p.G + w.g) * p.N;
+  float *slab_b = a.slab_b + slab_0, *slab_c = a.slab_c + slab_0;
+
+  // the tile in front of this one, in flight while this one is computed
+  T xn[OWN] = {}, dn[OWN] = {}, yn[OWN] = {}, zn[OWN] = {};
+  Rows<T, NP> Bn(p.B, p.B_st, p.B_sr, p.B_sg, w, p.N, lane), Cn(p.C, p.C_st, p.C_sr, p.C_sg, w, p.N, lane);   // (staged by wave 0 and, where there is one, wave 1)
+  uint8_t rn = 0;
+  const uint8_t *rp = p.reset ? p.reset + (int64_t)w.r * p.reset_sr + (lane % TS) * p.reset_st : nullptr;
+  const int cw = blockDim.x > 64 ? 1 : 0;
+  const auto fetch = [&](int t) {
 #pragma unroll
-    for (int i = 0; i < TS; ++i) {
-      const int ti = min(t + i, t1 - 1);
-      x[i] = X.at(ti);
-      del[i] = DT.at(ti) + bias;
-      dy[i] = DY.at(ti);
+    for (int q = 0; q < OWN; ++q) {
+      if (t + q * S + s < t1) {
+        xn[q] = X.at(t, q);
+        dn[q] = DT.at(t, q);
+        yn[q] = DY.at(t, q);
+        zn[q] = Z.at(t, q);
+      }
+    }
+    if (wave == 0) Bn.load(t, t1);
+    if (wave == cw) Cn.load(t, t1);
+    if (rp && t + lane % TS < t1) rn = rp[t * p.reset_st];
+  };
+  const auto put = [&](int buf) {
+    if (wave == 0) Bn.put(lB[buf], lane);
+    if (wave == cw) Cn.put(lC[buf], lane);
+  };
+  fetch(last);
+  put(0);
+  __syncthreads();
+  int buf = 0;
+  for (int t = last; t >= t0; t -= TS, buf ^= 1) {
+    const int nt = min(TS, t1 - t);
+    const unsigned rst = (unsigned)__ballot(lane < nt && rn != 0);
+    // steps of this lane (S = 1: all eight): delta, delta x, gated dy; slope of the softplus, what dz is of the ungated output
+    float x[OWN], del[OWN], dx[OWN], dy[OWN], slope[OWN], zf[OWN];
+#pragma unroll
+    for (int q = 0; q < OWN; ++q) {
+      x[q] = live ? to_f(xn[q]) : 0.f;
+      dy[q] = live ? to_f(yn[q]) : 0.f;
       if (p.z) {
-        const float z = Z.at(ti);
-        dy[i] *= z * sigmoid_f(z);
+        const float z = to_f(zn[q]), sg = sigmoid_f(z);
+        zf[q] = dy[q] * sg * fmaf(z, 1.f - sg, 1.f);
+        dy[q] *= z * sg;
       }
-      if (!live) x[i] = dy[i] = 0.f;
-      if (p.dt_softplus) del[i] = softplus_f(del[i]);
-      yc[i] = dd[i] = gx[i] = 0.f;
+      del[q] = to_f(dn[q]) + bias;
+      slope[q] = 1.f;
+      if (p.dt_softplus) del[q] = softplus_f(del[q], slope[q]);
+      dx[q] = del[q] * x[q];
+      lds_d[wave][q * S + s][c] = v4f{del[q], dx[q], dy[q], 0.f};
     }
-    __syncthreads();
-    const float *ck = p.checkpoints + lane_slot<NL, S>(a, t / TS, w) + lane;
+    wave_lds_fence();
+    if (t > t0) fetch(t - TS);
+    const float *ck = p.checkpoints + lane_slot<NL>(a, t / TS, w) + lane;
+    const float *tB = lB[buf] + s * NL, *tC = lC[buf] + s * NL;
+    float *red_w = red[buf][wave];
+    float yc[TS], dd[TS], gx[TS];
 #pragma unroll
-    for (int part = 0; part < PARTS; ++part) {
-      float h[TS + 1][4], e[TS][4];
+    for (int i = 0; i < TS; ++i) yc[i] = dd[i] = gx[i] = 0.f;
+    const auto tile = [&](auto whole) {
+      constexpr bool W = decltype(whole)::value;   // eight steps without a reset
+      float h0 = ck[0], h1 = ck[64];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) h[0][j] = ck[(part * 4 + j) * 64];
+      for (int m = 0; m < NL; m += 2) {
+        float h[TS + 1][2], e[TS][2];
+        pass_edge();
+        h[0][0] = h0, h[0][1] = h1;
+        if (m + 2 < NL) h0 = ck[(m + 2) * 64], h1 = ck[(m + 3) * 64];
 #pragma unroll
-      for (int i = 0; i < TS; ++i) {
-        const float dl = del[i] * LOG2E, dx = del[i] * x[i];
-        const bool cut = rst >> i & 1;
+        for (int i = 0; i < TS; ++i) {
+          if (W || i < nt) {
+            const v4f st = lds_d[wave][i][c];
+            const float dl = st[0], dxi = st[1];
+            const float2 B = *reinterpret_cast<const float2 *>(tB + i * NP + m), C = *reinterpret_cast<const float2 *>(tC + i * NP + m);
+            const bool cut = !W && (rst >> i & 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int n = s * NL + part * 4 + j;
-          if (i < nt) {
-            e[i][j] = __builtin_amdgcn_exp2f(dl * A[part * 4 + j]);
-            h[i + 1][j] = dx * lB[i * NP + n];
-            if (!cut) h[i + 1][j] = fmaf(e[i][j], h[i][j], h[i + 1][j]);
-            yc[i] = fmaf(h[i + 1][j], lC[i * NP + n], yc[i]);
-          } else {
-            e[i][j] = 0.f;
-            h[i + 1][j] = h[i][j];
-          }
-        }
-      }
-#pragma unroll
-      for (int ii = 0; ii < TS; ++ii) {
-        const int i = TS - 1 - ii;
-        if (i < nt) {
-          const float dx = del[i] * x[i];
-          const bool cut = rst >> i & 1;
-          float v[8];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int n = s * NL + part * 4 + j, m = part * 4 + j;
-            const float g = fmaf(dy[i], lC[i * NP + n], carry[m]);
-            float ga = 0.f;
-            if (!cut) {
-              ga = g * e[i][j];
-              const float q = ga * h[i][j];
-              dd[i] = fmaf(q, A[m], dd[i]);
-              dA[m] = fmaf(q, del[i], dA[m]);
+            for (int j = 0; j < 2; ++j) {
+              e[i][j] = __builtin_amdgcn_exp2f(dl * A[m + j]);
+              const float in = dxi * (j ? B.y : B.x);
+              h[i + 1][j] = cut ? in : fmaf(e[i][j], h[i][j], in);
+              yc[i] = fmaf(h[i + 1][j], j ? C.y : C.x, yc[i]);
             }
-            gx[i] = fmaf(g, lB[i * NP + n], gx[i]);
-            v[j] = g * dx;
-            v[4 + j] = h[i + 1][j] * dy[i];
-            carry[m] = ga;
-          }
-          const float o = sum8<CW>(v, lane);
-          // value index: dB (first bit clear) or dC, then the state; one lane of each holding group writes
-          if ((lane & (CW / 8 - 1)) == 0) {
-            const int b2 = (lane / (CW / 2)) & 1, b1 = (lane / (CW / 4)) & 1, b0 = (lane / (CW / 8)) & 1;
-            red[wave][i][b2][s * NL + part * 4 + 2 * b1 + b0] = o;
-          }
-        }
-      }
-    }
+          } else {
 #pragma unroll
-    for (int i = 0; i < TS; ++i) {
-      if (i < nt) {
-        yc[i] = sum_parts<S>(yc[i]);
-        dd[i] = sum_parts<S>(dd[i]);
-        gx[i] = sum_parts<S>(gx[i]);
-        const float core = fmaf(skip, x[i], yc[i]);
-        float ddt = fmaf(x[i], gx[i], dd[i]);
-        if (p.dt_softplus) ddt *= sigmoid_f(DT.at(t + i) + bias);
-        dskip = fmaf(dy[i], x[i], dskip);
-        dbias += ddt;
-        if (live && s == 0) {
-          const int64_t o = o0 + (int64_t)(t + i) * o_st;
-          if (p.dx) reinterpret_cast<T *>(p.dx)[o] = from_f<T>(fmaf(skip, dy[i], del[i] * gx[i]));
-          if (p.ddt) reinterpret_cast<T *>(p.ddt)[o] = from_f<T>(ddt);
-          if (p.z && p.dz) {
-            const float z = Z.at(t + i), sg = sigmoid_f(z);
-            reinterpret_cast<T *>(p.dz)[o] = from_f<T>(DY.at(t + i) * core * sg * fmaf(z, 1.f - sg, 1.f));
+            for (int j = 0; j < 2; ++j) e[i][j] = 0.f, h[i + 1][j] = 0.f;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < TS; ++i) settle(yc[i]);
+        pass_edge();
+#pragma unroll
+        for (int i = TS - 1; i >= 0; --i) {
+          if (W || i < nt) {
+            const v4f st = lds_d[wave][i][c];
+            const float dl = st[0], dxi = st[1], dyi = st[2];
+            const float2 B = *reinterpret_cast<const float2 *>(tB + i * NP + m), C = *reinterpret_cast<const float2 *>(tC + i * NP + m);
+            const bool cut = !W && (rst >> i & 1);
+            float v[4];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float g = fmaf(dyi, j ? C.y : C.x, carry[m + j]);
+              float ga = g * e[i][j], q = ga * h[i][j];
+              if (cut) ga = q = 0.f;
+              dd[i] = fmaf(q, A[m + j], dd[i]);        // (A log2 e: undone at the end)
+              dA[m + j] = fmaf(q, dl, dA[m + j]);
+              gx[i] = fmaf(g, j ? B.y : B.x, gx[i]);
+              v[j] = g * dxi;
+              v[2 + j] = h[i + 1][j] * dyi;
+              carry[m + j] = ga;
+            }
+            settle(dd[i]);
+            settle(gx[i]);
+            settle(dA[m]);
+            settle(dA[m + 1]);
+            settle(carry[m]);
+            settle(carry[m + 1]);
+            // over the 16 channels: lane bits 5 and 4 end with dB or dC and the state of the two, bits 3 and 2 are summed as they are
+            float o = fold<16>(fold<32>(v[0], v[2], lane), fold<32>(v[1], v[3], lane), lane);
+            o += dpp_ror<8>(o);
+            o += dpp_ror<4>(o);
+            if ((lane & 12) == 0) red_w[(i * 2 + (lane >> 5)) * NP + s * NL + m + (lane >> 4 & 1)] = o;
           }
         }
       }
+    };
+    if (rst == 0 && nt == TS) tile(std::true_type());
+    else tile(std::false_type());
+    if (t > t0) put(buf ^ 1);
+    __syncthreads();                             // red of this tile and the rows of the next one are there
+    {
+      float yo[OWN], d_o[OWN], go[OWN];
+      own_sums(yc, yo, lane);
+      own_sums(dd, d_o, lane);
+      own_sums(gx, go, lane);
+#pragma unroll
+      for (int q = 0; q < OWN; ++q) {
+        const int i = q * S + s;
+        if (i < nt && live) {
+          const float ddt = fmaf(x[q], go[q], d_o[q] * LN2) * slope[q];
+          dskip = fmaf(dy[q], x[q], dskip);
+          dbias += ddt;
+          const int64_t o = o0 + (int64_t)(t + q * S) * o_st;
+          reinterpret_cast<T *>(p.dx)[o] = from_f<T>(fmaf(skip, dy[q], del[q] * go[q]));
+          reinterpret_cast<T *>(p.ddt)[o] = from_f<T>(ddt);
+          if (p.z && p.dz) reinterpret_cast<T *>(p.dz)[o] = from_f<T>(zf[q] * fmaf(skip, x[q], yo[q]));
+        }
+      }
     }
-    __syncthreads();
     for (int i = threadIdx.x; i < nt * 2 * NP; i += nthreads) {
       const int n = i % NP, which = i / NP % 2, k2 = i / (2 * NP);
       if (n < p.N) {
-        float v = 0.f;
-        for (int q = 0; q < active; ++q) v += red[q][k2][which][n];
-        float *slab = which ? a.slab_c : a.slab_b;
-        slab[((((int64_t)wgt * p.T + t + k2) * p.R + w.r) * p.G + w.g) * p.N + n] = v;
+        const float *r = red[buf][0] + i;
+        float v = r[0];
+        for (int q = 1; q < active; ++q) v += r[q * TS * 2 * NP];
+        (which ? slab_c : slab_b)[(int64_t)(t + k2) * slab_st + n] = v;
       }
     }
-    __syncthreads();
   }
   if (idle) return;
   if (w.seg == 0 && p.dstate_in && live) {
@@ -503,9 +612,14 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
     for (int j = 0; j < NL; ++j)
       if (s * NL + j < p.N) p.dstate_in[((int64_t)w.r * p.D + d) * p.N + s * NL + j] = carry[j];
   }
-  const int64_t o = lane_slot<NL, S>(a, w.seg, w);
+  const int64_t o = lane_slot<NL>(a, w.seg, w);
 #pragma unroll
   for (int j = 0; j < NL; ++j) a.part_a[o + j * 64 + lane] = dA[j];
+  // the parts' own steps added up (each saw TS / S of a tile's)
+  dskip += dpp_xor1(dskip);
+  dbias += dpp_xor1(dbias);
+  dskip += dpp_xor2(dskip);
+  dbias += dpp_xor2(dbias);
   a.part_s[o / NL * 2 + lane] = dskip;
   a.part_s[o / NL * 2 + 64 + lane] = dbias;
 }
@@ -524,9 +638,8 @@ __global__ __launch_bounds__(256) void k_scan_bc_finish(Args a) {
 }
 
 // dA, dskip, ddt_bias: partials of the (segment, row) pairs added up; a workgroup per 64 lanes of one state, 16 slices of the pairs.
-template <int NL, int S>
+template <int NL>
 __global__ __launch_bounds__(1024) void k_scan_par_finish(Args a) {
-  constexpr int CW = 64 / S;
   __shared__ float red[16][64];
   const fdql_scan_t &p = a.p;
   const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
@@ -541,12 +654,12 @@ __global__ __launch_bounds__(1024) void k_scan_par_finish(Args a) {
   v = 0.f;
 #pragma unroll
   for (int q = 0; q < 16; ++q) v += red[q][lane];
-  const int g = blk / a.tpg, dc = blk % a.tpg * CW + lane % CW, n = lane / CW * NL + j;
+  const int g = blk / a.tpg, dc = blk % a.tpg * CW + lane / S, n = lane % S * NL + j;
   if (dc >= a.Dg) return;
   const int64_t d = (int64_t)g * a.Dg + dc;
   if (j < NL) {
     if (n < p.N && p.dA) p.dA[d * p.N + n] = v;
-  } else if (lane < CW) {
+  } else if (lane % S == 0) {
     float *out = j == NL ? p.dskip : p.ddt_bias;
     if (out) out[d] = v;
   }
@@ -610,30 +723,22 @@ __global__ __launch_bounds__(256) void k_scan_step(fdql_scan_t p, int Dg, int tp
 
 // ------------------------------------------------------------------------------------------------------------------- host
 struct Plan {
-  int NL, S, tpg, Dg, nseg, seglen, wgt, wpw;
+  int NL, tpg, Dg, nseg, seglen, wgt, wpw;
 };
 
 int cus() { return 256; }
 
-// States per lane and lanes per channel, then segments.
 Plan plan_of(const fdql_scan_t &p) {
   Plan q;
   q.Dg = p.D / p.G;
   const int64_t rows = (int64_t)p.R * p.G;
-  if (p.N <= 4) q.NL = 4, q.S = 1;
-  else if (p.N <= 16) {
-    const bool few = rows * ((q.Dg + 63) / 64) < 512;
-    q.NL = few ? 4 : p.N <= 8 ? 8 : 16;
-    q.S = few ? 4 : 1;
-  } else if (p.N <= 32) q.NL = 16, q.S = 2;
-  else q.NL = 16, q.S = 4;
-  const int CW = 64 / q.S;
+  q.NL = p.N <= 8 ? 2 : p.N <= 16 ? 4 : p.N <= 32 ? 8 : 16;
   q.tpg = (q.Dg + CW - 1) / CW;
   const int64_t waves = rows * q.tpg;
   q.nseg = 1;
   q.seglen = p.T;
   if (waves > 0 && waves < 1024 && p.T >= 128) {
-    const int64_t want = std::min<int64_t>((2048 + waves - 1) / waves, p.T / 64);
+    const int64_t want = std::min<int64_t>((4096 + waves - 1) / waves, p.T / 64);
     if (want > 1) {
       q.seglen = (int)(((p.T + want - 1) / want + TS - 1) / TS * TS);
       q.nseg = (p.T + q.seglen - 1) / q.seglen;
@@ -671,28 +776,28 @@ Args args_of(const fdql_scan_t &p, const Plan &q, bool backward) {
   return a;
 }
 
-template <int NL_, int S_>
-struct Var { static constexpr int NL = NL_, S = S_; };
-
 template <typename F>
-hipError_t with_variant(const Plan &q, F f) {
-  if (q.S == 4) return q.NL == 4 ? f(Var<4, 4>()) : f(Var<16, 4>());
-  if (q.S == 2) return f(Var<16, 2>());
-  return q.NL == 4 ? f(Var<4, 1>()) : q.NL == 8 ? f(Var<8, 1>()) : f(Var<16, 1>());
+hipError_t with_states(int NL, F f) {
+  switch (NL) {
+    case 2: return f(std::integral_constant<int, 2>());
+    case 4: return f(std::integral_constant<int, 4>());
+    case 8: return f(std::integral_constant<int, 8>());
+    default: return f(std::integral_constant<int, 16>());
+  }
 }
 
 template <typename T>
 hipError_t fwd(const fdql_scan_t &p, hipStream_t s) {
   const Plan q = plan_of(p);
-  return with_variant(q, [&](auto v) {
-    constexpr int NL = decltype(v)::NL, S = decltype(v)::S;
+  return with_states(q.NL, [&](auto v) {
+    constexpr int NL = decltype(v)::value;
     const Args a = args_of(p, q, false);
     const int64_t per = (int64_t)p.R * p.G * q.tpg;
     if (q.nseg > 1) {
-      hipLaunchKernelGGL((k_scan_carry<T, NL, S, 0>), dim3((unsigned)(((q.nseg - 1) * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
-      hipLaunchKernelGGL((k_scan_combine<NL, S, 0>), dim3((unsigned)((per * NL * 64 + 255) / 256)), dim3(256), 0, s, a);
+      hipLaunchKernelGGL((k_scan_fwd<T, NL, true>), dim3((unsigned)(((q.nseg - 1) * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
+      hipLaunchKernelGGL((k_scan_combine<NL, 0>), dim3((unsigned)((per * NL * 64 + 255) / 256)), dim3(256), 0, s, a);
     }
-    hipLaunchKernelGGL((k_scan_fwd<T, NL, S>), dim3((unsigned)((q.nseg * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
+    hipLaunchKernelGGL((k_scan_fwd<T, NL, false>), dim3((unsigned)((q.nseg * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
     return hipGetLastError();
   });
 }
@@ -700,18 +805,18 @@ hipError_t fwd(const fdql_scan_t &p, hipStream_t s) {
 template <typename T>
 hipError_t bwd(const fdql_scan_t &p, hipStream_t s) {
   const Plan q = plan_of(p);
-  return with_variant(q, [&](auto v) {
-    constexpr int NL = decltype(v)::NL, S = decltype(v)::S;
+  return with_states(q.NL, [&](auto v) {
+    constexpr int NL = decltype(v)::value;
     const Args a = args_of(p, q, true);
     const int64_t per = (int64_t)p.R * p.G * q.tpg;
     if (q.nseg > 1) {
-      hipLaunchKernelGGL((k_scan_carry<T, NL, S, 1>), dim3((unsigned)(((q.nseg - 1) * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
-      hipLaunchKernelGGL((k_scan_combine<NL, S, 1>), dim3((unsigned)((per * NL * 64 + 255) / 256)), dim3(256), 0, s, a);
+      hipLaunchKernelGGL((k_scan_carry_back<T, NL>), dim3((unsigned)(((q.nseg - 1) * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
+      hipLaunchKernelGGL((k_scan_combine<NL, 1>), dim3((unsigned)((per * NL * 64 + 255) / 256)), dim3(256), 0, s, a);
     }
-    hipLaunchKernelGGL((k_scan_bwd<T, NL, S>), dim3((unsigned)((int64_t)q.nseg * p.R * p.G * q.wgt)), dim3(q.wpw * 64), 0, s, a);
+    hipLaunchKernelGGL((k_scan_bwd<T, NL>), dim3((unsigned)((int64_t)q.nseg * p.R * p.G * q.wgt)), dim3(q.wpw * 64), 0, s, a);
     const int64_t bc = (int64_t)p.T * p.R * p.G * p.N;
     hipLaunchKernelGGL((k_scan_bc_finish<T>), dim3((unsigned)std::min<int64_t>((bc + 255) / 256, 8 * cus()), 2), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((k_scan_par_finish<NL, S>), dim3((unsigned)(p.G * q.tpg * (NL + 2))), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((k_scan_par_finish<NL>), dim3((unsigned)(p.G * q.tpg * (NL + 2))), dim3(1024), 0, s, a);
     return hipGetLastError();
   });
 }

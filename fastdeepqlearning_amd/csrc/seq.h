@@ -34,15 +34,13 @@ __device__ __forceinline__ float exp_acc(float v) {
   const float e = __builtin_amdgcn_exp2f(hi);
   return fabsf(hi) < 126.f ? fmaf(e, lo * LN2, e) : e;   // (infinite or vanishing: nothing to correct)
 }
-// 1 / (1 + e^-v)
-__device__ __forceinline__ float sigmoid_f(float v) { return __builtin_amdgcn_rcpf(1.f + exp_acc(-v)); }
-// log(1 + e^v) = max(v, 0) + log1p(w), w = e^-|v| in (0, 1]: log1p(w) = 2 atanh(w / (2 + w)), the odd series to the ninth term
+// 1 / (1 + e^-v); the power's error, |v| float steps of it, is at most 0.3 steps of the sum
+__device__ __forceinline__ float sigmoid_f(float v) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * v)); }
+// log(1 + e^v) = max(v, 0) + log1p(w), w = e^-|v| in (0, 1]: log1p(w) = 2 atanh(w / (2 + w)), the odd series to the eighth term
 // (argument at most 1/3: the first term left out is below 2e-9 of the sum).  Keeps its relative precision for small steps.
-__device__ __forceinline__ float softplus_f(float v) {
-  const float w = exp_acc(-fabsf(v));
+__device__ __forceinline__ float softplus_w(float v, float w) {
   const float q = w * __builtin_amdgcn_rcpf(2.f + w), q2 = q * q;
-  float s = fmaf(q2, 1.f / 17.f, 1.f / 15.f);
-  s = fmaf(q2, s, 1.f / 13.f);
+  float s = fmaf(q2, 1.f / 15.f, 1.f / 13.f);
   s = fmaf(q2, s, 1.f / 11.f);
   s = fmaf(q2, s, 1.f / 9.f);
   s = fmaf(q2, s, 1.f / 7.f);
@@ -50,6 +48,13 @@ __device__ __forceinline__ float softplus_f(float v) {
   s = fmaf(q2, s, 1.f / 3.f);
   s = fmaf(q2, s, 1.f);
   return fmaxf(v, 0.f) + 2.f * q * s;
+}
+__device__ __forceinline__ float softplus_f(float v) { return softplus_w(v, exp_acc(-fabsf(v))); }
+// ... and its slope 1 / (1 + e^-v) from the same power
+__device__ __forceinline__ float softplus_f(float v, float &slope) {
+  const float w = exp_acc(-fabsf(v)), r = __builtin_amdgcn_rcpf(1.f + w);
+  slope = v >= 0.f ? r : w * r;
+  return softplus_w(v, w);
 }
 #endif
 }  // namespace fdql

@@ -58,13 +58,26 @@ __device__ __forceinline__ void input_at(const fdql_causal_conv_t &p, int t, int
   }
 }
 
+// The weights of V channels lie one after the other: whole 16-byte runs where V is 4 or 8.
 template <int V, int K>
 __device__ __forceinline__ void weights_of(const fdql_causal_conv_t &p, int d, float w[K][V], float b[V]) {
+  float run[V * K];
+  if constexpr (V % 4 == 0) {
+#pragma unroll
+    for (int i = 0; i < V * K; i += 4) load_v<float, 4>(p.weight + (int64_t)d * K + i, run + i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V * K; ++i) run[i] = p.weight[(int64_t)d * K + i];
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) w[k][i] = p.weight[(int64_t)(d + i) * K + k];
-    b[i] = p.bias ? p.bias[d + i] : 0.f;
+    for (int k = 0; k < K; ++k) w[k][i] = run[i * K + k];
+    b[i] = 0.f;
+  }
+  if (p.bias) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] = p.bias[d + i];
   }
 }
 
@@ -167,16 +180,32 @@ __global__ __launch_bounds__(WPB * 64) void k_seqconv_bwd(Args a) {
     for (int k = 0; k < K; ++k)
 #pragma unroll
       for (int v = 0; v < V; ++v) pend[k][v] = 0.f;
-    for (int t = t0; t < t1 + K - 1; ++t) {
-      float x[V], dy[V], dp[V];
-      bool cut = false;
+    // two steps ahead of the arithmetic
+    constexpr int AHEAD = 2;
+    float xn[AHEAD][V], yn[AHEAD][V];
+    bool cn[AHEAD];
+    const auto fetch = [&](int t, int k) {
+      cn[k] = false;
 #pragma unroll
-      for (int v = 0; v < V; ++v) x[v] = dy[v] = 0.f;
-      if (t < p.T) {
-        load_v<T, V>(reinterpret_cast<const T *>(p.x) + (int64_t)t * p.x_st + (int64_t)r * p.x_sr + d, x);
-        load_v<T, V>(reinterpret_cast<const T *>(p.dy) + (int64_t)t * p.dy_st + (int64_t)r * p.dy_sr + d, dy);
-        cut = cut_at(p, t, r);
+      for (int v = 0; v < V; ++v) xn[k][v] = yn[k][v] = 0.f;
+      if (t < min(p.T, t1 + K - 1)) {
+        load_v<T, V>(reinterpret_cast<const T *>(p.x) + (int64_t)t * p.x_st + (int64_t)r * p.x_sr + d, xn[k]);
+        load_v<T, V>(reinterpret_cast<const T *>(p.dy) + (int64_t)t * p.dy_st + (int64_t)r * p.dy_sr + d, yn[k]);
+        cn[k] = cut_at(p, t, r);
       }
+    };
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) fetch(t0 + k, k);
+    for (int tt = t0; tt < t1 + K - 1; tt += AHEAD)
+#pragma unroll
+    for (int ahead = 0; ahead < AHEAD; ++ahead) {
+      const int t = tt + ahead;
+      if (t >= t1 + K - 1) break;
+      float x[V], dy[V], dp[V];
+      const bool cut = cn[ahead];
+#pragma unroll
+      for (int v = 0; v < V; ++v) x[v] = xn[ahead][v], dy[v] = yn[ahead][v];
+      fetch(t + AHEAD, ahead);
       age = cut ? 0 : min(age + 1, K);
       push<V, K>(win, x, cut);
 #pragma unroll
@@ -255,6 +284,7 @@ __global__ __launch_bounds__(1024) void k_seqconv_finish(const float *__restrict
   const int d = blockIdx.x * 64 + lane;
   float v = 0.f;
   if (d < D)
+#pragma unroll 8
     for (int q = slice; q < nslab; q += 16) v += slab[((int64_t)q * (K + 1) + k) * D + d];
   red[slice][lane] = v;
   __syncthreads();
@@ -278,15 +308,15 @@ Plan plan_of(const fdql_causal_conv_t &p, int V) {
   q.V = V;
   q.blocks = (p.D + 64 * V - 1) / (64 * V);
   q.len = 64;
-  while (q.len > 8 && (int64_t)q.blocks * p.R * ((p.T + q.len - 1) / q.len) < 4096) q.len >>= 1;
+  while (q.len > 8 && (int64_t)q.blocks * p.R * ((p.T + q.len - 1) / q.len) < 1536) q.len >>= 1;
   q.chunks = std::max(1, (p.T + q.len - 1) / q.len);
-  q.wgs = (int)std::min<int64_t>(((int64_t)p.R * q.chunks + WPB - 1) / WPB, std::max(1, 1024 / q.blocks));
+  q.wgs = (int)std::min<int64_t>(((int64_t)p.R * q.chunks + WPB - 1) / WPB, std::max(1, 768 / q.blocks));
   return q;
 }
 int width_of(const fdql_causal_conv_t &p, bool backward) {
   const int esz = p.dtype == FDQL_F32 ? 4 : 2, V = 16 / esz;
   const auto ok = [&](const void *q) { return ((uintptr_t)q & 15) == 0; };
-  bool v = p.D % V == 0 && p.x_st % V == 0 && p.x_sr % V == 0 && (!p.state_in || p.state_in_sr % V == 0) && ok(p.x) && ok(p.state_in);
+  bool v = p.D % V == 0 && p.x_st % V == 0 && p.x_sr % V == 0 && (!p.state_in || p.state_in_sr % V == 0) && ok(p.x) && ok(p.state_in) && ok(p.weight);
   if (backward) v = v && p.dy_st % V == 0 && p.dy_sr % V == 0 && ok(p.dy) && ok(p.dstate_out) && ok(p.dx) && ok(p.dstate_in);
   else v = v && ok(p.y) && ok(p.state_out);
   return v ? V : 1;

@@ -292,10 +292,11 @@ def test_gated(dev, seq, M, D, F, dtype, form):
         assert torch.equal(seq.gated_linear(x, wg, wu, bg, bu, activation=kind), y)
 
 
+# many rows, many features, many channels: every tile shape of every product, edges on all sides
 @pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16", "f16"])
-def test_gated_many_tiles(dev, seq, dtype):
-    """Enough tiles for the large tile shape, edges on every side, rows split over workgroups for the weights' gradients."""
-    M, D, F = 5000, 136, 1030
+@pytest.mark.parametrize("M,D,F", [(5000, 136, 1030), (9000, 72, 1030), (13000, 520, 40), (22000, 776, 72), (200, 2000, 1600), (100, 2104, 4200)])
+def test_gated_many_tiles(dev, seq, M, D, F, dtype):
+    """Enough tiles for the large tile shapes, edges on every side, rows split over workgroups for the weights' gradients."""
     x, wg, wu, bg, bu, dy = _gated_inputs(dev, M, D, F, dtype, True, seed=1)
     leaves = [t.requires_grad_() for t in (x, wg, wu, bg, bu)]
     y = seq.gated_linear(*leaves, activation="silu")

@@ -17,6 +17,7 @@ class EncoderConf:
     class JoinerModeEnum(Enum):
         feedforward = 1
         gru = 2
+        ssm = 3     # addition of this implementation: a state-space block (causal convolution, selective scan, gated output)
 
     joiner_mode = JoinerModeEnum.feedforward
 
@@ -26,6 +27,8 @@ class EncoderConf:
         learned = 2
 
     rnn_latent_state_training_mode = RnnLatentStateTrainMode.zero
+    ssm_inner_dim = 0       # state-space joiner: channels (0: twice hidden_features) and states per channel
+    ssm_state_dim = 16
     use_burn_in = False
     burn_in_portion = 0.2
     # addition of this implementation: the pixel encoder the reference never had (obs_2d in the obs space)

@@ -42,8 +42,11 @@ def native_config_from_conf(conf):
         # uint8 frames (the usual pixel space) stay uint8 from the ring to the first conv layer when that layer has an
         # implicit-GEMM kernel (DeepQLearning.__init__ falls back to float32 frames when it has not)
         u8_frames = np.dtype(getattr(spaces["obs_2d"], "dtype", np.float32)) == np.uint8 and not getattr(conf, "pixel_frames_float32", False)
-    gru = getattr(getattr(ec, "joiner_mode", None), "name", "feedforward") == "gru"
+    joiner = getattr(getattr(ec, "joiner_mode", None), "name", "feedforward")
+    gru, ssm = joiner == "gru", joiner == "ssm"
     gru_mode = getattr(getattr(ec, "rnn_latent_state_training_mode", None), "name", "zero")
+    if ssm and gru_mode == "learned":
+        raise ValueError("the state-space joiner starts a window from zeros or from the stored state (rnn_latent_state_training_mode)")
     obs = _space_dim(spaces["obs_1d"]) if "obs_1d" in spaces else 0
     goal = _space_dim(spaces["desired_goal"]) if "desired_goal" in spaces else 0
     if conf.discrete:
@@ -62,7 +65,7 @@ def native_config_from_conf(conf):
                        pi_hidden=tuple(conf.pi_hidden_dims), critic_hidden=tuple(conf.critic_hidden_dims),
                        distributional=bool(conf.use_distributional_sac), use_lowerbound=bool(conf.use_nStep_lowerbounds),
                        use_max_entropy=bool(conf.use_max_entropy_q), bootstrap_nstep=boot, joiner_gru=gru, gru_state_mode=gru_mode, img=img, conv=conv,
-                       obs_2d_u8=u8_frames,
+                       obs_2d_u8=u8_frames, joiner_ssm=ssm, ssm_inner=int(getattr(ec, "ssm_inner_dim", 0)), ssm_state=int(getattr(ec, "ssm_state_dim", 16)),
                        burn_in_steps=int(conf.temporal_len * ec.burn_in_portion) if getattr(ec, "use_burn_in", False) else 0, hard_updates=bool(conf.use_hard_updates),
                        keep_frozen_copy=True, world_size=int(getattr(conf, "world_size", 1) or 1),
                        gamma=float(conf.gamma), tau=float(conf.tau), lr=float(conf.learning_rate),
@@ -273,7 +276,10 @@ class DeepQLearning:
         pass
 
     def get_random_hidden(self):
-        """encoder.py:113-117: None for the feed-forward joiner, torch.rand(latent) for the GRU."""
+        """encoder.py:113-117: None for the feed-forward joiner, torch.rand(latent) for the GRU; zeros for the state-space joiner
+        (nothing seen yet)."""
+        if self.native.cfg.joiner_ssm:
+            return torch.zeros(self.native.state_floats())
         if not self.native.cfg.joiner_gru:
             return None
         return torch.rand(int(self.native.cfg.latent))
@@ -359,7 +365,7 @@ class DeepQLearning:
             experiences.get("exploit_mask"), noise=noise, seed=self._seed ^ 0xAC7, counter=self._act_calls,
             want_info=log_now, agent_state=experiences.get("agent_state"), obs_2d=experiences.get("obs_2d"))
         action, log_prob, explore, exploit = res[:4]
-        hidden = res[4] if len(res) > 4 else None   # GRU joiner: the state the runner feeds back (runner.py:157)
+        hidden = res[4] if len(res) > 4 else None   # GRU / state-space joiner: the state the runner feeds back (runner.py:157)
         info = {}
         if conf.discrete:   # deepQlearning.py:175-178: argmax(-1, True) -> int64 indices
             action = action.long()

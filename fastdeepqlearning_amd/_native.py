@@ -45,6 +45,7 @@ class AgentConfig(C.Structure):
         ("img_c", C.c_int32), ("img_h", C.c_int32), ("img_w", C.c_int32), ("n_conv", C.c_int32),
         ("conv_out", C.c_int32 * MAX_CONV), ("conv_k", C.c_int32 * MAX_CONV), ("conv_s", C.c_int32 * MAX_CONV),
         ("joiner_gru", C.c_int32), ("gru_state_mode", C.c_int32),
+        ("joiner_ssm", C.c_int32), ("ssm_inner", C.c_int32), ("ssm_state", C.c_int32),
         ("distributional", C.c_int32), ("use_lowerbound", C.c_int32), ("use_max_entropy", C.c_int32),
         ("hard_updates", C.c_int32), ("keep_frozen_copy", C.c_int32), ("bootstrap_nstep", C.c_int32), ("obs_2d_u8", C.c_int32),
         ("burn_in_steps", C.c_int32),
@@ -90,7 +91,7 @@ class CausalConv(C.Structure):
     _fields_ = [(k, C.c_int32) for k in ("size", "dtype", "T", "R", "D", "K", "silu")] + [
         ("x", C.c_void_p), ("x_st", C.c_int64), ("x_sr", C.c_int64), ("weight", C.c_void_p), ("bias", C.c_void_p),
         ("reset", C.c_void_p), ("reset_st", C.c_int64), ("reset_sr", C.c_int64), ("state_in", C.c_void_p), ("state_in_sr", C.c_int64),
-        ("y", C.c_void_p), ("state_out", C.c_void_p), ("dy", C.c_void_p), ("dy_st", C.c_int64), ("dy_sr", C.c_int64),
+        ("y", C.c_void_p), ("state_out", C.c_void_p), ("state_out_sr", C.c_int64), ("dy", C.c_void_p), ("dy_st", C.c_int64), ("dy_sr", C.c_int64),
         ("dstate_out", C.c_void_p), ("dx", C.c_void_p), ("dstate_in", C.c_void_p), ("dweight", C.c_void_p), ("dbias", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
 
@@ -101,7 +102,7 @@ class Scan(C.Structure):
         (k, C.c_int64) for k in ("x_st", "x_sr", "dt_st", "dt_sr", "z_st", "z_sr")] + [("B", C.c_void_p), ("C", C.c_void_p)] + [
         (k, C.c_int64) for k in ("B_st", "B_sr", "B_sg", "C_st", "C_sr", "C_sg")] + [
         (k, C.c_void_p) for k in ("A", "skip", "dt_bias", "reset")] + [("reset_st", C.c_int64), ("reset_sr", C.c_int64),
-        ("state_in", C.c_void_p), ("state_in_sr", C.c_int64), ("y", C.c_void_p), ("state_out", C.c_void_p), ("checkpoints", C.c_void_p),
+        ("state_in", C.c_void_p), ("state_in_sr", C.c_int64), ("y", C.c_void_p), ("state_out", C.c_void_p), ("state_out_sr", C.c_int64), ("checkpoints", C.c_void_p),
         ("dy", C.c_void_p), ("dy_st", C.c_int64), ("dy_sr", C.c_int64)] + [
         (k, C.c_void_p) for k in ("dstate_out", "dx", "ddt", "dz", "dB", "dC", "dA", "dskip", "ddt_bias", "dstate_in", "workspace")] + [
         ("workspace_bytes", C.c_int64)]
@@ -153,6 +154,7 @@ SIGNATURES = {
     "fdql_agent_arena_floats": (_i64, [_vp, _i32]),
     "fdql_agent_tensor_info": (_i32, [_vp, _i32, C.c_char_p, _i32, C.POINTER(_i32), C.POINTER(_i64), C.POINTER(_i32)]),
     "fdql_agent_workspace_bytes": (_i64, [_vp]),
+    "fdql_agent_state_floats": (_i64, [_vp]),
     "fdql_agent_conv_reads_ring": (_i32, [_vp]),
     "fdql_agent_bind": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64]),
     "fdql_agent_update": (C.c_int, [_vp, C.POINTER(Batch), _vp, _vp, _u64, _i32, _vp]),

@@ -5,6 +5,7 @@ compute on the hot path runs in libfdql_hip.so.  The franQ-shaped classes in
 fastdeepqlearning_amd.Replay / .Agent are built on these two.
 """
 import ctypes as C
+import math
 from collections import OrderedDict
 
 import numpy as np
@@ -243,7 +244,7 @@ def make_config(obs_dim, act_dim, T, B, goal_dim=0, discrete=False, n_critics=2,
                 distributional=True, use_lowerbound=True, use_max_entropy=True, hard_updates=False,
                 keep_frozen_copy=True, world_size=1, gamma=0.99, tau=5e-2, lr=3e-4, beta1=0.9, beta2=0.999,
                 adam_eps=1e-8, init_log_alpha=-2.0, drop_frac=0.2, bootstrap_nstep=False, burn_in_steps=0, joiner_gru=False,
-                gru_state_mode=0, img=(), conv=(), obs_2d_u8=False):
+                gru_state_mode=0, img=(), conv=(), obs_2d_u8=False, joiner_ssm=False, ssm_inner=0, ssm_state=16):
     c = N.AgentConfig()
     c.obs_dim, c.goal_dim, c.act_dim, c.discrete = obs_dim, goal_dim, act_dim, int(discrete)
     c.n_critics, c.n_quantiles, c.latent, c.enc_features = n_critics, n_quantiles, latent, enc_features
@@ -269,7 +270,10 @@ def make_config(obs_dim, act_dim, T, B, goal_dim=0, discrete=False, n_critics=2,
         for i, (co, k, st) in enumerate(conv):
             c.conv_out[i], c.conv_k[i], c.conv_s[i] = int(co), int(k), int(st)
     c.joiner_gru = int(bool(joiner_gru))
-    c.gru_state_mode = {"zero": 0, "store": 1, "learned": 2}.get(gru_state_mode, gru_state_mode) if joiner_gru else 0
+    c.gru_state_mode = {"zero": 0, "store": 1, "learned": 2}.get(gru_state_mode, gru_state_mode) if joiner_gru or joiner_ssm else 0
+    c.joiner_ssm = int(bool(joiner_ssm))    # state-space joiner (the reference has none); ssm_inner 0: twice the encoder's features
+    if joiner_ssm:
+        c.ssm_inner, c.ssm_state = int(ssm_inner) or 2 * int(enc_features), int(ssm_state)
     c.T, c.B, c.world_size = T, B, world_size
     c.gamma, c.tau, c.lr, c.beta1, c.beta2, c.adam_eps = gamma, tau, lr, beta1, beta2, adam_eps
     c.init_log_alpha, c.drop_frac = init_log_alpha, drop_frac
@@ -474,12 +478,13 @@ class NativeAgent:
         explore = torch.empty(rows, adim, device=dev) if want_info else None
         exploit = torch.empty(rows, adim, device=dev) if want_info else None
         hs_in = hs_out = None
-        if cfg.joiner_gru:
-            hs_out = torch.empty(rows, cfg.latent, device=dev)
+        width = self.state_floats()
+        if width:
+            hs_out = torch.empty(rows, width, device=dev)
             if agent_state is not None:
                 hs_in = f32(agent_state)
-                if tuple(hs_in.shape) != (rows, cfg.latent):
-                    raise ValueError(f"act(): agent_state must be [rows, {cfg.latent}]")
+                if tuple(hs_in.shape) != (rows, width):
+                    raise ValueError(f"act(): agent_state must be [rows, {width}]")
         self._act_keep = (obs, ag, dg, mask, noise, hs_in, img)
         with torch.cuda.device(dev):
             N.check(self.lib.fdql_agent_act(self.handle, N.ptr(obs), N.ptr(ag), N.ptr(dg), N.ptr(img), N.ptr(hs_in),
@@ -488,9 +493,13 @@ class NativeAgent:
                                             N.ptr(exploit), N.ptr(hs_out), C.c_void_p(self._act_ws.data_ptr()),
                                             self._act_ws.numel(),
                                             N.current_stream(dev)))
-        if cfg.joiner_gru:
+        if width:
             return action, logp, explore, exploit, hs_out
         return action, logp, explore, exploit
+
+    def state_floats(self):
+        """Floats of one row's carried state (agent_state / the hidden state act() returns); 0 for the feed-forward joiner."""
+        return int(self.lib.fdql_agent_state_floats(self.handle))
 
     def scalars(self):
         out = (C.c_float * 8)()
@@ -562,6 +571,13 @@ class NativeAgent:
                 v.copy_(((torch.rand(v.shape, generator=g) * 2 - 1) * a).to(self.device))
             elif k == "encoder.hidden_state":                              # encoder.py:42,117
                 v.copy_(torch.rand(v.shape, generator=g).to(self.device))
+            elif k == "encoder.joiner.A_log":                              # decay rates 1 .. ssm_state in every channel
+                v.copy_(torch.arange(1, v.shape[1] + 1, dtype=torch.float32).log().expand(v.shape).to(self.device))
+            elif k == "encoder.joiner.skip":
+                v.fill_(1.0)
+            elif k == "encoder.joiner.dt_bias":                            # softplus(dt_bias) log-uniform in 0.001 .. 0.1
+                step = torch.exp(torch.rand(v.shape, generator=g) * math.log(100.0) + math.log(1e-3))
+                v.copy_((step + torch.log(-torch.expm1(-step))).to(self.device))
             elif k.endswith("weight"):
                 fan_out, fan_in = v.shape
                 a = (6.0 / (fan_in + fan_out)) ** 0.5

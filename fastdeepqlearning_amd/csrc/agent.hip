@@ -123,8 +123,8 @@ int prepare_update(fdql_agent *a, const fdql_batch_t *batch, const float *noise_
                "batch.obs_2d_slots (frames read from the ring in place) needs fdql_agent_conv_reads_ring()");
   FDQL_REQUIRE(!a->cfg.goal_dim || (batch->achieved_goal && batch->desired_goal), "goal_dim > 0 needs achieved/desired goal");
   FDQL_REQUIRE(!a->cfg.use_lowerbound || batch->mc_return, "use_lowerbound needs mc_return");
-  FDQL_REQUIRE(!(a->cfg.joiner_gru && a->cfg.gru_state_mode == 1) || batch->agent_state,
-               "GRU joiner in store mode needs batch.agent_state");
+  FDQL_REQUIRE(!(a->recurrent() && a->cfg.gru_state_mode == 1) || batch->agent_state,
+               "a recurrent joiner in store mode needs batch.agent_state");
   if (!a->plan_ready || memcmp(&a->batch, batch, sizeof(*batch)) != 0) {
     if (a->plan_ready) {   // keep the plan being replaced
       a->plan_cache.push_back({a->batch, std::move(a->stages), a->tables_dev, a->graph});
@@ -206,6 +206,10 @@ int fdql_agent_create(fdql_agent_t **out, const fdql_agent_config_t *cfg) {
                "GRU joiner: one layer only (len(joint_hidden_dims) == 1) - the reference's own hidden-state plumbing "
                "(encoder.py:83-87, 117) carries a [latent] vector per row");
   FDQL_REQUIRE(!c.joiner_gru || (c.gru_state_mode >= 0 && c.gru_state_mode <= 2), "gru_state_mode must be 0, 1 or 2");
+  FDQL_REQUIRE(!(c.joiner_gru && c.joiner_ssm), "joiner_gru and joiner_ssm exclude each other");
+  FDQL_REQUIRE(!c.joiner_ssm || (c.ssm_inner >= 1 && c.ssm_inner <= 1 << 16 && c.ssm_state >= 1 && c.ssm_state <= 64),
+               "state-space joiner: ssm_inner 1..65536 and ssm_state 1..64, got %d and %d", c.ssm_inner, c.ssm_state);
+  FDQL_REQUIRE(!c.joiner_ssm || c.gru_state_mode == 0 || c.gru_state_mode == 1, "state-space joiner: gru_state_mode must be 0 (zeros) or 1 (stored)");
   FDQL_REQUIRE(c.burn_in_steps >= 0 && c.burn_in_steps <= c.T - 1, "burn_in_steps outside [0, T-1]");
   FDQL_REQUIRE(!c.bootstrap_nstep || (!c.distributional && c.use_lowerbound),
                "bootstrap_nstep needs distributional == 0 and use_lowerbound == 1 (the reference forms the term only in "
@@ -323,6 +327,7 @@ int32_t fdql_agent_tensor_info(const fdql_agent_t *a, int32_t index, char *name,
   return 0;
 }
 
+int64_t fdql_agent_state_floats(const fdql_agent_t *a) { return a ? a->state_floats() : -1; }
 int64_t fdql_agent_workspace_bytes(const fdql_agent_t *a) { return a ? a->ws_need : -1; }
 
 int fdql_agent_bind(fdql_agent_t *a, float *params, float *grads, float *adam_m, float *adam_v, float *targets,

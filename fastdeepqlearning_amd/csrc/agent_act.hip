@@ -16,6 +16,10 @@ int64_t fdql_agent_act_workspace_bytes(const fdql_agent_t *a, int32_t rows) {
   int64_t joiner = act_mlp_floats(a->joiner, rows);
   if (a->cfg.joiner_gru)   // gi, gh [rows, 3L], zero start state and the new state [rows, L]
     joiner = 2 * pad4((int64_t)rows * 3 * a->cfg.latent) + 2 * pad4((int64_t)rows * a->cfg.latent);
+  if (a->cfg.joiner_ssm) {   // (x, z), x behind the convolution, (dt, B, C), y, the latent state, A, the new state
+    const int64_t Di = a->cfg.ssm_inner, Ns = a->cfg.ssm_state, r = rows;
+    joiner = pad4(r * 2 * Di) + pad4(r * Di) + pad4(r * (Di + 2 * Ns)) + pad4(r * Di) + pad4(r * a->cfg.latent) + pad4(Di * Ns) + pad4(r * a->state_floats());
+  }
   int64_t conv = 0;   // im2col matrix + NHWC output of every conv layer
   for (const auto &Lc : a->conv) {
     const int64_t pos = (int64_t)rows * Lc.g.OH * Lc.g.OW;
@@ -125,7 +129,38 @@ int fdql_agent_act(fdql_agent_t *a, const float *obs_1d, const float *achieved_g
     if (!a->conv.empty()) in[nin++] = {cin, a->conv_feat, a->conv_feat};
   }
   if (e == hipSuccess) e = act_mlp(a, a->enc_obs, in, nin, rows, top, &enc, s);
-  if (e == hipSuccess && !c.joiner_gru) {
+  if (e == hipSuccess && c.joiner_ssm) {
+    // one step of the state-space joiner from the carried state (NULL = zeros)
+    const int Di = c.ssm_inner, Ns = c.ssm_state, F = c.enc_features, W = Di + 2 * Ns;
+    const int64_t r = rows, sf = a->state_floats();
+    float *xz = top; top += pad4(r * 2 * Di);
+    float *xc = top; top += pad4(r * Di);
+    float *sel = top; top += pad4(r * W);
+    float *y = top; top += pad4(r * Di);
+    float *lat = top; top += pad4(r * c.latent);
+    float *A = top; top += pad4((int64_t)Di * Ns);
+    float *next = hidden_state ? hidden_state : top;
+    top += pad4(r * sf);
+    e = ssm_prep_launch(nullptr, nullptr, 0, rows, nullptr, a->params + a->ssm.a_log, A, Di * Ns, s);
+    ActLayerArgs l;
+    memset(&l, 0, sizeof(l));
+    l.in[0] = {enc, F, F}; l.nseg = 1; l.W = a->params + a->ssm.w_in; l.ldw = F; l.bias = a->params + a->ssm.b_in;
+    l.out = xz; l.ldo = 2 * Di; l.N = 2 * Di; l.rows = rows; l.leaky = 0;
+    if (e == hipSuccess) e = act_layer_launch(l, s);
+    fdql_causal_conv_t cv = ssm_conv_of(a, 1, rows);
+    cv.x = xz; cv.y = xc; cv.state_in = agent_state; cv.state_in_sr = sf; cv.state_out = next; cv.state_out_sr = sf;
+    if (e == hipSuccess) e = seqconv_fwd_launch(cv, s);
+    l.in[0] = {xc, Di, Di}; l.W = a->params + a->ssm.w_sel; l.ldw = Di; l.bias = nullptr; l.out = sel; l.ldo = W; l.N = W;
+    if (e == hipSuccess) e = act_layer_launch(l, s);
+    fdql_scan_t sc = ssm_scan_of(a, 1, rows);
+    sc.x = xc; sc.z = xz + Di; sc.dt = sel; sc.B = sel + Di; sc.C = sel + Di + Ns; sc.A = A; sc.y = y;
+    sc.state_in = agent_state ? agent_state + 3 * Di : nullptr; sc.state_in_sr = sf; sc.state_out = next + 3 * Di; sc.state_out_sr = sf;
+    if (e == hipSuccess) e = scan_fwd_launch(sc, s);
+    fdql_gated_t g = ssm_gated_of(a, rows);
+    g.x = y; g.y = lat;
+    if (e == hipSuccess) e = gated_fwd_launch(g, s);
+    state = lat;
+  } else if (e == hipSuccess && !c.joiner_gru) {
     ActSeg x = {enc, a->enc_obs.dout, a->enc_obs.dout};
     e = act_mlp(a, a->joiner, &x, 1, rows, top, &state, s);
   } else if (e == hipSuccess) {

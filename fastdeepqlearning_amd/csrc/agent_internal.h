@@ -19,6 +19,7 @@
 #include <string>
 #include <vector>
 
+#include "seq.h"
 #include "chain.h"
 #include "wstat.h"
 #include "wgrad.h"
@@ -191,6 +192,11 @@ struct fdql_agent {
   // GRU joiner (cfg.joiner_gru): offsets of weight_ih_l0 [3L,F], weight_hh_l0 [3L,L], bias_ih_l0, bias_hh_l0 [3L],
   // encoder.hidden_state [L] in the trainable arena
   int64_t gru_wih = 0, gru_whh = 0, gru_bih = 0, gru_bhh = 0, gru_h0 = 0;
+  // state-space joiner (cfg.joiner_ssm): Di = ssm_inner, Ns = ssm_state.  in_proj [2 Di, F], conv [Di, 4], sel_proj [Di + 2 Ns, Di], dt_bias [Di],
+  // A_log [Di, Ns], skip [Di], gate / up [L, Di] with their biases
+  struct SsmOffsets { int64_t w_in, b_in, w_conv, b_conv, w_sel, dt_bias, a_log, skip, w_gate, b_gate, w_up, b_up; } ssm = {};
+  bool recurrent() const { return cfg.joiner_gru || cfg.joiner_ssm; }
+  int64_t state_floats() const { return cfg.joiner_gru ? cfg.latent : cfg.joiner_ssm ? (int64_t)cfg.ssm_inner * (3 + cfg.ssm_state) : 0; }
   int64_t n_train = 0, tgt_begin = 0, tgt_end = 0, crit_begin = 0, crit_end = 0;
   std::vector<TensorInfo> tensors;
 
@@ -290,6 +296,10 @@ namespace fdql {
 constexpr int STREAM_WGRAD_MAX_SLAB_ROWS = 640;   // K-split slabs up to this many rows: narrow weight gradients on the streaming launch
 int layout(fdql_agent *a);            // agent_plan.hip: parameter arenas under the reference's state_dict names
 void carve(fdql_agent *a);            // ... the workspace
+// structs of the state-space joiner's operators on `rows` rows of T steps (agent_plan.hip; act() uses T = 1); tensors are filled in by the caller
+fdql_causal_conv_t ssm_conv_of(const fdql_agent *a, int T, int rows);
+fdql_scan_t ssm_scan_of(const fdql_agent *a, int T, int rows);
+fdql_gated_t ssm_gated_of(const fdql_agent *a, int64_t rows);
 int build_plan(fdql_agent *a);        // ... the launch list for a->batch (ends with upload_tables)
 int upload_tables(fdql_agent *a);
 }  // namespace fdql

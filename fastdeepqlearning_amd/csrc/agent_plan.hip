@@ -51,6 +51,28 @@ int layout(fdql_agent *a) {
     a->gru_bih = top; top += pad4(L3);
     a->tensors.push_back({"encoder.joiner.bias_hh_l0", 0, top, L3, 0});
     a->gru_bhh = top; top += pad4(L3);
+  } else if (c.joiner_ssm) {   // no counterpart in the reference (fdql_agent_config_t::joiner_ssm)
+    const int Di = c.ssm_inner, Ns = c.ssm_state, L = c.latent;
+    a->joiner = MlpDesc();
+    a->joiner.din = c.enc_features; a->joiner.dout = L;
+    auto add = [&](const char *name, int rows, int cols) {
+      a->tensors.push_back({std::string("encoder.joiner.") + name, 0, top, rows, cols});
+      const int64_t at = top;
+      top += pad4((int64_t)rows * (cols ? cols : 1));
+      return at;
+    };
+    a->ssm.w_in = add("in_proj.weight", 2 * Di, c.enc_features);
+    a->ssm.b_in = add("in_proj.bias", 2 * Di, 0);
+    a->ssm.w_conv = add("conv.weight", Di, 4);
+    a->ssm.b_conv = add("conv.bias", Di, 0);
+    a->ssm.w_sel = add("sel_proj.weight", Di + 2 * Ns, Di);
+    a->ssm.dt_bias = add("dt_bias", Di, 0);
+    a->ssm.a_log = add("A_log", Di, Ns);
+    a->ssm.skip = add("skip", Di, 0);
+    a->ssm.w_gate = add("gate_proj.weight", L, Di);
+    a->ssm.b_gate = add("gate_proj.bias", L, 0);
+    a->ssm.w_up = add("up_proj.weight", L, Di);
+    a->ssm.b_up = add("up_proj.bias", L, 0);
   } else {
     add_mlp(a, a->joiner, "encoder.joiner", c.enc_features, c.joint_hidden, c.n_joint_hidden, c.latent, top);
   }
@@ -94,6 +116,33 @@ int layout(fdql_agent *a) {
     }
   }
   return 0;
+}
+
+// ------------------------------------------------------------------------------ state-space joiner
+fdql_causal_conv_t ssm_conv_of(const fdql_agent *a, int T, int rows) {
+  fdql_causal_conv_t p = {};
+  p.size = sizeof(p); p.dtype = FDQL_F32; p.T = T; p.R = rows; p.D = a->cfg.ssm_inner; p.K = 4; p.silu = 1;
+  p.weight = a->params + a->ssm.w_conv; p.bias = a->params + a->ssm.b_conv;
+  p.x_sr = 2ll * p.D; p.x_st = (int64_t)rows * p.x_sr;      // the first half of every (x, z) row
+  return p;
+}
+fdql_scan_t ssm_scan_of(const fdql_agent *a, int T, int rows) {
+  fdql_scan_t p = {};
+  p.size = sizeof(p); p.dtype = FDQL_F32; p.T = T; p.R = rows; p.D = a->cfg.ssm_inner; p.N = a->cfg.ssm_state; p.G = 1; p.dt_softplus = 1;
+  p.skip = a->params + a->ssm.skip; p.dt_bias = a->params + a->ssm.dt_bias;
+  p.x_sr = p.D; p.x_st = (int64_t)rows * p.x_sr;
+  p.z_sr = 2ll * p.D; p.z_st = (int64_t)rows * p.z_sr;
+  p.dt_sr = p.B_sr = p.C_sr = p.D + 2ll * p.N;              // (dt, B, C) rows
+  p.dt_st = p.B_st = p.C_st = (int64_t)rows * p.dt_sr;
+  return p;
+}
+fdql_gated_t ssm_gated_of(const fdql_agent *a, int64_t rows) {
+  fdql_gated_t p = {};
+  p.size = sizeof(p); p.dtype = FDQL_F32; p.M = rows; p.D = a->cfg.ssm_inner; p.F = a->cfg.latent; p.act = FDQL_ACT_SILU;
+  p.x_sr = p.D;
+  p.w_gate = a->params + a->ssm.w_gate; p.b_gate = a->params + a->ssm.b_gate;
+  p.w_up = a->params + a->ssm.w_up; p.b_up = a->params + a->ssm.b_up;
+  return p;
 }
 
 // ------------------------------------------------------------------------------ workspace
@@ -149,6 +198,31 @@ void carve(fdql_agent *a) {
     a->alloc("gru.wpack_f", (int64_t)c.latent * L3);      // persistent scans (gruscan.hip): W_hh packed in the forward scan's stream order
     a->alloc("gru.wpack_b", (int64_t)c.latent * L3);      // ... and W_hh^T in the backward scan's
     a->alloc("gru.dh_init", Bw * c.latent);               // ... and d h_{-1} per row (learned start state)
+  } else if (c.joiner_ssm) {
+    const int64_t Di = c.ssm_inner, Ns = c.ssm_state;
+    const int B = a->B;
+    a->alloc("ssm.reset", (N + 3) / 4);          // bytes [T, B]
+    a->alloc("ssm.A", Di * Ns);
+    a->alloc("ssm.xz", N * 2 * Di);
+    a->alloc("ssm.xc", N * Di);
+    a->alloc("ssm.sel", N * (Di + 2 * Ns));
+    a->alloc("ssm.y", N * Di);
+    a->alloc("ssm.pre", 2 * M * c.latent);
+    a->alloc("ssm.dy", M * Di);
+    a->alloc("ssm.dxs", M * Di);                 // d x through the scan alone, then with the selection's part
+    a->alloc("ssm.dxc", M * Di);
+    a->alloc("ssm.ddt", M * Di);
+    a->alloc("ssm.dz", M * Di);
+    a->alloc("ssm.dB", M * Ns);
+    a->alloc("ssm.dC", M * Ns);
+    a->alloc("ssm.dx", M * Di);
+    a->alloc("ssm.dA", Di * Ns);
+    const fdql_scan_t sc = ssm_scan_of(a, a->T, B), sb = ssm_scan_of(a, a->T - 1, B);
+    a->alloc("ssm.ck", scan_checkpoint_floats(sc));
+    const int64_t ws = std::max(std::max(scan_workspace_bytes(sc, false), scan_workspace_bytes(sb, true)),
+                                std::max(seqconv_workspace_bytes(ssm_conv_of(a, a->T - 1, B)),
+                                         std::max(gated_workspace_bytes(ssm_gated_of(a, M), false), gated_workspace_bytes(ssm_gated_of(a, M), true))));
+    a->alloc("ssm.ws", std::max<int64_t>((ws + 3) / 4, 4));   // scratch of whichever operator runs
   } else {
     mlp_bufs("joiner", a->joiner, N, true, false);
   }
@@ -471,10 +545,10 @@ int build_plan(fdql_agent *a) {
     eo.in.push_back({feat, a->conv_feat, a->conv_feat});
   }
   eo.out = a->buf("enc_obs.out"); eo.ldout = c.enc_features;
-  const bool gru = c.joiner_gru != 0;
+  const bool gru = c.joiner_gru != 0, ssm = c.joiner_ssm != 0, recurrent = gru || ssm;   // (recurrent: no joiner MLP)
   MlpInst jo;
   float *state = a->buf("state");
-  if (!gru) {
+  if (!recurrent) {
     jo = make_inst(a, a->joiner, "joiner", params, 0, N, true);
     jo.in.push_back({eo.out, c.enc_features, c.enc_features});
     jo.out = state; jo.ldout = L;
@@ -609,7 +683,7 @@ int build_plan(fdql_agent *a) {
   // Round 6: the same four networks on 16- / 32-row blocks, two workgroups per CU, weights eight groups ahead (fwdchain.hip) when
   // they have the reference's default shape (one hidden layer of 256 everywhere) - k_chain's blocks are latency-bound below a
   // dispatch round of them
-  if (chain_mode == 1 && !gru && nconv == 0 && a->enc_obs.hid.size() == 1 && a->joiner.hid.size() == 1 && a->actor.hid.size() == 1 &&
+  if (chain_mode == 1 && !recurrent && nconv == 0 && a->enc_obs.hid.size() == 1 && a->joiner.hid.size() == 1 && a->actor.hid.size() == 1 &&
       a->enc_obs.hid[0] == F3_W && a->joiner.hid[0] == F3_W && a->actor.hid[0] == F3_W && c.enc_features == F3_W && L == F3_W &&
       (int)eo.in.size() <= F3_MAX_IN) {
     Fwd3Args fa;
@@ -644,7 +718,7 @@ int build_plan(fdql_agent *a) {
       enc_chained = true;
     }
   }
-  for (size_t t = 0; t < bms.size() && !enc_chained && (chain_all || chain_on) && !gru; ++t) {
+  for (size_t t = 0; t < bms.size() && !enc_chained && (chain_all || chain_on) && !recurrent; ++t) {
     Stage cs;
     cs.kind = ST_CHAIN; cs.name = "enc_joiner_actors"; cs.chain_bm = bms[t];
     ChainBuilder cb(cs);
@@ -661,8 +735,46 @@ int build_plan(fdql_agent *a) {
     // nothing left to launch for these three networks
   } else {
   fwd_chain({&eo}, "enc_obs");
-  if (!gru) {
+  if (!recurrent) {
     fwd_chain({&jo}, "joiner");
+  } else if (ssm) {
+    // state-space joiner: two projections on the grouped GEMM, the sequence operators' own launches between them
+    const int Di = c.ssm_inner, Ns = c.ssm_state, F = c.enc_features, T = a->T, W = Di + 2 * Ns;
+    float *xz = a->buf("ssm.xz"), *xc = a->buf("ssm.xc"), *sel = a->buf("ssm.sel"), *y = a->buf("ssm.y"), *A = a->buf("ssm.A"), *scratch = a->buf("ssm.ws");
+    uint8_t *reset = reinterpret_cast<uint8_t *>(a->buf("ssm.reset"));
+    const float *td = x.task_done, *es = x.episode_step, *a_log = params + a->ssm.a_log;
+    const float *carried = c.gru_state_mode == 1 ? x.agent_state : nullptr;
+    const int64_t carried_sr = a->state_floats();
+    b.func_stage("ssm.prep", [=](hipStream_t s) { return ssm_prep_launch(td, es, T, B, reset, a_log, A, Di * Ns, s); });
+    {
+      Stage &gs = b.gemm_stage("ssm.in");
+      GemmProblem p = Builder::new_gemm(N, 2 * Di, xz, 2 * Di);
+      Builder::add_seg(p, eo.out, F, 1, params + a->ssm.w_in, F, 1, F);
+      p.bias = params + a->ssm.b_in;
+      gs.gemm.push_back(p);
+    }
+    fdql_causal_conv_t cv = ssm_conv_of(a, T, B);
+    cv.x = xz; cv.y = xc; cv.reset = reset; cv.reset_st = B; cv.reset_sr = 1; cv.state_in = carried; cv.state_in_sr = carried_sr;
+    b.func_stage("ssm.conv", [=](hipStream_t s) { return seqconv_fwd_launch(cv, s); });
+    {
+      Stage &gs = b.gemm_stage("ssm.sel");
+      GemmProblem p = Builder::new_gemm(N, W, sel, W);
+      Builder::add_seg(p, xc, Di, 1, params + a->ssm.w_sel, Di, 1, Di);
+      gs.gemm.push_back(p);
+    }
+    fdql_scan_t sc = ssm_scan_of(a, T, B);
+    sc.x = xc; sc.z = xz + Di; sc.dt = sel; sc.B = sel + Di; sc.C = sel + Di + Ns; sc.A = A; sc.y = y;
+    sc.reset = reset; sc.reset_st = B; sc.reset_sr = 1; sc.checkpoints = a->buf("ssm.ck"); sc.workspace = scratch;
+    if (carried) { sc.state_in = carried + 3 * Di; sc.state_in_sr = carried_sr; }
+    b.func_stage("ssm.scan", [=](hipStream_t s) { return scan_fwd_launch(sc, s); });
+    // the last step's rows feed no gradient: their pre-activations are not kept
+    fdql_gated_t g1 = ssm_gated_of(a, M), g2 = ssm_gated_of(a, B);
+    g1.x = y; g1.y = state; g1.pre = a->buf("ssm.pre");
+    g2.x = y + (int64_t)M * Di; g2.y = state + (int64_t)M * L;
+    b.func_stage("ssm.gated", [=](hipStream_t s) {
+      const hipError_t e = gated_fwd_launch(g1, s);
+      return e == hipSuccess ? gated_fwd_launch(g2, s) : e;
+    });
   } else {
     // GRU joiner (encoder.py:40-42, 63-65): the input projection of all T*B rows is one GEMM; the scan over t is
     // T x (recurrent GEMM [B, L] x [L, 3L] + gate kernel) - sequential by nature and latency-bound at B = 256
@@ -1166,7 +1278,7 @@ int build_plan(fdql_agent *a) {
   // round - one rank's share of a data-parallel batch (config 2 at 128 / 64 / 32 windows: 98 / 49 / 24.5 blocks of 64) and
   // temporal_len 2 - instead of the summing launch + three tile / small-batch launches.  chain_bm: 0 = the 64-row rules above.
   int chain_bm = 0;
-  if (a->dstate_split && L % 4 == 0 && !gru && !a->joiner.hid.empty()) {
+  if (a->dstate_split && L % 4 == 0 && !recurrent && !a->joiner.hid.empty()) {
     MlpInst jq = jo;
     jq.rows = M;
     GemmProblem p = b.bwd_dpre(jq, (int)a->joiner.hid.size() - 1, a->buf("dstate"), L);
@@ -1234,6 +1346,45 @@ int build_plan(fdql_agent *a) {
     }
     if (!chain_bm) hosts.push_back(a->stages.size() - 1);   // (a member of the small-block chain carries no riders: it must stay a lone problem)
   }
+  if (ssm) {
+    // the steps t <= T-2 carry gradient (the last state only feeds no_grad targets)
+    const int Di = c.ssm_inner, Ns = c.ssm_state, T1 = a->T - 1;
+    const float *xz = a->buf("ssm.xz"), *xc = a->buf("ssm.xc"), *sel = a->buf("ssm.sel"), *A = a->buf("ssm.A");
+    float *slab = a->buf("slabs"), *dy = a->buf("ssm.dy"), *dxs = a->buf("ssm.dxs"), *dxc = a->buf("ssm.dxc"), *ddt = a->buf("ssm.ddt"), *dz = a->buf("ssm.dz"),
+          *dB = a->buf("ssm.dB"), *dC = a->buf("ssm.dC"), *dA = a->buf("ssm.dA"), *scratch = a->buf("ssm.ws");
+    const uint8_t *reset = reinterpret_cast<const uint8_t *>(a->buf("ssm.reset"));
+    const float *carried = c.gru_state_mode == 1 ? x.agent_state : nullptr;
+    const int64_t carried_sr = a->state_floats();
+    fdql_gated_t g = ssm_gated_of(a, M);
+    g.x = a->buf("ssm.y"); g.pre = a->buf("ssm.pre"); g.dy = a->buf("dstate"); g.dy_sr = L; g.dx = dy;
+    g.dw_gate = slab + a->ssm.w_gate; g.db_gate = slab + a->ssm.b_gate; g.dw_up = slab + a->ssm.w_up; g.db_up = slab + a->ssm.b_up;
+    g.workspace = scratch;
+    b.func_stage("ssm.gated_bwd", [=](hipStream_t s) { return gated_bwd_launch(g, s); });
+    fdql_scan_t sc = ssm_scan_of(a, T1, B);
+    sc.x = xc; sc.z = xz + Di; sc.dt = sel; sc.B = sel + Di; sc.C = sel + Di + Ns; sc.A = A;
+    sc.reset = reset; sc.reset_st = B; sc.reset_sr = 1; sc.checkpoints = a->buf("ssm.ck"); sc.workspace = scratch;
+    if (carried) { sc.state_in = carried + 3 * Di; sc.state_in_sr = carried_sr; }
+    sc.dy = dy; sc.dy_sr = Di; sc.dy_st = (int64_t)B * Di;
+    sc.dx = dxs; sc.ddt = ddt; sc.dz = dz; sc.dB = dB; sc.dC = dC; sc.dA = dA; sc.dskip = slab + a->ssm.skip; sc.ddt_bias = slab + a->ssm.dt_bias;
+    b.func_stage("ssm.scan_bwd", [=](hipStream_t s) { return scan_bwd_launch(sc, s); });
+    float *da_log = slab + a->ssm.a_log;
+    b.func_stage("ssm.dA_log", [=](hipStream_t s) { return ssm_dalog_launch(dA, A, Di * Ns, da_log, s); });
+    {
+      Stage &gs = b.gemm_stage("ssm.dsel");        // + what reaches x through (dt, B, C)
+      GemmProblem p = Builder::new_gemm(M, Di, dxc, Di);
+      const float *w = params + a->ssm.w_sel;
+      Builder::add_seg(p, ddt, Di, 1, w, Di, 0, Di);
+      Builder::add_seg(p, dB, Ns, 1, w + (int64_t)Di * Di, Di, 0, Ns);
+      Builder::add_seg(p, dC, Ns, 1, w + (int64_t)(Di + Ns) * Di, Di, 0, Ns);
+      p.epi = EPI_ADD_REF; p.ref = dxs; p.ldref = Di;
+      gs.gemm.push_back(p);
+    }
+    fdql_causal_conv_t cv = ssm_conv_of(a, T1, B);
+    cv.x = xz; cv.reset = reset; cv.reset_st = B; cv.reset_sr = 1; cv.state_in = carried; cv.state_in_sr = carried_sr;
+    cv.dy = dxc; cv.dy_sr = Di; cv.dy_st = (int64_t)B * Di; cv.dx = a->buf("ssm.dx");
+    cv.dweight = slab + a->ssm.w_conv; cv.dbias = slab + a->ssm.b_conv; cv.workspace = scratch;
+    b.func_stage("ssm.conv_bwd", [=](hipStream_t s) { return seqconv_bwd_launch(cv, s); });
+  }
   if (gru) {
     // back-propagation through time over the T-1 rows that carry gradient (h_{T-1} only feeds no_grad targets):
     //   dh_t = d state[t] + dh_{t+1} * z_{t+1} + d gh_{t+1} W_hh
@@ -1281,7 +1432,11 @@ int build_plan(fdql_agent *a) {
     Stage &gs = b.gemm_stage("denc");
     GemmProblem p = Builder::new_gemm(M, c.enc_features, a->buf("denc"), c.enc_features);
     if (gru) Builder::add_seg(p, a->buf("gru.dgi"), 3 * L, 1, params + a->gru_wih, c.enc_features, 0, 3 * L);
-    else b.input_grad_segs(jb, a->buf("dstate"), L, 0, p);
+    else if (ssm) {
+      const int Di = c.ssm_inner;
+      Builder::add_seg(p, a->buf("ssm.dx"), Di, 1, params + a->ssm.w_in, c.enc_features, 0, Di);
+      Builder::add_seg(p, a->buf("ssm.dz"), Di, 1, params + a->ssm.w_in + (int64_t)Di * c.enc_features, c.enc_features, 0, Di);
+    } else b.input_grad_segs(jb, a->buf("dstate"), L, 0, p);
     p.colsum = a->buf("cs.denc");
     gs.gemm.push_back(p);
     if (fold_dsum) gs.rd_max_blocks = rd_max_blocks;
@@ -1347,7 +1502,19 @@ int build_plan(fdql_agent *a) {
     // actor: needs d logits / its dpre -> from the d state launch on
     b.wgrads(ao, a->buf("dlogits"), a->actor.dout, nullptr, a->stages[idx_dstate], tail, ws);
     // joiner: needs d state and its dpre -> the d enc launch; encoder MLP: needs d enc and its dpre -> the tail
-    if (!gru) {
+    if (ssm) {   // the projections' weights; the operators have left theirs in slab 0
+      const int Di = c.ssm_inner, Ns = c.ssm_state, F = c.enc_features;
+      float *slab = a->buf("slabs");
+      Stage &host = a->stages[idx_denc];
+      const float *xc = a->buf("ssm.xc"), *dx = a->buf("ssm.dx"), *dz = a->buf("ssm.dz");
+      b.wgrad_gemm(M, dx, Di, Di, eo.out, F, F, slab + a->ssm.w_in, F, host, tail);
+      b.wgrad_gemm(M, dz, Di, Di, eo.out, F, F, slab + a->ssm.w_in + (int64_t)Di * F, F, host, tail);
+      b.wgrad_bias(M, dx, Di, Di, nullptr, slab + a->ssm.b_in, ws);
+      b.wgrad_bias(M, dz, Di, Di, nullptr, slab + a->ssm.b_in + Di, ws);
+      b.wgrad_gemm(M, a->buf("ssm.ddt"), Di, Di, xc, Di, Di, slab + a->ssm.w_sel, Di, host, tail);
+      b.wgrad_gemm(M, a->buf("ssm.dB"), Ns, Ns, xc, Di, Di, slab + a->ssm.w_sel + (int64_t)Di * Di, Di, host, tail);
+      b.wgrad_gemm(M, a->buf("ssm.dC"), Ns, Ns, xc, Di, Di, slab + a->ssm.w_sel + (int64_t)(Di + Ns) * Di, Di, host, tail);
+    } else if (!gru) {
       b.wgrads(jb, a->buf("dstate"), L, cs_dstate, chain_bm ? tail : a->stages[idx_denc], tail, ws, cs_dstate_rows);
     } else {   // GRU weights: dW_hh = d gh^T h_prev, dW_ih = d gi^T e, biases = column sums (all over the M rows)
       const int L3 = 3 * L, F = c.enc_features;

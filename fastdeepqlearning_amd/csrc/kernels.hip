@@ -2371,7 +2371,7 @@ __device__ __forceinline__ void act_layer_body(const ActLayerArgs &a, float *xs,
     }
   }
   if (lane == 0) {
-    const float b0 = a.bias[n0], b1 = has1 ? a.bias[n0 + 1] : 0.f;
+    const float b0 = a.bias ? a.bias[n0] : 0.f, b1 = a.bias && has1 ? a.bias[n0 + 1] : 0.f;
 #pragma unroll
     for (int r = 0; r < ACT_RCH; ++r) {
       if (r < nr) {

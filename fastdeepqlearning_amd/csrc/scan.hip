@@ -277,7 +277,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
   } else if (p.state_out && t1 == p.T && live) {
 #pragma unroll
     for (int j = 0; j < NL; ++j)
-      if (s * NL + j < p.N) p.state_out[((int64_t)w.r * p.D + d) * p.N + s * NL + j] = h[j];
+      if (s * NL + j < p.N) p.state_out[(int64_t)w.r * p.state_out_sr + (int64_t)d * p.N + s * NL + j] = h[j];
   }
 }
 
@@ -707,7 +707,7 @@ __global__ __launch_bounds__(256) void k_scan_step(fdql_scan_t p, int Dg, int tp
         if (fresh) h[k] = dx_c * B[k];
         acc = fmaf(h[k], C[k], acc);
       }
-      if (p.state_out) *reinterpret_cast<vec *>(p.state_out + ((int64_t)r * p.D + dd) * p.N + n) = h;
+      if (p.state_out) *reinterpret_cast<vec *>(p.state_out + (int64_t)r * p.state_out_sr + dd * p.N + n) = h;
     }
     for (int m = 1; m < lpc; m <<= 1) acc += __shfl_xor(acc, m);
     const float back = __shfl(acc, (lane % cpt) * lpc);            // the sum of channel it * cpt + (lane % cpt)
@@ -825,7 +825,7 @@ template <typename T>
 hipError_t step(const fdql_scan_t &p, hipStream_t s) {
   const int Dg = p.D / p.G, tpg = (Dg + 63) / 64;
   const auto al = [](const void *q) { return ((uintptr_t)q & 15) == 0; };
-  const bool vec = p.N % 4 == 0 && al(p.A) && al(p.state_in) && al(p.state_out) && (!p.state_in || p.state_in_sr % 4 == 0);
+  const bool vec = p.N % 4 == 0 && al(p.A) && al(p.state_in) && al(p.state_out) && (!p.state_in || p.state_in_sr % 4 == 0) && (!p.state_out || p.state_out_sr % 4 == 0);
   int lpc = 1;
   while (lpc * (vec ? 4 : 1) < p.N) lpc <<= 1;
   const dim3 grid((unsigned)(((int64_t)p.R * p.G * tpg + 3) / 4));

@@ -18,6 +18,10 @@ int64_t gated_workspace_bytes(const fdql_gated_t &p, bool backward);
 hipError_t gated_fwd_launch(const fdql_gated_t &p, hipStream_t s);
 hipError_t gated_bwd_launch(const fdql_gated_t &p, hipStream_t s);
 
+// Pieces of the agent's state-space joiner (agent_plan.hip); T = 0: A alone
+hipError_t ssm_prep_launch(const float *task_done, const float *episode_step, int T, int B, uint8_t *reset, const float *A_log, float *A, int n, hipStream_t s);
+hipError_t ssm_dalog_launch(const float *dA, const float *A, int n, float *out, hipStream_t s);
+
 #if defined(__HIPCC__)
 // Element types: float, bf16 and fp16 in memory, float in registers; conversions round to nearest even.
 typedef __bf16 bf16_t;

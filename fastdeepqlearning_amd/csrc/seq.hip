@@ -13,9 +13,9 @@ __global__ __launch_bounds__(256) void k_seq_zero(float *p, int64_t n) {
 __global__ __launch_bounds__(256) void k_seq_zero16(uint16_t *p, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = 0;
 }
-// dst [R, per] dense = src (row stride sr) or zeros
-__global__ __launch_bounds__(256) void k_seq_copy_rows(const float *src, int64_t sr, float *dst, int64_t R, int64_t per) {
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < R * per; i += (int64_t)gridDim.x * 256) dst[i] = src ? src[i / per * sr + i % per] : 0.f;
+// dst [R, per] (row stride dr) = src (row stride sr) or zeros
+__global__ __launch_bounds__(256) void k_seq_copy_rows(const float *src, int64_t sr, float *dst, int64_t dr, int64_t R, int64_t per) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < R * per; i += (int64_t)gridDim.x * 256) dst[i / per * dr + i % per] = src ? src[i / per * sr + i % per] : 0.f;
 }
 dim3 grid_for(int64_t n) { return dim3((unsigned)(n < 256 * 1024 ? (n + 255) / 256 : 1024)); }
 
@@ -26,9 +26,9 @@ int zero(void *p, int64_t n, int32_t dtype, hipStream_t s) {   // a kernel, not 
   FDQL_HIP(hipGetLastError());
   return FDQL_OK;
 }
-int copy_rows(const float *src, int64_t sr, float *dst, int64_t R, int64_t per, hipStream_t s) {
+int copy_rows(const float *src, int64_t sr, float *dst, int64_t dr, int64_t R, int64_t per, hipStream_t s) {
   if (!dst || R * per == 0) return FDQL_OK;
-  hipLaunchKernelGGL(k_seq_copy_rows, grid_for(R * per), dim3(256), 0, s, src, sr, dst, R, per);
+  hipLaunchKernelGGL(k_seq_copy_rows, grid_for(R * per), dim3(256), 0, s, src, sr, dst, dr, R, per);
   FDQL_HIP(hipGetLastError());
   return FDQL_OK;
 }
@@ -74,14 +74,40 @@ int check_workspace(const char *what, const void *ws, int64_t have, int64_t need
     if (_rc != FDQL_OK) return _rc; \
   } while (0)
 
+// State-space joiner: reset[t][b] where window b breaks between t - 1 and t (the same test as is_contiguous: episode_step runs on and the step
+// before was not terminal), and A = -exp(A_log).
+__global__ __launch_bounds__(256) void k_ssm_prep(const float *task_done, const float *episode_step, int T, int B, uint8_t *reset, const float *A_log, float *A, int n) {
+  const int64_t rows = (int64_t)T * B;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows + n; i += (int64_t)gridDim.x * 256) {
+    if (i < rows) reset[i] = i >= B && !(episode_step[i] == episode_step[i - B] + 1.f && task_done[i - B] == 0.f);
+    else A[i - rows] = -exp_acc(A_log[i - rows]);
+  }
+}
+// d A_log = dA * dA/dA_log = dA * A
+__global__ __launch_bounds__(256) void k_ssm_dalog(const float *dA, const float *A, int n, float *out) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) out[i] = dA[i] * A[i];
+}
+
 }  // namespace
+
+namespace fdql {
+hipError_t ssm_prep_launch(const float *task_done, const float *episode_step, int T, int B, uint8_t *reset, const float *A_log, float *A, int n, hipStream_t s) {
+  hipLaunchKernelGGL(k_ssm_prep, grid_for((int64_t)T * B + n), dim3(256), 0, s, task_done, episode_step, T, B, reset, A_log, A, n);
+  return hipGetLastError();
+}
+hipError_t ssm_dalog_launch(const float *dA, const float *A, int n, float *out, hipStream_t s) {
+  hipLaunchKernelGGL(k_ssm_dalog, dim3((n + 255) / 256), dim3(256), 0, s, dA, A, n, out);
+  return hipGetLastError();
+}
+}  // namespace fdql
 
 extern "C" int fdql_causal_conv(const fdql_causal_conv_t *p, void *stream) {
   FDQL_TRY(check_conv(p));
   if (p->R == 0) return FDQL_OK;
   FDQL_REQUIRE(p->weight && (p->T == 0 || (p->x && p->y)), "causal_conv: x, weight and y are needed");
-  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1 && p->state_in_sr == (int64_t)(p->K - 1) * p->D),
-               "causal_conv: the state is updated in place only in a single step over dense rows");
+  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1 && p->state_in_sr == p->state_out_sr),
+               "causal_conv: the state is updated in place only in a single step");
   FDQL_HIP(seqconv_fwd_launch(*p, (hipStream_t)stream));
   return FDQL_OK;
 }
@@ -106,9 +132,9 @@ extern "C" int fdql_scan(const fdql_scan_t *p, void *stream) {
   hipStream_t s = (hipStream_t)stream;
   FDQL_TRY(check_scan(p));
   if (p->R == 0) return FDQL_OK;
-  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1 && !p->checkpoints && p->state_in_sr == (int64_t)p->D * p->N),
-               "scan: the state is updated in place only in a single step over dense rows");
-  if (p->T == 0) return copy_rows(p->state_in, p->state_in_sr, p->state_out, p->R, (int64_t)p->D * p->N, s);
+  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1 && !p->checkpoints && p->state_in_sr == p->state_out_sr),
+               "scan: the state is updated in place only in a single step");
+  if (p->T == 0) return copy_rows(p->state_in, p->state_in_sr, p->state_out, p->state_out_sr, p->R, (int64_t)p->D * p->N, s);
   FDQL_REQUIRE(p->x && p->dt && p->A && p->B && p->C && p->y, "scan: x, dt, A, B, C and y are needed");
   FDQL_TRY(check_workspace("scan", p->workspace, p->workspace_bytes, scan_workspace_bytes(*p, false)));
   FDQL_HIP(scan_fwd_launch(*p, s));
@@ -129,7 +155,7 @@ extern "C" int fdql_scan_backward(const fdql_scan_t *p, void *stream) {
     FDQL_TRY(zero(p->dA, (int64_t)p->D * p->N, FDQL_F32, s));
     FDQL_TRY(zero(p->dskip, p->D, FDQL_F32, s));
     FDQL_TRY(zero(p->ddt_bias, p->D, FDQL_F32, s));
-    return copy_rows(p->dstate_out, (int64_t)p->D * p->N, p->dstate_in, p->R, (int64_t)p->D * p->N, s);
+    return copy_rows(p->dstate_out, (int64_t)p->D * p->N, p->dstate_in, (int64_t)p->D * p->N, p->R, (int64_t)p->D * p->N, s);
   }
   FDQL_REQUIRE(p->x && p->dt && p->A && p->B && p->C && p->dy, "scan backward: x, dt, A, B, C and dy are needed");
   FDQL_REQUIRE(p->checkpoints, "scan backward: the forward call's checkpoints are needed");

@@ -139,7 +139,7 @@ __global__ __launch_bounds__(WPB * 64) void k_seqconv_fwd(Args a) {
   }
   if (p.state_out && t1 == p.T) {
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) store_v<T, V>(reinterpret_cast<T *>(p.state_out) + ((int64_t)r * (K - 1) + k) * p.D + d, win[k + 1]);
+    for (int k = 0; k < K - 1; ++k) store_v<T, V>(reinterpret_cast<T *>(p.state_out) + (int64_t)r * p.state_out_sr + (int64_t)k * p.D + d, win[k + 1]);
   }
 }
 
@@ -318,7 +318,7 @@ int width_of(const fdql_causal_conv_t &p, bool backward) {
   const auto ok = [&](const void *q) { return ((uintptr_t)q & 15) == 0; };
   bool v = p.D % V == 0 && p.x_st % V == 0 && p.x_sr % V == 0 && (!p.state_in || p.state_in_sr % V == 0) && ok(p.x) && ok(p.state_in) && ok(p.weight);
   if (backward) v = v && p.dy_st % V == 0 && p.dy_sr % V == 0 && ok(p.dy) && ok(p.dstate_out) && ok(p.dx) && ok(p.dstate_in);
-  else v = v && ok(p.y) && ok(p.state_out);
+  else v = v && ok(p.y) && ok(p.state_out) && (!p.state_out || p.state_out_sr % V == 0);
   return v ? V : 1;
 }
 

@@ -143,6 +143,7 @@ std::pair<Tensor, Tensor> conv_run(const Tensor &x, const Tensor &weight, const 
   fdql_causal_conv_t p = conv_args(x, weight, bias, state, reset, silu);
   p.y = ptr(y);
   p.state_out = ptr(out_state);
+  if (out_state.defined()) p.state_out_sr = out_state.stride(0);
   check(api.conv(&p, stream_of(x)));
   return {y, out_state};
 }
@@ -208,7 +209,7 @@ std::pair<Tensor, Tensor> causal_conv_step(const Tensor &x, const Opt &state_, c
   check_reset(what, x, reset);
   no_grad(what, {x, state, weight, bias});
   same(what, "out_state", x, out, state.sizes(), x.scalar_type());
-  TORCH_CHECK_VALUE(!out.defined() || out.is_contiguous(), what, ": out_state must be contiguous");
+  TORCH_CHECK_VALUE(!out.defined() || out.size(0) == 0 || out.select(0, 0).is_contiguous(), what, ": rows of out_state must be dense");
   return conv_run(dense(x), whole(weight), whole(bias), rows_dense(state), reset, silu, true, out);
 }
 
@@ -256,6 +257,7 @@ std::tuple<Tensor, Tensor, Tensor> scan_run(const ScanIn &i, bool want, bool tra
   if (p.T > 1) ws = scratch(api.scan_ws(&p, 0), i.x);
   p.y = ptr(y);
   p.state_out = fptr(out_state);
+  if (out_state.defined()) p.state_out_sr = out_state.stride(0);
   p.checkpoints = fptr(ck);
   p.workspace = ptr(ws);
   p.workspace_bytes = ws.defined() ? ws.numel() : 0;
@@ -345,7 +347,7 @@ std::pair<Tensor, Tensor> selective_scan_step(const Tensor &x, const Tensor &dt,
   const ScanIn i = scan_check(what, x, dt, A, B, C, val(skip), val(z), val(dt_bias), state, val(reset), softplus);
   no_grad(what, {x, dt, A, B, C, i.skip, i.z, i.dt_bias, state});
   same(what, "out_state", x, out, state.sizes(), at::kFloat);
-  TORCH_CHECK_VALUE(!out.defined() || out.is_contiguous(), what, ": out_state must be contiguous");
+  TORCH_CHECK_VALUE(!out.defined() || out.size(0) == 0 || out.select(0, 0).is_contiguous(), what, ": rows of out_state must be dense");
   auto r = scan_run(i, true, false, out);
   return {std::get<0>(r), std::get<1>(r)};
 }

@@ -84,7 +84,7 @@ struct ActLayerArgs {
   int nseg;
   const float *W;     // [N, ldw] row-major (torch Linear.weight)
   int ldw;
-  const float *bias;  // [N]
+  const float *bias;  // [N] or null
   float *out;         // [rows, ldo]
   int ldo, N, rows, leaky;
   // Optional pre-layer (a first hidden layer over FEW input columns - the observation): every workgroup of the launch

@@ -259,6 +259,14 @@ typedef struct {
    * (parameter encoder.hidden_state repeated over the batch).  With the GRU, is_contiguous becomes its
    * cumulative product over t (a window counts up to its first break). */
   int32_t joiner_gru, gru_state_mode;
+  /* joiner_ssm = 1 (not with joiner_gru): a state-space block in the joiner's place, a design of this implementation (the reference has the MLP and
+   * the GRU only).  From the encoder features e [T, B, enc_features]:
+   *   (x, z) = e W_in^T + b_in;  x = causal_conv(x) (4 taps, SiLU);  (dt, B, C) = x W_sel^T;  y = scan(x, dt, -exp(A_log), B, C, skip, z, dt_bias);
+   *   state = SiLU(y Wg^T + bg) * (y Wu^T + bu)          (fdql_causal_conv, fdql_scan, fdql_gated; x, z [ssm_inner], B, C [ssm_state])
+   * with a reset wherever a window breaks (the steps behind a break start from zeros, so is_contiguous stays per step, no cumulative
+   * product).  gru_state_mode: 0 the windows start from zeros, 1 from batch.agent_state[0].  The carried state of a row (act(), agent_state)
+   * is the convolution's last 3 inputs [3, ssm_inner], then the scan's state [ssm_inner, ssm_state]: fdql_agent_state_floats(). */
+  int32_t joiner_ssm, ssm_inner, ssm_state;
   /* algorithm switches */
   int32_t distributional;           /* conf.use_distributional_sac                           */
   int32_t use_lowerbound;           /* conf.use_nStep_lowerbounds                            */
@@ -291,6 +299,9 @@ int64_t fdql_agent_arena_floats(const fdql_agent_t *agent, int32_t which);
 int32_t fdql_agent_tensor_info(const fdql_agent_t *agent, int32_t index, char *name, int32_t name_cap,
                                int32_t *arena, int64_t *offset_floats, int32_t *shape2);
 int64_t fdql_agent_workspace_bytes(const fdql_agent_t *agent);
+/* Floats of one row's carried state (act()'s agent_state / hidden_state, batch.agent_state): latent with the GRU joiner, 3 ssm_inner + ssm_inner *
+ * ssm_state with the state-space joiner, 0 with the feed-forward one. */
+int64_t fdql_agent_state_floats(const fdql_agent_t *agent);
 /* 1 when the pixel encoder's first layer runs on the implicit-GEMM kernel (csrc/conv.hip) and may therefore read the ring's
  * uint8 block in place (fdql_batch_t.obs_2d_slots); 0: the batch must carry the frames themselves. */
 int32_t fdql_agent_conv_reads_ring(const fdql_agent_t *agent);
@@ -311,8 +322,8 @@ typedef struct {
                                  (obs_2d_slots == NULL) or the ring's own block of the key (fdql_ring_key_ptr_u8) read in place  */
   const int32_t *obs_2d_slots;/* ... through one slot index per row, int32 [T,B] (fdql_ring_window_slots); needs
                                  fdql_agent_conv_reads_ring() != 0                                                               */
-  const float *agent_state;   /* [T,B,latent]: hidden state the actor had at each step (runner.py:157); read iff
-                                 joiner_gru && gru_state_mode == 1, row block t = 0 only (encoder.py:83-84)     */
+  const float *agent_state;   /* [T,B,state_floats]: hidden state the actor had at each step (runner.py:157); read iff
+                                 (joiner_gru || joiner_ssm) && gru_state_mode == 1, row block t = 0 only (encoder.py:83-84)     */
 } fdql_batch_t;
 
 #define FDQL_PHASE_ALL 0   /* loss + backward + Adam + polyak                               */
@@ -374,8 +385,8 @@ int fdql_agent_debug_ptr(fdql_agent_t *agent, const char *name, const float **de
  *   keyed by (seed, counter);
  *   action [rows, act_dim] (continuous) or [rows] action index as float (discrete) =
  *   exploit*mask + explore*!mask; log_prob [rows], explore_action, exploit_action: optional (the
- *   reference's `info` dict).  GRU joiner: agent_state [rows, latent] is the hidden state the runner carries
- *   (NULL = zeros) and hidden_state [rows, latent] receives the next one (encoder.py:72-76); both are NULL
+ *   reference's `info` dict).  GRU and state-space joiner: agent_state [rows, state_floats] is the hidden state the runner carries
+ *   (NULL = zeros) and hidden_state [rows, state_floats] receives the next one (encoder.py:72-76); both are NULL
  *   for the feed-forward joiner, whose hidden state is None in the reference's return triple.  workspace: caller-owned device scratch of at least
  *   fdql_agent_act_workspace_bytes(agent, rows) bytes, 16-byte aligned, private to this call
  *   stream (it may run beside fdql_agent_update on another stream; it then reads whatever mix of
@@ -432,7 +443,8 @@ int32_t fdql_agent_profile_update(fdql_agent_t *agent, const fdql_batch_t *batch
 
 /* y_t = f(bias + sum_{j<K} weight[:, K-1-j] * x_{t-j}), f = SiLU or identity, channel by channel; x_{t-j} counts as zero when a
  * reset lies in (t-j, t].  Inputs before step 0 come from state_in [R, K-1, D] (row stride state_in_sr, oldest first; NULL: zeros); state_out
- * [R, K-1, D] (or NULL) receives the last K-1 inputs (zeros for those before the last reset).  state_out may be state_in when T == 1.
+ * [R, K-1, D] (row stride state_out_sr; or NULL) receives the last K-1 inputs (zeros for those before the last reset).  state_out may be
+ * state_in, with the same stride, when T == 1.
  * Backward: dy [T, R, D] (strides dy_st, dy_sr) and dstate_out (or NULL) -> dx, dweight [D, K], dbias [D], dstate_in (each or NULL).                  */
 typedef struct {
   int32_t size, dtype;
@@ -446,6 +458,7 @@ typedef struct {
   const void *state_in;
   int64_t state_in_sr;
   void *y, *state_out;                /* forward                                                */
+  int64_t state_out_sr;
   const void *dy;                     /* backward                                               */
   int64_t dy_st, dy_sr;
   const void *dstate_out;             /* [R, K-1, D] dense                                      */
@@ -462,7 +475,8 @@ int fdql_causal_conv_backward(const fdql_causal_conv_t *p, void *stream);
  *   delta = softplus(dt_t + dt_bias)   (dt_t + dt_bias itself without dt_softplus)
  *   h     = exp(delta * A[d]) * h + delta * x_t * B_t[g]      (the first term dropped at a reset)
  *   y_t   = (C_t[g] . h + skip[d] * x_t) * SiLU(z_t)          (factors that are NULL left out)
- * state_in [R, D, N] (row stride state_in_sr, NULL: zeros), state_out [R, D, N] dense (or NULL; may be state_in when T == 1).
+ * state_in [R, D, N] (row stride state_in_sr, NULL: zeros), state_out [R, D, N] (row stride state_out_sr; or NULL; may be state_in, with the
+ * same stride, when T == 1).
  * checkpoints: fdql_scan_checkpoint_floats() floats that the forward call fills for the backward call of the same inputs (NULL
  * when there is none).  Backward: dy (strides dy_st, dy_sr) and dstate_out (or NULL) -> every gradient; those of optional inputs that are NULL may be NULL,
  * dstate_in always.                                                                                              */
@@ -482,6 +496,7 @@ typedef struct {
   int64_t state_in_sr;
   void *y;                            /* forward                                                */
   float *state_out;
+  int64_t state_out_sr;
   float *checkpoints;
   const void *dy;                     /* backward                                               */
   int64_t dy_st, dy_sr;

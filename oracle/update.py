@@ -64,6 +64,11 @@ class Spec:
     conv: Tuple[Tuple[int, int, int], ...] = ()   # per layer (out_channels, kernel, stride)
     gru: str = ""                 # "" = feed-forward joiner; else EncoderConf.JoinerModeEnum.gru with the latent-state
                                   # training mode "zero" | "learned" | "store" (encoder.py:40-42, 78-94)
+    # State-space joiner.  NO REFERENCE EXISTS for it: two input projections, a causal convolution of 4 taps, a selective scan
+    # gated by the second projection, a gated output layer.  "" = off, else the start state "zero" | "store".
+    ssm: str = ""
+    ssm_inner: int = 0            # channels (0: 2 enc_features)
+    ssm_state: int = 16           # states per channel
 
     @property
     def conv_shapes(self):        # per layer (Cin, H_in, W_in, Cout, k, s, H_out, W_out)
@@ -80,6 +85,10 @@ class Spec:
             return 0
         cs = self.conv_shapes
         return cs[-1][3] * cs[-1][6] * cs[-1][7] if cs else self.img[0] * self.img[1] * self.img[2]
+
+    @property
+    def ssm_dims(self):           # channels, states per channel
+        return self.ssm_inner or 2 * self.enc_features, self.ssm_state
 
     @property
     def enc_in(self):             # encoder.py:26-32 (+ the flattened conv features)
@@ -135,6 +144,12 @@ def net_shapes(spec: Spec, which: str):
             return [("encoder.joiner.weight_ih_l0", (3 * L, F_)), ("encoder.joiner.weight_hh_l0", (3 * L, L)),
                     ("encoder.joiner.bias_ih_l0", (3 * L,)), ("encoder.joiner.bias_hh_l0", (3 * L,)),
                     ("encoder.hidden_state", (L,))]
+        if spec.ssm:
+            (D, S), L, F_ = spec.ssm_dims, spec.latent, spec.enc_features
+            return [("encoder.joiner." + n, shape) for n, shape in (
+                ("in_proj.weight", (2 * D, F_)), ("in_proj.bias", (2 * D,)), ("conv.weight", (D, 4)), ("conv.bias", (D,)),
+                ("sel_proj.weight", (D + 2 * S, D)), ("dt_bias", (D,)), ("A_log", (D, S)), ("skip", (D,)),
+                ("gate_proj.weight", (L, D)), ("gate_proj.bias", (L,)), ("up_proj.weight", (L, D)), ("up_proj.bias", (L,)))]
         return mlp_shapes("encoder.joiner", spec.enc_features, spec.joint_hidden, spec.latent)
     if which in ("actor", "actor_target"):
         return mlp_shapes(f"actor_critic.{which}", spec.latent, spec.pi_hidden, spec.pi_out)
@@ -177,6 +192,13 @@ def init_params(spec: Spec, seed=0) -> Dict[str, Tensor]:
             p[name] = (torch.rand(shape, generator=g, dtype=torch.float32) * 2 - 1) * k
         elif name == "encoder.hidden_state":                       # encoder.py:42, 117: torch.rand(out_features)
             p[name] = torch.rand(shape, generator=g, dtype=torch.float32)
+        elif name == "encoder.joiner.A_log":
+            p[name] = torch.arange(1, shape[1] + 1, dtype=torch.float32).log().expand(shape).clone()
+        elif name == "encoder.joiner.skip":
+            p[name] = torch.ones(shape)
+        elif name == "encoder.joiner.dt_bias":                     # softplus(dt_bias) log-uniform in 0.001 .. 0.1
+            step = torch.exp(torch.rand(shape, generator=g, dtype=torch.float32) * math.log(100.0) + math.log(1e-3))
+            p[name] = step + torch.log(-torch.expm1(-step))
         elif name.endswith("weight"):
             fan_out, fan_in = shape
             a = math.sqrt(6.0 / (fan_in + fan_out))
@@ -259,9 +281,34 @@ def gru_cell(p, x_t, h):
     return (1 - z) * n + z * h
 
 
-def encoder(p, spec: Spec, xp, h0=None, return_hidden=False):
+def ssm_joiner(p, spec: Spec, e, h0, reset):
+    """State-space joiner over [T, B, F] features; h0 [B, 3 D + D S] (the convolution's last inputs, then the scan's state; None: zeros);
+    reset [T, B]: the step starts from zeros."""
+    w = lambda name: p["encoder.joiner." + name]
+    D, S = spec.ssm_dims
+    B = e.shape[1]
+    h0 = torch.zeros(B, 3 * D + D * S, dtype=e.dtype) if h0 is None else h0.to(e.dtype)
+    win, h = h0[:, :3 * D].reshape(B, 3, D), h0[:, 3 * D:].reshape(B, D, S)
+    u, z = F.linear(e, w("in_proj.weight"), w("in_proj.bias")).chunk(2, -1)
+    A = -w("A_log").exp()
+    ys = []
+    for t in range(e.shape[0]):
+        keep = ~reset[t].view(B, 1, 1)
+        full = torch.cat([win * keep, u[t][:, None]], 1)                                   # [B, 4, D], oldest first
+        win, h = full[:, 1:], h * keep
+        x = F.silu((full * w("conv.weight").t()).sum(1) + w("conv.bias"))
+        dt, Bt, Ct = F.linear(x, w("sel_proj.weight")).split([D, S, S], -1)
+        dt = F.softplus(dt + w("dt_bias"))
+        h = torch.exp(dt[..., None] * A) * h + (dt * x)[..., None] * Bt[:, None]
+        ys.append(((h * Ct[:, None]).sum(-1) + w("skip") * x) * F.silu(z[t]))
+    y = torch.stack(ys)
+    out = F.silu(F.linear(y, w("gate_proj.weight"), w("gate_proj.bias"))) * F.linear(y, w("up_proj.weight"), w("up_proj.bias"))
+    return out, torch.cat([win.reshape(B, -1), h.reshape(B, -1)], 1)
+
+
+def encoder(p, spec: Spec, xp, h0=None, return_hidden=False, reset=None):
     """encoder.py:52-67: obs MLP, then the feed-forward joiner or (spec.gru) one GRU layer scanned over the
-    leading (time) axis from ``h0`` [B, L] (zeros when None)."""
+    leading (time) axis from ``h0`` [B, L] (zeros when None); spec.ssm: the state-space joiner, restarted where ``reset`` [T, B]."""
     parts = [xp["obs_1d"]] if spec.obs else []
     if spec.goal:
         parts += [xp["achieved_goal"], xp["desired_goal"]]
@@ -269,6 +316,9 @@ def encoder(p, spec: Spec, xp, h0=None, return_hidden=False):
         parts.append(conv_features(p, spec, xp["obs_2d"]))
     x = torch.cat(parts, dim=-1)
     e = skip_head_mlp(p, "encoder.visible_layer_encoders.obs_1d", x, len(spec.enc_hidden))
+    if spec.ssm:
+        y, h = ssm_joiner(p, spec, e, h0, torch.zeros(e.shape[:2], dtype=torch.bool) if reset is None else reset)
+        return (y, h) if return_hidden else y
     if not spec.gru:
         return skip_head_mlp(p, "encoder.joiner", e, len(spec.joint_hidden))
     h = h0 if h0 is not None else torch.zeros(e.shape[1:-1] + (spec.latent,), dtype=e.dtype)
@@ -328,7 +378,7 @@ def act(p, spec: Spec, xp, noise):
     supplied by the caller.  Returns (action, log_prob, explore_action, exploit_action)."""
     with torch.no_grad():
         hidden = None
-        if spec.gru:   # forward_eval: one GRU step from xp["agent_state"] (encoder.py:72-76; runner.py:103-106)
+        if spec.gru or spec.ssm:   # forward_eval: one GRU step from xp["agent_state"] (encoder.py:72-76; runner.py:103-106)
             s, hidden = encoder(p, spec, {k: v.unsqueeze(0) for k, v in xp.items()}, h0=xp.get("agent_state"),
                                 return_hidden=True)
             s = s[0]
@@ -343,7 +393,7 @@ def act(p, spec: Spec, xp, noise):
             exploit = torch.tanh(torch.chunk(logits, 2, dim=-1)[0])   # gaussian_mlp.py:38 tanh(mean)
         mask = xp["exploit_mask"]
         action = (exploit * mask) + (explore * torch.logical_not(mask))
-        return (action, logp, explore, exploit, hidden) if spec.gru else (action, logp, explore, exploit)
+        return (action, logp, explore, exploit, hidden) if spec.gru or spec.ssm else (action, logp, explore, exploit)
 
 
 # ---------------------------------------------------------------------------------------
@@ -376,7 +426,11 @@ def losses(p, spec: Spec, xp, noise_target, noise_actor, alpha):
             h0 = xp["agent_state"][0]
         elif spec.gru == "learned":
             h0 = p["encoder.hidden_state"].view(1, -1).repeat(contig.shape[1], 1)
-    state = encoder(p, spec, xp, h0=h0)                                    # :213
+    reset = None
+    if spec.ssm:   # the state restarts behind every break, the rows stay valid
+        reset = torch.cat([torch.zeros_like(contig[:1]), ~contig]).squeeze(-1)
+        h0 = xp["agent_state"][0] if spec.ssm == "store" else None
+    state = encoder(p, spec, xp, h0=h0, reset=reset)                       # :213
     s_cur, s_nxt = state[:-1], state[1:]                                   # :251-258
     with torch.no_grad():                                                  # q_loss target
         a_n, logp_n = policy(p, spec, "actor_target", s_nxt, noise_target)

@@ -541,3 +541,29 @@ def test_second_derivative_is_refused(dev, seq):
     g, = torch.autograd.grad(seq.gated_linear(x, w, w).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("D,N,pad", [(64, 16, 0), (37, 5, 0), (64, 16, 1), (40, 64, 4)])
+@pytest.mark.parametrize("inplace", [False, True])
+def test_states_as_columns_of_one_row(dev, seq, D, N, pad, inplace):
+    """Both states of a row side by side in one buffer (rows of 3 D + D N + pad floats): read from and written to strided views, in place and
+    into another buffer; the columns between and behind stay as they were; equal to dense states bit for bit."""
+    R, W = 5, 3 * D + D * N + pad
+    g = _gen(D + N)
+    buf = torch.randn(R, W, generator=g).to(dev)
+    out = buf if inplace else torch.full((R, W), 7.0, device=dev)
+    views = lambda t: (t[:, :3 * D].view(R, 3, D), t[:, 3 * D:3 * D + D * N].view(R, D, N))  # noqa: E731
+    x, w = torch.randn(R, D, generator=g).to(dev), torch.randn(D, 4, generator=g).to(dev)
+    A, bc = -torch.rand(D, N, generator=g).to(dev), torch.randn(2, R, N, generator=g).to(dev)
+    (cs, hs), (co, ho) = views(buf), views(out)
+    rest = out[:, 3 * D + D * N:].clone()
+    want_y, want_c = seq.causal_conv_step(x, cs.clone(), w)
+    want_v, want_h = seq.selective_scan_step(want_y, x, A, bc[0], bc[1], hs.contiguous().clone())
+    y, c = seq.causal_conv_step(x, cs, w, out_state=co)
+    v, h = seq.selective_scan_step(y, x, A, bc[0], bc[1], hs, out_state=ho)
+    assert c.data_ptr() == co.data_ptr() and h.data_ptr() == ho.data_ptr()
+    for got, want in ((y, want_y), (co, want_c), (ho, want_h)):
+        assert torch.equal(got, want)
+    terms = (want_h.double() * bc[1].double()[:, None]).abs().sum(-1)
+    assert ((v.double() - want_v.double()).abs() <= 2.02 * (N + 1) * 2.0 ** -24 * terms).all()
+    assert torch.equal(out[:, 3 * D + D * N:], rest)

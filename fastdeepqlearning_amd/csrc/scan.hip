@@ -396,18 +396,28 @@ __global__ __launch_bounds__(256) void k_scan_combine(Args a) {
     if (REV) cur = p.dstate_out ? p.dstate_out[((int64_t)r * p.D + d) * p.N + n] : 0.f;
     else cur = p.state_in ? p.state_in[(int64_t)r * p.state_in_sr + (int64_t)d * p.N + n] : 0.f;
   }
-  for (int k = 0; k < a.nseg; ++k) {
-    const int seg = REV ? a.nseg - 1 - k : k;
-    float *at = a.seg_h + seg * per + i;
-    if (k < a.nseg - 1) {
-      const float own = *at, sum = a.seg_d[((int64_t)seg * p.R * p.G * a.tpg + blk) * 64 + lane];
-      *at = cur;
-      const float e = __builtin_amdgcn_exp2f(sum * A);
-      cur = a.seg_f[(int64_t)seg * p.R + r] ? own : fmaf(e, cur, own);
-    } else {
-      *at = cur;
+  // AHEAD segments' values are read together: one by one, each read behind the last one's store, 64 segments took 24 us
+  constexpr int AHEAD = 16;
+  const auto seg_of = [&](int k) { return REV ? a.nseg - 1 - k : k; };
+  for (int k0 = 0; k0 < a.nseg - 1; k0 += AHEAD) {
+    float own[AHEAD], sum[AHEAD];
+    int any[AHEAD];
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      const int64_t seg = seg_of(min(k0 + q, a.nseg - 2));
+      own[q] = a.seg_h[seg * per + i];
+      sum[q] = a.seg_d[(seg * p.R * p.G * a.tpg + blk) * 64 + lane];
+      any[q] = a.seg_f[seg * p.R + r];
+    }
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      if (k0 + q < a.nseg - 1) {
+        a.seg_h[seg_of(k0 + q) * per + i] = cur;
+        cur = any[q] ? own[q] : fmaf(__builtin_amdgcn_exp2f(sum[q] * A), cur, own[q]);
+      }
     }
   }
+  a.seg_h[seg_of(a.nseg - 1) * per + i] = cur;
 }
 
 // --------------------------------------------------------------------------------------------------------------- backward

@@ -305,7 +305,13 @@ __global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
 // The DMA writes lanes in order, so the swizzles against bank conflicts are applied to the addresses that lanes read from memory.  Chunks past
 // an edge come from a block of zeros.
 // Shapes: 256 x 256 (KS 32, 4 slices) and 128 x 256 (KS 64, 3 slices) with one workgroup per CU for 16-bit types and many tiles; 64 x 128 for
-// few tiles and for float, whose matrix instructions take so long that the ring needs only two slices and three workgroups share a CU.
+// few tiles; 64 x 128 and 128 x 128 for float, whose matrix instructions take so long that the ring needs only two slices and three or two
+// workgroups share a CU.
+// Measured (bf16, 8192 rows, F 4096): forward 502 us at D 4096 = 1095 TFLOP/s, 165 at D 1024 (about 45 us of it outside the contraction: filling
+// the ring, activations, stores); float 12800 x 2048 x 1024 115 TFLOP/s.  What bounds the 16-bit loop is the way from L2 into LDS: with every
+// request at one address it takes 80% of the time, with none 76%, without LDS reads 97%; 128 x 256 tiles, which need half as much again per
+// product, lose a third to it.  Splitting each slice between two groups of four waves (a third fewer LDS reads) gave 172 us instead of 182 for dx
+// and lost as much on the weight gradients.
 __device__ const v4i g_zeros = {0, 0, 0, 0};
 
 template <typename T, int BM, int BN>
@@ -446,44 +452,53 @@ __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
 
   v16f acc[MT][NT];
   clear(acc);
-  // (s_barrier by itself: __syncthreads would wait for every DMA in flight.  A wave's LDS reads are done when it arrives: their products are issued)
+  // (s_barrier by itself: __syncthreads would wait for every DMA in flight)
   int issued = 0;
   for (; issued < min(NBUF - 1, steps); ++issued) fetch(issued, issued, 0, 1);
   if (issued == NBUF - 1) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((NBUF - 2) * (NA + NB)) : "memory");
   else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  // The next fragments are on their way while these are multiplied, across slices too: the wait and the barrier stand in front of a slice's
+  // last products (behind them, every wave would start the next slice with the latency of its LDS reads).
+  constexpr int PIECES = NBUF == 2 ? KSTEPS - 1 : KSTEPS;                 // two slices: the next one must be on its way whole by then
+  constexpr int EARLY = ((KSTEPS - 1) * (NA + NB) + PIECES - 1) / PIECES; // requests of a slice that go out before the wait
+  constexpr int FLYING = NBUF == 2 ? 0 : (NBUF - 3) * (NA + NB) + EARLY;  // ... and may be under way behind it
   int buf = 0;
+  v4i ra[2][MT], rb[2][NT];
+  const auto frags = [&](int of, int kk) {
+    const char *ta = lds + of * (ABYTES + BBYTES), *tb = ta + ABYTES;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      if constexpr (MODE == FWD) rb[kk & 1][j] = row_frag(tb, wn * 64 + j * 32, kk);
+      else rb[kk & 1][j] = col_frag(tb + at_b[j], kk, BCols::RB);
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+      if constexpr (MODE == DW) ra[kk & 1][i] = col_frag(ta + at_a[i], kk, ACols::RB);
+      else ra[kk & 1][i] = row_frag(ta, wm * (BM / 2) + i * 32, kk);
+    }
+  };
+  if (steps > 0) frags(0, 0);
   for (int step = 0; step < steps; ++step) {
     const bool more = step + NBUF - 1 < steps;
-    const char *ta = lds + buf * (ABYTES + BBYTES), *tb = ta + ABYTES;
-    // the next fragments are on their way while these are multiplied
-    v4i ra[2][MT], rb[2][NT];
-    const auto frags = [&](int kk) {
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        if constexpr (MODE == FWD) rb[kk & 1][j] = row_frag(tb, wn * 64 + j * 32, kk);
-        else rb[kk & 1][j] = col_frag(tb + at_b[j], kk, BCols::RB);
-      }
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        if constexpr (MODE == DW) ra[kk & 1][i] = col_frag(ta + at_a[i], kk, ACols::RB);
-        else ra[kk & 1][i] = row_frag(ta, wm * (BM / 2) + i * 32, kk);
-      }
-    };
-    frags(0);
+    const int next = buf == NBUF - 1 ? 0 : buf + 1;
 #pragma unroll
     for (int kk = 0; kk < KSTEPS; ++kk) {
-      if (kk + 1 < KSTEPS) frags(kk + 1);
+      if (kk + 1 < KSTEPS) {
+        frags(buf, kk + 1);
+      } else if (step + 1 < steps) {
+        if (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(FLYING) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        frags(next, 0);
+      }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int j = 0; j < NT; ++j) Mma<T>::mma32(acc[i][j], ra[kk & 1][i], rb[kk & 1][j]);
       __builtin_amdgcn_sched_barrier(0);
-      if (more) fetch(step + NBUF - 1, buf ? buf - 1 : NBUF - 1, kk, KSTEPS);   // into the slice that the last step was done with
+      if (more) fetch(step + NBUF - 1, buf ? buf - 1 : NBUF - 1, kk, PIECES);   // into the slice that the last step was done with
     }
-    if (more) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"((NBUF - 2) * (NA + NB)) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    buf = buf == NBUF - 1 ? 0 : buf + 1;
+    buf = next;
   }
   store_tile<T, MODE, MT, BM, BN>(a, acc, m0, n0, f0, wm, wn, which, ks);
 }
@@ -625,13 +640,19 @@ struct Shape {
   int64_t tiles_m, tiles_n;
 };
 constexpr int CUS = 256;
-Shape shape_of(bool wide, int64_t rows, int64_t cols, int tile_of_256, int copies) {     // tile_of_256: columns that a 256-wide tile covers
+enum Choice { SMALL, WIDE, FLOAT };        // which tiles there are: 64 x 128 alone; and 128, 256 x 256 of 16-bit types; and 128 x 128 of float
+Shape shape_of(Choice choice, int64_t rows, int64_t cols, int tile_of_256, int copies) {     // tile_of_256: columns that a 256-wide tile covers
   const auto tiles = [&](int bm, int bn) { return (rows + bm - 1) / bm * ((cols + tile_of_256 * bn / 256 - 1) / (tile_of_256 * bn / 256)); };
   Shape s = {64, 128, 0, 0};
-  if (wide && tiles(128, 256) * copies >= 192) {
+  const auto rounds = [&](int64_t n) { return (n * copies + CUS - 1) / CUS; };      // tiles on the CU that has most
+  // float: two workgroups of 128 x 128 on a CU or three of 64 x 128, both near the rate of the matrix units while they share it and slow when the
+  // last one is alone: the larger tile (fewer bytes through LDS) where it needs no more row-steps of the card.  Forward at D 512, F 256:
+  // 12800 rows 79 us -> 70 (800 tiles or 400), 8192 rows 42 either way; where it needs more, 20000 rows, it would take 113 us instead of 101.
+  if (choice == FLOAT && tiles(128, 128) >= CUS && 2 * rounds(tiles(128, 128)) <= rounds(tiles(64, 128))) s.bm = 128;
+  if (choice == WIDE && tiles(128, 256) * copies >= 192) {
     // one workgroup per CU: the tile that needs fewer row-steps of the card, the larger one where they need the same
     s.bn = 256;
-    s.bm = (tiles(256, 256) * copies + CUS - 1) / CUS * 2 <= (tiles(128, 256) * copies + CUS - 1) / CUS ? 256 : 128;
+    s.bm = rounds(tiles(256, 256)) * 2 <= rounds(tiles(128, 256)) ? 256 : 128;
   }
   s.tiles_m = (rows + s.bm - 1) / s.bm;
   s.tiles_n = (cols + tile_of_256 * s.bn / 256 - 1) / (tile_of_256 * s.bn / 256);
@@ -670,7 +691,7 @@ hipError_t launch_mma(const Args &a, dim3 grid, hipStream_t s) {
 template <typename T, int MODE>
 hipError_t product(Args a, int64_t rows, int64_t cols, bool aligned, hipStream_t s) {
   const int copies = MODE == DW ? 2 : 1;
-  const Shape q = shape_of(sizeof(T) == 2 && aligned, rows, cols, MODE == FWD ? 128 : 256, copies);
+  const Shape q = shape_of(!aligned ? SMALL : sizeof(T) == 2 ? WIDE : MODE == DW ? SMALL : FLOAT, rows, cols, MODE == FWD ? 128 : 256, copies);
   a.tiles_m = (int)q.tiles_m;
   a.tiles_n = (int)q.tiles_n;
   if (MODE == DW && q.bn == 256) a.ksplit = 1, a.kper = (int)((a.p.M + 63) / 64 * 64);
@@ -682,6 +703,9 @@ hipError_t product(Args a, int64_t rows, int64_t cols, bool aligned, hipStream_t
   if constexpr (sizeof(T) == 2) {
     if (q.bm == 256) return launch_mma<T, MODE, 256, 256>(a, grid, s);
     if (q.bm == 128) return launch_mma<T, MODE, 128, 256>(a, grid, s);
+  }
+  if constexpr (sizeof(T) == 4 && MODE != DW) {
+    if (q.bm == 128) return launch_mma<T, MODE, 128, 128>(a, grid, s);
   }
   return launch_mma<T, MODE, 64, 128>(a, grid, s);
 }
@@ -718,7 +742,7 @@ hipError_t bwd(const fdql_gated_t &p, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && p.dx) e = product<T, DX>(a, p.M, p.D, p.D % E == 0 && al16(p.w_gate) && al16(p.w_up), s);
   const bool w = p.dw_gate && p.dw_up, vec = p.D % E == 0 && p.x_sr % E == 0 && al16(p.x);
-  if (w && shape_of(sizeof(T) == 2 && vec, p.F, p.D, 256, 2).bn == 256) a.ksplit = 1;
+  if (w && shape_of(sizeof(T) == 2 && vec ? WIDE : SMALL, p.F, p.D, 256, 2).bn == 256) a.ksplit = 1;
   if (e == hipSuccess && w) e = product<T, DW>(a, p.F, p.D, vec, s);
   const bool sum_w = w && a.ksplit > 1;
   if (e == hipSuccess && (sum_w || p.db_gate || p.db_up)) {

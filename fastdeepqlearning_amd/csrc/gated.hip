@@ -32,8 +32,8 @@ enum Mode { FWD, DX, DW };
 
 struct Args {
   fdql_gated_t p;
-  int Fp;                          // row length of d (F rounded up to 8)
-  void *d;                         // [2][M][Fp] dg, du in the operand type, zeros behind column F
+  int Fp, parts;                   // row length of d (F rounded up to 8); 2: d in two parts whose sum has twice the digits
+  void *d;                         // [2][parts][M][Fp] dg, du in the operand type, zeros behind column F
   float *colsum;                   // [row blocks][2][F]
   float *slab;                     // [ksplit][2][F][D] when ksplit > 1
   int ksplit, kper;                // DW: slices of the rows and their length (a multiple of the K slice)
@@ -227,6 +227,11 @@ __device__ __forceinline__ void clear(v16f (&acc)[MT][2]) {
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 }
 
+// The backward products pass over their contraction once for every part of d, DX for the gate's side, then the up side's.
+template <int MODE>
+__device__ __forceinline__ int passes_of(const Args &a) { return MODE == FWD ? 1 : MODE == DX ? 2 * a.parts : a.parts; }
+__device__ __forceinline__ int pass_of(int step, int len) { return (step >= len) + (step >= 2 * len) + (step >= 3 * len); }
+
 // Float sums over a long contraction: RUN slices (512 products) at a time, the runs added up apart, so that the rounding error grows with the run's
 // length and their number instead of the whole length (dx at F 2000: 1.2e-6 of its norm in one chain).  16-bit results round at 2^-12
 // or 2^-9 and keep one chain.
@@ -275,9 +280,9 @@ __global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
   const int64_t M = p.M, D = p.D, F = p.F, m0 = (int64_t)tm * BM, f0 = (int64_t)tn * (BN / 2), n0 = (int64_t)tn * BN;
   const int which = MODE == DW ? blockIdx.y : 0, ks = MODE == DW ? blockIdx.z : 0;
   const T *x = reinterpret_cast<const T *>(p.x), *wg = reinterpret_cast<const T *>(p.w_gate), *wu = reinterpret_cast<const T *>(p.w_up);
-  const T *dd = reinterpret_cast<const T *>(a.d);
+  const T *dd = reinterpret_cast<const T *>(a.d) + (MODE == DW ? which * a.parts * M * a.Fp : 0);
   const int64_t kbeg = MODE == DW ? (int64_t)ks * a.kper : 0, kend = MODE == FWD ? D : MODE == DX ? F : min(M, kbeg + a.kper);
-  const int half = (int)((kend - kbeg + BK - 1) / BK), steps = MODE == DX ? 2 * half : half;     // DX: the gate's pass, then the up side's
+  const int half = (int)((kend - kbeg + BK - 1) / BK), steps = passes_of<MODE>(a) * half;
 
   Flight<2> fa;
   Flight<4> fb;
@@ -290,14 +295,15 @@ __global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
         return f < F ? (n & 32 ? wu : wg) + f * D : (const T *)nullptr;
       }, k0, D);
     } else if constexpr (MODE == DX) {
-      const int up = step >= half;
-      const int64_t k0 = (int64_t)(step - up * half) * BK;
-      const T *src = dd + up * M * a.Fp;
+      const int pass = pass_of(step, half), up = a.parts == 2 ? pass >> 1 : pass;
+      const int64_t k0 = (int64_t)(step - pass * half) * BK;
+      const T *src = dd + pass * M * a.Fp;
       fetch_rows<T>(fa, [&](int n) { return m0 + n < M ? src + (m0 + n) * a.Fp : (const T *)nullptr; }, k0, F);
       fetch_cols<T>(fb, up ? wu : wg, D, k0, F, n0, D);
     } else {
-      const int64_t k0 = kbeg + (int64_t)step * BK;
-      fetch_cols<T>(fa, dd + which * M * a.Fp, a.Fp, k0, kend, m0, F);
+      const int pass = pass_of(step, half);
+      const int64_t k0 = kbeg + (int64_t)(step - pass * half) * BK;
+      fetch_cols<T>(fa, dd + pass * M * a.Fp, a.Fp, k0, kend, m0, F);
       fetch_cols<T>(fb, x, p.x_sr, k0, kend, n0, D);
     }
   };
@@ -402,10 +408,10 @@ __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
   const int64_t M = p.M, D = p.D, F = p.F, m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN, f0 = (int64_t)tn * (BN / 2);
   const int which = MODE == DW ? blockIdx.y : 0, ks = MODE == DW ? blockIdx.z : 0;
   const T *x = reinterpret_cast<const T *>(p.x), *wg = reinterpret_cast<const T *>(p.w_gate), *wu = reinterpret_cast<const T *>(p.w_up);
-  const T *dd = reinterpret_cast<const T *>(a.d) + which * M * a.Fp;
-  // contraction [kbeg, K) of one pass; DX makes two, gate and up
+  const T *dd = reinterpret_cast<const T *>(a.d) + which * a.parts * M * a.Fp;
+  // contraction [kbeg, K) of one pass
   const int64_t kbeg = MODE == DW ? (int64_t)ks * a.kper : 0, K = MODE == FWD ? D : MODE == DX ? a.Fp : min(M, kbeg + a.kper);
-  const int half = (int)((K - kbeg + KS - 1) / KS), steps = MODE == DX ? 2 * half : half;
+  const int half = (int)((K - kbeg + KS - 1) / KS), steps = passes_of<MODE>(a) * half;
 
   // where this lane's chunks come from: an element offset from the operand's start for slice 0, and the chunk's place in the contraction
   int64_t oa[NA], ob[NB];
@@ -445,10 +451,10 @@ __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
   // piece `piece` of `pieces` of a slice's DMA (a wave is held up while its requests are taken: in one go, with the other waves', that left the
   // matrix unit idle for a quarter of a step)
   const auto fetch = [&](int step, int buf, int piece, int pieces) {
-    const int up = MODE == DX && step >= half;
-    const int64_t k0 = kbeg + (int64_t)(step - up * half) * KS;
+    const int pass = MODE == FWD ? 0 : pass_of(step, half), up = MODE == DX ? (a.parts == 2 ? pass >> 1 : pass) : 0;
+    const int64_t k0 = kbeg + (int64_t)(step - pass * half) * KS;
     const unsigned la = lds_addr(lds) + buf * (ABYTES + BBYTES) + wave * NA * 1024, lb = lds_addr(lds) + buf * (ABYTES + BBYTES) + ABYTES + wave * NB * 1024;
-    const T *pa = MODE == FWD ? x + k0 : MODE == DX ? dd + up * M * a.Fp + k0 : dd + k0 * a.Fp;
+    const T *pa = MODE == FWD ? x + k0 : MODE == DX ? dd + pass * M * a.Fp + k0 : dd + pass * M * a.Fp + k0 * a.Fp;
     const int64_t kx = k0 * (MODE == DX ? D : p.x_sr);
 #pragma unroll
     for (int q = 0; q < NA + NB; ++q) {
@@ -609,6 +615,12 @@ __global__ __launch_bounds__(256) void k_gated_rows(Args a) {
   }
 }
 
+// what rounding v to its first part left over (nothing where that overflowed)
+template <typename T>
+__device__ __forceinline__ T rest_of(float v, T part) {
+  const float p = to_f(part);
+  return from_f<T>(fabsf(p) < INFINITY ? v - p : 0.f);
+}
 // dg, du of 64 columns x RB rows and their sums over those rows.
 constexpr int RB = 128;
 template <typename T>
@@ -633,8 +645,13 @@ __global__ __launch_bounds__(256) void k_gated_grad(Args a) {
       }
       sg += dg;
       su += du;
-      d[m * a.Fp + f] = from_f<T>(dg);
-      d[(M + m) * a.Fp + f] = from_f<T>(du);
+      const T hg = from_f<T>(dg), hu = from_f<T>(du);
+      d[m * a.Fp + f] = hg;
+      d[(a.parts * M + m) * a.Fp + f] = hu;
+      if (a.parts == 2) {
+        d[(M + m) * a.Fp + f] = rest_of(dg, hg);
+        d[(3 * M + m) * a.Fp + f] = rest_of(du, hu);
+      }
     }
   }
   if (wave) {
@@ -700,13 +717,18 @@ Shape shape_of(Choice choice, int64_t rows, int64_t cols, int tile_of_256, int c
   return s;
 }
 
+// Rounding d to 16 bits adds as much to the gradients' error as rounding the results does: sqrt(2) of it over many elements, more by chance over few.
+// So small problems keep d in two parts, which puts a second pass into products that their launches dominate; large ones would
+// pay for it (8192 x 1024 x 4096: twice 350 us).
 struct Plan {
-  int Fp, ksplit, kper;
+  int Fp, parts, ksplit, kper;
   int64_t rblocks;
 };
 Plan plan_of(const fdql_gated_t &p) {
   Plan q;
   q.Fp = (p.F + 7) / 8 * 8;
+  const int64_t few = std::min((int64_t)p.F * p.D, std::min(p.M * p.F, p.M * p.D));
+  q.parts = p.dtype != FDQL_F32 && few < 8192 && p.M * p.F <= 1 << 20 ? 2 : 1;
   q.rblocks = (p.M + RB - 1) / RB;
   // rows split for the 64 x 128 tiles of the weight gradients (larger tiles are chosen where there are enough of them): three workgroups
   // per CU, at least 256 rows each
@@ -771,9 +793,10 @@ hipError_t bwd(const fdql_gated_t &p, hipStream_t s) {
   Args a = {};
   a.p = p;
   a.Fp = q.Fp;
+  a.parts = q.parts;
   char *ws = reinterpret_cast<char *>(p.workspace);
   a.d = ws;
-  ws += up16(2 * p.M * q.Fp * (int64_t)sizeof(T));
+  ws += up16(2 * q.parts * p.M * q.Fp * (int64_t)sizeof(T));
   a.colsum = reinterpret_cast<float *>(ws);
   ws += up16(q.rblocks * 2 * p.F * 4);
   a.slab = reinterpret_cast<float *>(ws);
@@ -800,7 +823,7 @@ int64_t gated_workspace_bytes(const fdql_gated_t &p, bool backward) {
   if (!backward) return 0;
   const Plan q = plan_of(p);
   const int64_t esz = p.dtype == FDQL_F32 ? 4 : 2;
-  return up16(2 * p.M * q.Fp * esz) + up16(q.rblocks * 2 * p.F * 4) + (q.ksplit > 1 ? (int64_t)q.ksplit * 2 * p.F * p.D * 4 : 0);
+  return up16(2 * q.parts * p.M * q.Fp * esz) + up16(q.rblocks * 2 * p.F * 4) + (q.ksplit > 1 ? (int64_t)q.ksplit * 2 * p.F * p.D * 4 : 0);
 }
 hipError_t gated_fwd_launch(const fdql_gated_t &p, hipStream_t s) {
   return p.dtype == FDQL_F32 ? fwd<float>(p, s) : p.dtype == FDQL_BF16 ? fwd<bf16_t>(p, s) : fwd<f16_t>(p, s);

@@ -567,3 +567,27 @@ def test_states_as_columns_of_one_row(dev, seq, D, N, pad, inplace):
     terms = (want_h.double() * bc[1].double()[:, None]).abs().sum(-1)
     assert ((v.double() - want_v.double()).abs() <= 2.02 * (N + 1) * 2.0 ** -24 * terms).all()
     assert torch.equal(out[:, 3 * D + D * N:], rest)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("M,D,F", [(1, 358, 316), (3, 61, 22), (5, 64, 64), (40, 17, 19), (473, 42, 18), (1417, 48, 16), (16, 18, 98), (9, 800, 112), (200, 8, 8)])
+@pytest.mark.parametrize("kind", ["silu", "gelu", "sigmoid"])
+def test_gated_small_gradients_round_once(dev, seq, M, D, F, kind, dtype):
+    """Few values: the gradients in front of the products are kept in two 16-bit parts.  Two parts leave at most u^2 of a value (u: half a step;
+    the second part's own rounding; fp16's smallest step, 2^-24, bounds it from below), the float products and the activation's slope a few
+    dozen 2^-24 of the terms' magnitudes, and the result is rounded once: in one part the terms themselves would be off by u."""
+    g = _gen(M + D + F)
+    x, wg, wu = torch.randn(M, D, generator=g), torch.randn(F, D, generator=g) * D ** -0.5, torch.randn(F, D, generator=g) * D ** -0.5
+    dy = torch.randn(M, F, generator=g)
+    x, wg, wu, dy = (t.to(dtype) for t in (x, wg, wu, dy))
+    leaves = [t.to(dev).requires_grad_() for t in (x, wg, wu)]
+    got = torch.autograd.grad(seq.gated_linear(*leaves, activation=kind), leaves, dy.to(dev))
+    o = osq.gated_linear(x, wg, wu, None, None, kind, dy)
+    u, e = torch.finfo(dtype).eps / 2, 2.0 ** -24
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0
+    for name, have, n, other in (("dx", got[0], 2 * F, torch.stack([wg, wu])), ("dw_gate", got[1], M, x), ("dw_up", got[2], M, x)):
+        want = o[name]
+        exact = o["r_" + name] * (1.01 * u * u + (2 * n + 32) * e) + o["e_" + name] * (2 * D + 32) * e + tiny * n * float(other.abs().max())
+        bound = (want.abs() + exact) * u * 1.01 + exact + tiny
+        off = (have.cpu().double() - want).abs()
+        assert (off <= bound).all(), (name, float((off / bound.clamp_min(1e-300)).max()))

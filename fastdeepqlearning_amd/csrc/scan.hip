@@ -2,18 +2,21 @@
 //
 //   delta_t = softplus(dt_t + bias),  h_t[n] = e^(delta_t A[n]) h_{t-1}[n] + delta_t x_t B_t[n],  y_t = (C_t . h_t + skip x_t) SiLU(z_t)
 //
-// Layout.  A wave owns CW = 64 / S channels of one row and walks the time axis: lane = s * CW + c holds the NL states
-// [s NL, s NL + NL) of channel c in registers, so the sum over n stays in a lane (S = 1) or crosses S lanes, every x / dt / z / y access
-// is a run of consecutive channels, and B_t, C_t are the same for the whole wave: they pass through a small LDS tile of TS
-// steps and are read back as broadcasts.  Waves of the forward kernels share nothing, so there is no barrier in them.
-// Decays are e^(delta A) = exp2((delta log2 e) A): one multiply and one v_exp_f32 per state and step, which is what bounds the
-// kernels at N >= 16 (about 28 cycles of a SIMD per 64 states and step forward, 60 backward).
+// Layout.  A wave owns 16 channels of one row and walks the time axis: four neighbouring lanes share a channel, lane = 4 c + s holds the NL
+// states [s NL, s NL + NL) of channel c in registers (NL 2, 4, 8, 16 for up to 8, 16, 32, 64 states).  The sum over n crosses a quad of lanes, and
+// what a step has to do beside its states (loads, softplus, gate, store) is dealt to the quad, two of a tile's eight steps each.  B_t and
+// C_t are the same for the whole wave: they pass through a small LDS tile of eight steps and are read back as broadcasts.  The next tile's
+// reads are under way while one is computed.  Waves of the forward kernels share nothing, so there is no barrier in them.
+// Decays are e^(delta A) = exp2((delta log2 e) A): one multiply and one v_exp_f32 per state and step.  Vector instructions bound the kernels:
+// they are issued in 75 to 82% of all cycles (forward at N 16: five per state and step, of which the power takes four times as long, and
+// some 150 per tile for the rest; backward 18).  Measured: float 50 x 256 x 512, N 16: forward 47 us (213 MB with the checkpoints would take 41),
+// backward 130; bf16 prompt 16383 x 1 x 1024: carries 65, join 14, outputs 89 us.
 //
-// Few rows and a long time axis leave most of the card idle, so the axis is cut into segments: k_scan_carry gets each segment's
+// Few rows and a long time axis leave most of the card idle, so the axis is cut into segments: k_scan_fwd<CARRY> gets each segment's
 // final state from a zero start and the sum of its steps (the product of the decays is e^(A sum delta)), k_scan_combine joins
 // them in order, and the main kernel runs every segment from its true start.  Backward does the same from the right.
 //
-// Backward.  The forward pass keeps the state in front of every TS steps (checkpoints, N floats per channel and tile).  The
+// Backward.  The forward pass keeps the state in front of every eighth step (checkpoints, N floats per channel and tile).  The
 // backward kernel rebuilds a tile's states from it, two states of a lane at a time (decays and states of TS steps then stay in registers), and
 // walks the tile in reverse with g_t = carry + C_t dy_t, carry <- e^(delta A) g_t.  dB and dC sum over channels, 4 values per step, lane and
 // pass: permlane swaps halve the values while they add (v_permlane32_swap exchanges half of one register's lanes with half of another's),
@@ -379,11 +382,10 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
 
 // seg_h becomes the state every segment starts from (REV = 0) / the carry that enters every segment from the right (REV = 1).
 template <int NL, int REV>
-__global__ __launch_bounds__(256) void k_scan_combine(Args a) {
+__global__ __launch_bounds__(64) void k_scan_combine(Args a) {
   const fdql_scan_t &p = a.p;
   const int64_t per = (int64_t)p.R * p.G * a.tpg * NL * 64;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= per) return;
+  const int64_t i = (int64_t)blockIdx.x * 64 + threadIdx.x;
   const int lane = (int)(i & 63), j = (int)(i / 64 % NL);
   const int64_t blk = i / (64 * NL);
   const int tile = (int)(blk % a.tpg), g = (int)(blk / a.tpg % p.G), r = (int)(blk / a.tpg / p.G);
@@ -396,12 +398,13 @@ __global__ __launch_bounds__(256) void k_scan_combine(Args a) {
     if (REV) cur = p.dstate_out ? p.dstate_out[((int64_t)r * p.D + d) * p.N + n] : 0.f;
     else cur = p.state_in ? p.state_in[(int64_t)r * p.state_in_sr + (int64_t)d * p.N + n] : 0.f;
   }
-  // AHEAD segments' values are read together: one by one, each read behind the last one's store, 64 segments took 24 us
+  // AHEAD segments' values are read together, the next ones before these are joined: one by one, each read behind the last one's store, 64
+  // segments took 24 us
   constexpr int AHEAD = 16;
   const auto seg_of = [&](int k) { return REV ? a.nseg - 1 - k : k; };
-  for (int k0 = 0; k0 < a.nseg - 1; k0 += AHEAD) {
-    float own[AHEAD], sum[AHEAD];
-    int any[AHEAD];
+  float own[AHEAD], sum[AHEAD];
+  int any[AHEAD];
+  const auto fetch = [&](int k0) {
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q) {
       const int64_t seg = seg_of(min(k0 + q, a.nseg - 2));
@@ -409,11 +412,23 @@ __global__ __launch_bounds__(256) void k_scan_combine(Args a) {
       sum[q] = a.seg_d[(seg * p.R * p.G * a.tpg + blk) * 64 + lane];
       any[q] = a.seg_f[seg * p.R + r];
     }
+  };
+  fetch(0);
+  for (int k0 = 0; k0 < a.nseg - 1; k0 += AHEAD) {
+    float to[AHEAD], e[AHEAD];
+    bool cut[AHEAD];
+#pragma unroll
+    for (int q = 0; q < AHEAD; ++q) {
+      to[q] = own[q];
+      e[q] = __builtin_amdgcn_exp2f(sum[q] * A);
+      cut[q] = any[q] != 0;
+    }
+    if (k0 + AHEAD < a.nseg - 1) fetch(k0 + AHEAD);
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q) {
       if (k0 + q < a.nseg - 1) {
         a.seg_h[seg_of(k0 + q) * per + i] = cur;
-        cur = any[q] ? own[q] : fmaf(__builtin_amdgcn_exp2f(sum[q] * A), cur, own[q]);
+        cur = cut[q] ? to[q] : fmaf(e[q], cur, to[q]);
       }
     }
   }
@@ -736,7 +751,7 @@ struct Plan {
   int NL, tpg, Dg, nseg, seglen, wgt, wpw;
 };
 
-int cus() { return 256; }
+constexpr int CUS = 256;
 
 Plan plan_of(const fdql_scan_t &p) {
   Plan q;
@@ -747,8 +762,12 @@ Plan plan_of(const fdql_scan_t &p) {
   const int64_t waves = rows * q.tpg;
   q.nseg = 1;
   q.seglen = p.T;
-  if (waves > 0 && waves < 1024 && p.T >= 128) {
-    const int64_t want = std::min<int64_t>((4096 + waves - 1) / waves, p.T / 64);
+  // Segments: fewer than two waves per SIMD and at least three segments of 32 steps, since each is walked twice; eight waves per SIMD where the
+  // length allows.  Training passes, N 16, float, cut or in one piece: 256 x 4 x 128 56 us or 181, 512 x 40 x 512 (1280 waves) 335 or 425; the
+  // other way 256 x 64 x 512 (2048 waves) 270 or 237, 64 x 24 x 512 in two segments 69 or 62.  bf16 16383 x 1 x 1024: 542 us with eight waves per
+  // SIMD, 575 with four, 11304 in one piece.
+  if (waves > 0 && waves < 2048 && p.T >= 96) {
+    const int64_t want = std::min<int64_t>((8192 + waves - 1) / waves, p.T / 32);
     if (want > 1) {
       q.seglen = (int)(((p.T + want - 1) / want + TS - 1) / TS * TS);
       q.nseg = (p.T + q.seglen - 1) / q.seglen;
@@ -805,7 +824,7 @@ hipError_t fwd(const fdql_scan_t &p, hipStream_t s) {
     const int64_t per = (int64_t)p.R * p.G * q.tpg;
     if (q.nseg > 1) {
       hipLaunchKernelGGL((k_scan_fwd<T, NL, true>), dim3((unsigned)(((q.nseg - 1) * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
-      hipLaunchKernelGGL((k_scan_combine<NL, 0>), dim3((unsigned)((per * NL * 64 + 255) / 256)), dim3(256), 0, s, a);
+      hipLaunchKernelGGL((k_scan_combine<NL, 0>), dim3((unsigned)(per * NL)), dim3(64), 0, s, a);
     }
     hipLaunchKernelGGL((k_scan_fwd<T, NL, false>), dim3((unsigned)((q.nseg * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
     return hipGetLastError();
@@ -821,11 +840,11 @@ hipError_t bwd(const fdql_scan_t &p, hipStream_t s) {
     const int64_t per = (int64_t)p.R * p.G * q.tpg;
     if (q.nseg > 1) {
       hipLaunchKernelGGL((k_scan_carry_back<T, NL>), dim3((unsigned)(((q.nseg - 1) * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
-      hipLaunchKernelGGL((k_scan_combine<NL, 1>), dim3((unsigned)((per * NL * 64 + 255) / 256)), dim3(256), 0, s, a);
+      hipLaunchKernelGGL((k_scan_combine<NL, 1>), dim3((unsigned)(per * NL)), dim3(64), 0, s, a);
     }
     hipLaunchKernelGGL((k_scan_bwd<T, NL>), dim3((unsigned)((int64_t)q.nseg * p.R * p.G * q.wgt)), dim3(q.wpw * 64), 0, s, a);
     const int64_t bc = (int64_t)p.T * p.R * p.G * p.N;
-    hipLaunchKernelGGL((k_scan_bc_finish<T>), dim3((unsigned)std::min<int64_t>((bc + 255) / 256, 8 * cus()), 2), dim3(256), 0, s, a);
+    hipLaunchKernelGGL((k_scan_bc_finish<T>), dim3((unsigned)std::min<int64_t>((bc + 255) / 256, 8 * CUS), 2), dim3(256), 0, s, a);
     hipLaunchKernelGGL((k_scan_par_finish<NL>), dim3((unsigned)(p.G * q.tpg * (NL + 2))), dim3(1024), 0, s, a);
     return hipGetLastError();
   });

@@ -290,6 +290,10 @@ int fdql_agent_create(fdql_agent_t **out, const fdql_agent_config_t *cfg) {
     // slices would walk 2 (C + 1) K-segments in four serial load passes: 0.344 against 0.325 ms per temporal_len-2 step)
     a->dstate_split = a->M <= DSTATE_SPLIT_MAX_ROWS || ws_ok;
   }
+  if (c.joiner_ssm && ssm_check(a, a->T, a->B) != FDQL_OK) {
+    delete a;
+    return FDQL_EINVAL;
+  }
   carve(a);
   a->ws_need = a->carve_top;
   *out = a;

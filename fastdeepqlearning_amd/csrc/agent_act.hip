@@ -98,6 +98,7 @@ int fdql_agent_act(fdql_agent_t *a, const float *obs_1d, const float *achieved_g
                    (reinterpret_cast<uintptr_t>(workspace) & 15) == 0,
                "fdql_agent_act: workspace too small or misaligned (need %lld bytes)",
                (long long)fdql_agent_act_workspace_bytes(a, rows));
+  if (c.joiner_ssm && ssm_check(a, 1, rows) != FDQL_OK) return FDQL_EINVAL;
   FDQL_REQUIRE((int)a->enc_obs.hid.size() + 3 <= ACT_MAX_SEG, "too many hidden layers for act()");
   hipStream_t s = (hipStream_t)stream;
   float *top = (float *)workspace;

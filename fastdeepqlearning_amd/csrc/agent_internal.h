@@ -300,6 +300,7 @@ void carve(fdql_agent *a);            // ... the workspace
 fdql_causal_conv_t ssm_conv_of(const fdql_agent *a, int T, int rows);
 fdql_scan_t ssm_scan_of(const fdql_agent *a, int T, int rows);
 fdql_gated_t ssm_gated_of(const fdql_agent *a, int64_t rows);
+int ssm_check(const fdql_agent *a, int T, int rows);   // the operators' limits on such a call
 int build_plan(fdql_agent *a);        // ... the launch list for a->batch (ends with upload_tables)
 int upload_tables(fdql_agent *a);
 }  // namespace fdql

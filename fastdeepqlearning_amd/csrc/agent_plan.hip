@@ -145,6 +145,13 @@ fdql_gated_t ssm_gated_of(const fdql_agent *a, int64_t rows) {
   return p;
 }
 
+int ssm_check(const fdql_agent *a, int T, int rows) {
+  const fdql_causal_conv_t c = ssm_conv_of(a, T, rows);
+  const fdql_scan_t s = ssm_scan_of(a, T, rows);
+  const fdql_gated_t g = ssm_gated_of(a, (int64_t)T * rows);
+  return fdql_causal_conv_workspace_bytes(&c) < 0 || fdql_scan_workspace_bytes(&s, 0) < 0 || fdql_gated_workspace_bytes(&g, 0) < 0 ? FDQL_EINVAL : FDQL_OK;
+}
+
 // ------------------------------------------------------------------------------ workspace
 void carve(fdql_agent *a) {
   a->carve_top = 0;

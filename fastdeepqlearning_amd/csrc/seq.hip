@@ -49,8 +49,9 @@ int check_scan(const fdql_scan_t *p) {
   FDQL_REQUIRE(p->T >= 0 && p->R >= 0 && p->D >= 1, "scan: T %d, R %d, D %d", p->T, p->R, p->D);
   FDQL_REQUIRE(p->N >= 1 && p->N <= 64, "scan: %d states (1 to 64)", p->N);
   FDQL_REQUIRE(p->G >= 1 && p->D % p->G == 0, "scan: %d groups do not divide %d channels", p->G, p->D);
-  // at most 2048 + rows x tiles waves, finish kernels of 1024 threads per 16 channels and state
-  FDQL_REQUIRE(((int64_t)p->R * p->G * ((p->D / p->G + 15) / 16) + 4096) * 64 * 16 < MAX_THREADS, "scan: R %d x D %d is more than one launch", p->R, p->D);
+  // waves of 16 channels (a time axis cut into segments: 10240 of them at most), 16 of the joining kernel's each; 18 finish workgroups of 1024 threads
+  const int64_t tiles = (int64_t)p->G * ((p->D / p->G + 15) / 16);
+  FDQL_REQUIRE((p->R * tiles + 10240) * 64 * 16 < MAX_THREADS && tiles * 18 * 1024 < MAX_THREADS, "scan: R %d x D %d is more than one launch", p->R, p->D);
   return FDQL_OK;
 }
 int check_gated(const fdql_gated_t *p) {
@@ -106,8 +107,9 @@ extern "C" int fdql_causal_conv(const fdql_causal_conv_t *p, void *stream) {
   FDQL_TRY(check_conv(p));
   if (p->R == 0) return FDQL_OK;
   FDQL_REQUIRE(p->weight && (p->T == 0 || (p->x && p->y)), "causal_conv: x, weight and y are needed");
-  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1 && p->state_in_sr == p->state_out_sr),
-               "causal_conv: the state is updated in place only in a single step");
+  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1), "causal_conv: the state is updated in place only in a single step");
+  FDQL_REQUIRE(!p->state_out || p->R == 1 || p->state_out_sr >= (p->K - 1ll) * p->D, "causal_conv: rows of state_out %lld apart overlap", (long long)p->state_out_sr);
+  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || p->state_in_sr == p->state_out_sr, "causal_conv: a state updated in place has one row stride");
   FDQL_HIP(seqconv_fwd_launch(*p, (hipStream_t)stream));
   return FDQL_OK;
 }
@@ -132,8 +134,9 @@ extern "C" int fdql_scan(const fdql_scan_t *p, void *stream) {
   hipStream_t s = (hipStream_t)stream;
   FDQL_TRY(check_scan(p));
   if (p->R == 0) return FDQL_OK;
-  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1 && !p->checkpoints && p->state_in_sr == p->state_out_sr),
-               "scan: the state is updated in place only in a single step");
+  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1 && !p->checkpoints), "scan: the state is updated in place only in a single step");
+  FDQL_REQUIRE(!p->state_out || p->R == 1 || p->state_out_sr >= (int64_t)p->D * p->N, "scan: rows of state_out %lld apart overlap", (long long)p->state_out_sr);
+  FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || p->state_in_sr == p->state_out_sr, "scan: a state updated in place has one row stride");
   if (p->T == 0) return copy_rows(p->state_in, p->state_in_sr, p->state_out, p->state_out_sr, p->R, (int64_t)p->D * p->N, s);
   FDQL_REQUIRE(p->x && p->dt && p->A && p->B && p->C && p->y, "scan: x, dt, A, B, C and y are needed");
   FDQL_TRY(check_workspace("scan", p->workspace, p->workspace_bytes, scan_workspace_bytes(*p, false)));

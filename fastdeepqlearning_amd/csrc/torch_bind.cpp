@@ -94,6 +94,10 @@ bool graded(std::initializer_list<Tensor> ts) {
 void no_grad(const char *what, std::initializer_list<Tensor> ts) {
   TORCH_CHECK_VALUE(!graded(ts), what, " has no gradient: call it under torch.no_grad(), or the windowed form with T = 1");
 }
+// A tensor that a kernel writes in place counts as changed: a backward pass that saved it refuses, as behind torch's own in-place operators.
+void written(const Tensor &t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 // Gradients of a backward pass that itself is recorded (create_graph): differentiating them again is an error, not a silent zero.
 variable_list once(const char *what, variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -207,10 +211,12 @@ std::pair<Tensor, Tensor> causal_conv_step(const Tensor &x, const Opt &state_, c
   TORCH_CHECK_VALUE(state.defined(), what, ": a state is needed");
   conv_check(what, x, weight, bias, state);
   check_reset(what, x, reset);
-  no_grad(what, {x, state, weight, bias});
+  no_grad(what, {x, state, weight, bias, out});
   same(what, "out_state", x, out, state.sizes(), x.scalar_type());
   TORCH_CHECK_VALUE(!out.defined() || out.size(0) == 0 || out.select(0, 0).is_contiguous(), what, ": rows of out_state must be dense");
-  return conv_run(dense(x), whole(weight), whole(bias), rows_dense(state), reset, silu, true, out);
+  auto r = conv_run(dense(x), whole(weight), whole(bias), rows_dense(state), reset, silu, true, out);
+  written(out);
+  return r;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------- scan
@@ -345,10 +351,11 @@ std::pair<Tensor, Tensor> selective_scan_step(const Tensor &x, const Tensor &dt,
   head(what, x, 2);
   TORCH_CHECK_VALUE(state.defined(), what, ": a state is needed");
   const ScanIn i = scan_check(what, x, dt, A, B, C, val(skip), val(z), val(dt_bias), state, val(reset), softplus);
-  no_grad(what, {x, dt, A, B, C, i.skip, i.z, i.dt_bias, state});
+  no_grad(what, {x, dt, A, B, C, i.skip, i.z, i.dt_bias, state, out});
   same(what, "out_state", x, out, state.sizes(), at::kFloat);
   TORCH_CHECK_VALUE(!out.defined() || out.size(0) == 0 || out.select(0, 0).is_contiguous(), what, ": rows of out_state must be dense");
   auto r = scan_run(i, true, false, out);
+  written(out);
   return {std::get<0>(r), std::get<1>(r)};
 }
 

@@ -426,7 +426,7 @@ int32_t fdql_agent_profile_update(fdql_agent_t *agent, const fdql_batch_t *batch
 /* Sequence operators: a recurrent block over replay windows                             */
 /* ------------------------------------------------------------------------------------ */
 /* The reference's only learned operator over the time axis is nn.GRU (franQ/Agent/components/encoder.py:40-42, 78-94).  These
- * three are a design of this build: the short causal convolution, the selective state-space scan and the gated linear unit of
+ * three are a design of this implementation: the short causal convolution, the selective state-space scan and the gated linear unit of
  * a recurrent block, for training on [T, rows, *] windows, for prompts and for one acting step (T = 1).
  *
  * Common to all: `size` is sizeof the struct (checked); dtype is FDQL_F32, FDQL_BF16 or FDQL_F16 and is the type of every
@@ -443,7 +443,7 @@ int32_t fdql_agent_profile_update(fdql_agent_t *agent, const fdql_batch_t *batch
 
 /* y_t = f(bias + sum_{j<K} weight[:, K-1-j] * x_{t-j}), f = SiLU or identity, channel by channel; x_{t-j} counts as zero when a
  * reset lies in (t-j, t].  Inputs before step 0 come from state_in [R, K-1, D] (row stride state_in_sr, oldest first; NULL: zeros); state_out
- * [R, K-1, D] (row stride state_out_sr; or NULL) receives the last K-1 inputs (zeros for those before the last reset).  state_out may be
+ * [R, K-1, D] (row stride state_out_sr >= (K-1) D; or NULL) receives the last K-1 inputs (zeros for those before the last reset).  state_out may be
  * state_in, with the same stride, when T == 1.
  * Backward: dy [T, R, D] (strides dy_st, dy_sr) and dstate_out (or NULL) -> dx, dweight [D, K], dbias [D], dstate_in (each or NULL).                  */
 typedef struct {
@@ -475,8 +475,8 @@ int fdql_causal_conv_backward(const fdql_causal_conv_t *p, void *stream);
  *   delta = softplus(dt_t + dt_bias)   (dt_t + dt_bias itself without dt_softplus)
  *   h     = exp(delta * A[d]) * h + delta * x_t * B_t[g]      (the first term dropped at a reset)
  *   y_t   = (C_t[g] . h + skip[d] * x_t) * SiLU(z_t)          (factors that are NULL left out)
- * state_in [R, D, N] (row stride state_in_sr, NULL: zeros), state_out [R, D, N] (row stride state_out_sr; or NULL; may be state_in, with the
- * same stride, when T == 1).
+ * state_in [R, D, N] (row stride state_in_sr, NULL: zeros), state_out [R, D, N] (row stride state_out_sr >= D N; or NULL; may be state_in,
+ * with the same stride, when T == 1).
  * checkpoints: fdql_scan_checkpoint_floats() floats that the forward call fills for the backward call of the same inputs (NULL
  * when there is none).  Backward: dy (strides dy_st, dy_sr) and dstate_out (or NULL) -> every gradient; those of optional inputs that are NULL may be NULL,
  * dstate_in always.                                                                                              */

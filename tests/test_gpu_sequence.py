@@ -591,3 +591,35 @@ def test_gated_small_gradients_round_once(dev, seq, M, D, F, kind, dtype):
         bound = (want.abs() + exact) * u * 1.01 + exact + tiny
         off = (have.cpu().double() - want).abs()
         assert (off <= bound).all(), (name, float((off / bound.clamp_min(1e-300)).max()))
+
+
+def test_a_state_updated_in_place_counts_as_changed(dev, seq):
+    """A window that saved the state for its backward pass refuses to run it once a step has written that state; out_state rows that share
+    memory, and one that wants a gradient, are refused."""
+    g = _gen(5)
+    x = torch.randn(3, 2, 8, generator=g).to(dev)
+    w, A = torch.randn(8, 4, generator=g).to(dev).requires_grad_(), -torch.rand(8, 4, generator=g).to(dev)
+    B = torch.randn(3, 2, 4, generator=g).to(dev)
+    cs, hs = torch.randn(2, 3, 8, generator=g).to(dev), torch.randn(2, 8, 4, generator=g).to(dev)
+    y = seq.causal_conv(x, w, initial_state=cs)
+    v = seq.selective_scan(y, x, A, B, B, initial_state=hs)
+    kept = [seq.causal_conv(x, w, initial_state=cs.clone()).sum(), v.sum()]
+    with torch.no_grad():
+        seq.causal_conv_step(x[0], cs, w, out_state=cs)
+        seq.selective_scan_step(x[0], x[0], A, B[0], B[0], hs, out_state=hs)
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.sum().backward()
+    with pytest.raises(RuntimeError, match="inplace"):
+        kept[1].backward()
+    kept[0].backward()
+    with torch.no_grad():
+        with pytest.raises(Exception, match="overlap"):
+            seq.causal_conv_step(x[0], cs, w, out_state=cs[:1].expand(2, 3, 8))
+        with pytest.raises(Exception, match="overlap"):
+            seq.selective_scan_step(x[0], x[0], A, B[0], B[0], hs, out_state=hs[:1].expand(2, 8, 4))
+    with pytest.raises(ValueError, match="no gradient"):
+        seq.selective_scan_step(x[0], x[0], A, B[0], B[0], hs, out_state=torch.zeros(2, 8, 4, device=dev, requires_grad=True))
+    with torch.inference_mode():
+        s = torch.zeros(2, 3, 8, device=dev)
+        seq.causal_conv_step(x[0], s, w, out_state=s)
+        assert s.any()

@@ -149,3 +149,19 @@ def test_workspace_queries():
     assert lib.fdql_scan_workspace_bytes(C.byref(_scan(N=99)), 1) == nat.FDQL_EINVAL
     assert lib.fdql_causal_conv_workspace_bytes(C.byref(_conv(K=9))) == nat.FDQL_EINVAL
     assert lib.fdql_gated_workspace_bytes(C.byref(_gated(F=0)), 1) == nat.FDQL_EINVAL
+
+
+@pytest.mark.parametrize("entry,make,kw,least", [("fdql_causal_conv", _conv, dict(x=P, weight=P, y=P, T=1), 24), ("fdql_scan", _scan, dict(x=P, dt=P, A=P, B=P, C=P, y=P, T=1), 32)])
+def test_state_rows_that_would_overlap_are_refused(entry, make, kw, least):
+    """A row stride of state_out below a row's length (0: every row in one place) would let rows overwrite each other."""
+    lib = nat.load()
+    for sr in (0, least - 1, -least):
+        assert getattr(lib, entry)(C.byref(make(state_out=P, state_out_sr=sr, **kw)), None) == nat.FDQL_EINVAL
+        assert "overlap" in lib.fdql_last_error().decode()
+
+
+def test_more_channels_than_the_finish_kernels_take_are_refused():
+    lib = nat.load()
+    assert lib.fdql_scan_workspace_bytes(C.byref(_scan(R=1, D=1 << 22)), 1) == nat.FDQL_EINVAL
+    assert "one launch" in lib.fdql_last_error().decode()
+    assert lib.fdql_scan_workspace_bytes(C.byref(_scan(R=1, D=1 << 21)), 1) > 0

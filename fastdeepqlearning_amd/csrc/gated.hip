@@ -574,6 +574,15 @@ __global__ __launch_bounds__(NW * 64) void k_gated_rows(Args a) {
 #pragma unroll
     for (int w = 0; w < 2; ++w) acc[m][w] = v4f{0.f, 0.f, 0.f, 0.f};
   const bool two = p.M > 16;
+  float bg[4] = {}, bu[4] = {};                         // read now, added behind the sums
+  if (wave == 0 && p.b_gate) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t o = min(f0 + 4 * q + r, F - 1);
+      bg[r] = to_f(reinterpret_cast<const T *>(p.b_gate)[o]);
+      bu[r] = to_f(reinterpret_cast<const T *>(p.b_up)[o]);
+    }
+  }
   const int64_t steps = (D + KS - 1) / KS, per = (steps + NW - 1) / NW, s1 = min(steps, (wave + 1) * per);
 #pragma unroll 4
   for (int64_t st = wave * per; st < s1; ++st) {
@@ -607,8 +616,8 @@ __global__ __launch_bounds__(NW * 64) void k_gated_rows(Args a) {
     for (int r = 0; r < 4; ++r) {
       const int64_t o = f0 + 4 * q + r;
       if (o < F) {
-        const float g = acc[m][0][r] + (p.b_gate ? to_f(reinterpret_cast<const T *>(p.b_gate)[o]) : 0.f);
-        const float u = acc[m][1][r] + (p.b_up ? to_f(reinterpret_cast<const T *>(p.b_up)[o]) : 0.f);
+        const float g = acc[m][0][r] + bg[r];
+        const float u = acc[m][1][r] + bu[r];
         reinterpret_cast<T *>(p.y)[row * F + o] = from_f<T>(act_f(p.act, g) * u);
         if (p.pre) {
           p.pre[row * F + o] = g;

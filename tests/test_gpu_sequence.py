@@ -658,3 +658,10 @@ def test_capturing_beside_an_eager_graph_of_the_same_leaves_is_refused(dev, seq,
         torch.cuda.synchronize(dev)
         assert torch.equal(got, want)
         assert torch.equal(step(), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("R,D,N,G", [(700, 192, 16, 1), (1100, 65, 5, 1), (2050, 7, 33, 1), (360, 258, 64, 2), (2048, 64, 4, 1), (2047, 64, 4, 1)])
+def test_scan_steps_of_many_rows(dev, seq, R, D, N, G, dtype):
+    """Both sides of the rule that gives few rows a kernel of their own."""
+    test_scan_steps_follow_the_definition(dev, seq, R, D, N, G, dtype)

@@ -228,9 +228,16 @@ __device__ __forceinline__ void clear(v16f (&acc)[MT][2]) {
 }
 
 // The backward products pass over their contraction once for every part of d, DX for the gate's side, then the up side's.
-template <int MODE>
-__device__ __forceinline__ int passes_of(const Args &a) { return MODE == FWD ? 1 : MODE == DX ? 2 * a.parts : a.parts; }
-__device__ __forceinline__ int pass_of(int step, int len) { return (step >= len) + (step >= 2 * len) + (step >= 3 * len); }
+// PARTS: there may be two of them (the tiles of 256 columns are never given such a problem).
+template <int MODE, bool PARTS>
+__device__ __forceinline__ int passes_of(const Args &a) { return (MODE == DX ? 2 : 1) * (PARTS && MODE != FWD ? a.parts : 1); }
+template <int MODE, bool PARTS>
+__device__ __forceinline__ int pass_of(int step, int len) {
+  if (PARTS && MODE != FWD) return (step >= len) + (step >= 2 * len) + (step >= 3 * len);
+  return MODE == DX && step >= len;
+}
+template <int MODE, bool PARTS>
+__device__ __forceinline__ int side_of(const Args &a, int pass) { return MODE != DX ? 0 : PARTS && a.parts == 2 ? pass >> 1 : pass; }
 
 // Float sums over a long contraction: RUN slices (512 products) at a time, the runs added up apart, so that the rounding error grows with the run's
 // length and their number instead of the whole length (dx at F 2000: 1.2e-6 of its norm in one chain).  16-bit results round at 2^-12
@@ -272,6 +279,7 @@ struct Runs {
 template <typename T, int MODE>
 __global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
   constexpr int BM = 64, BN = 128, BK = 128 / sizeof(T);
+  constexpr bool PARTS = sizeof(T) == 2;
   __shared__ __align__(16) char lds[2][(BM + BN) * 128];
   const fdql_gated_t &p = a.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
@@ -282,7 +290,7 @@ __global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
   const T *x = reinterpret_cast<const T *>(p.x), *wg = reinterpret_cast<const T *>(p.w_gate), *wu = reinterpret_cast<const T *>(p.w_up);
   const T *dd = reinterpret_cast<const T *>(a.d) + (MODE == DW ? which * a.parts * M * a.Fp : 0);
   const int64_t kbeg = MODE == DW ? (int64_t)ks * a.kper : 0, kend = MODE == FWD ? D : MODE == DX ? F : min(M, kbeg + a.kper);
-  const int half = (int)((kend - kbeg + BK - 1) / BK), steps = passes_of<MODE>(a) * half;
+  const int half = (int)((kend - kbeg + BK - 1) / BK), steps = passes_of<MODE, PARTS>(a) * half;
 
   Flight<2> fa;
   Flight<4> fb;
@@ -295,13 +303,13 @@ __global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
         return f < F ? (n & 32 ? wu : wg) + f * D : (const T *)nullptr;
       }, k0, D);
     } else if constexpr (MODE == DX) {
-      const int pass = pass_of(step, half), up = a.parts == 2 ? pass >> 1 : pass;
+      const int pass = pass_of<MODE, PARTS>(step, half), up = side_of<MODE, PARTS>(a, pass);
       const int64_t k0 = (int64_t)(step - pass * half) * BK;
       const T *src = dd + pass * M * a.Fp;
       fetch_rows<T>(fa, [&](int n) { return m0 + n < M ? src + (m0 + n) * a.Fp : (const T *)nullptr; }, k0, F);
       fetch_cols<T>(fb, up ? wu : wg, D, k0, F, n0, D);
     } else {
-      const int pass = pass_of(step, half);
+      const int pass = pass_of<MODE, PARTS>(step, half);
       const int64_t k0 = kbeg + (int64_t)(step - pass * half) * BK;
       fetch_cols<T>(fa, dd + pass * M * a.Fp, a.Fp, k0, kend, m0, F);
       fetch_cols<T>(fb, x, p.x_sr, k0, kend, n0, D);
@@ -395,6 +403,7 @@ __device__ __forceinline__ int2 tr_read(const char *p) {
 template <typename T, int MODE, int BM, int BN>
 __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
   typedef Ring<T, BM, BN> R;
+  constexpr bool PARTS = sizeof(T) == 2 && BN == 128;
   constexpr int KS = R::KS, NBUF = R::NBUF, ABYTES = R::ABYTES, BBYTES = R::BBYTES, E = 16 / sizeof(T), RB = KS * sizeof(T), WAVES = BN / 32;
   constexpr int MT = BM / 64, NT = 2, NA = ABYTES / (WAVES * 1024), NB = BBYTES / (WAVES * 1024), KSTEPS = RB / 32;
   typedef RowTile<RB> Rows;
@@ -408,10 +417,10 @@ __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
   const int64_t M = p.M, D = p.D, F = p.F, m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN, f0 = (int64_t)tn * (BN / 2);
   const int which = MODE == DW ? blockIdx.y : 0, ks = MODE == DW ? blockIdx.z : 0;
   const T *x = reinterpret_cast<const T *>(p.x), *wg = reinterpret_cast<const T *>(p.w_gate), *wu = reinterpret_cast<const T *>(p.w_up);
-  const T *dd = reinterpret_cast<const T *>(a.d) + which * a.parts * M * a.Fp;
+  const T *dd = reinterpret_cast<const T *>(a.d) + which * (PARTS ? a.parts : 1) * M * a.Fp;
   // contraction [kbeg, K) of one pass
   const int64_t kbeg = MODE == DW ? (int64_t)ks * a.kper : 0, K = MODE == FWD ? D : MODE == DX ? a.Fp : min(M, kbeg + a.kper);
-  const int half = (int)((K - kbeg + KS - 1) / KS), steps = passes_of<MODE>(a) * half;
+  const int half = (int)((K - kbeg + KS - 1) / KS), steps = passes_of<MODE, PARTS>(a) * half;
 
   // where this lane's chunks come from: an element offset from the operand's start for slice 0, and the chunk's place in the contraction
   int64_t oa[NA], ob[NB];
@@ -451,7 +460,7 @@ __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
   // piece `piece` of `pieces` of a slice's DMA (a wave is held up while its requests are taken: in one go, with the other waves', that left the
   // matrix unit idle for a quarter of a step)
   const auto fetch = [&](int step, int buf, int piece, int pieces) {
-    const int pass = MODE == FWD ? 0 : pass_of(step, half), up = MODE == DX ? (a.parts == 2 ? pass >> 1 : pass) : 0;
+    const int pass = pass_of<MODE, PARTS>(step, half), up = side_of<MODE, PARTS>(a, pass);
     const int64_t k0 = kbeg + (int64_t)(step - pass * half) * KS;
     const unsigned la = lds_addr(lds) + buf * (ABYTES + BBYTES) + wave * NA * 1024, lb = lds_addr(lds) + buf * (ABYTES + BBYTES) + ABYTES + wave * NB * 1024;
     const T *pa = MODE == FWD ? x + k0 : MODE == DX ? dd + pass * M * a.Fp + k0 : dd + pass * M * a.Fp + k0 * a.Fp;
@@ -758,6 +767,12 @@ Plan plan_of(const fdql_gated_t &p) {
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 bool al16(const void *q) { return ((uintptr_t)q & 15) == 0; }
 
+template <typename T, int MODE>
+Choice choice_of(const Args &a, bool aligned) {
+  if (!aligned || a.parts == 2) return SMALL;
+  return sizeof(T) == 2 ? WIDE : MODE == DW ? SMALL : FLOAT;
+}
+
 template <typename T, int MODE, int BM, int BN>
 hipError_t launch_mma(const Args &a, dim3 grid, hipStream_t s) {
   constexpr int bytes = Ring<T, BM, BN>::BYTES;
@@ -770,7 +785,7 @@ hipError_t launch_mma(const Args &a, dim3 grid, hipStream_t s) {
 template <typename T, int MODE>
 hipError_t product(Args a, int64_t rows, int64_t cols, bool aligned, hipStream_t s) {
   const int copies = MODE == DW ? 2 : 1;
-  const Shape q = shape_of(!aligned ? SMALL : sizeof(T) == 2 ? WIDE : MODE == DW ? SMALL : FLOAT, rows, cols, MODE == FWD ? 128 : 256, copies);
+  const Shape q = shape_of(choice_of<T, MODE>(a, aligned), rows, cols, MODE == FWD ? 128 : 256, copies);
   a.tiles_m = (int)q.tiles_m;
   a.tiles_n = (int)q.tiles_n;
   if (MODE == DW && q.bn == 256) a.ksplit = 1, a.kper = (int)((a.p.M + 63) / 64 * 64);
@@ -822,7 +837,7 @@ hipError_t bwd(const fdql_gated_t &p, hipStream_t s) {
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && p.dx) e = product<T, DX>(a, p.M, p.D, p.D % E == 0 && al16(p.w_gate) && al16(p.w_up), s);
   const bool w = p.dw_gate && p.dw_up, vec = p.D % E == 0 && p.x_sr % E == 0 && al16(p.x);
-  if (w && shape_of(sizeof(T) == 2 && vec ? WIDE : SMALL, p.F, p.D, 256, 2).bn == 256) a.ksplit = 1;
+  if (w && shape_of(choice_of<T, DW>(a, vec), p.F, p.D, 256, 2).bn == 256) a.ksplit = 1;
   if (e == hipSuccess && w) e = product<T, DW>(a, p.F, p.D, vec, s);
   const bool sum_w = w && a.ksplit > 1;
   if (e == hipSuccess && (sum_w || p.db_gate || p.db_up)) {

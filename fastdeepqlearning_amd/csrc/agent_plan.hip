@@ -776,7 +776,7 @@ int build_plan(fdql_agent *a) {
     b.func_stage("ssm.scan", [=](hipStream_t s) { return scan_fwd_launch(sc, s); });
     // the last step's rows feed no gradient: their pre-activations are not kept
     fdql_gated_t g1 = ssm_gated_of(a, M), g2 = ssm_gated_of(a, B);
-    g1.x = y; g1.y = state; g1.pre = a->buf("ssm.pre");
+    g1.x = y; g1.y = state; g1.pre = a->buf("ssm.pre"); g1.workspace = g2.workspace = scratch;
     g2.x = y + (int64_t)M * Di; g2.y = state + (int64_t)M * L;
     b.func_stage("ssm.gated", [=](hipStream_t s) {
       const hipError_t e = gated_fwd_launch(g1, s);

@@ -7,8 +7,9 @@
 // their column sums; then dx = dg Wg + du Wu is one product over 2 F, and dWg = dg^T x, dWu = du^T x are one launch with the rows
 // split over workgroups where the weights alone leave the card idle (float32 slabs, added in order).
 //
-// k_gated_mma serves all three products: tiles of BM x BN, slices of the contraction in an LDS ring filled by LDS-DMA (see there).  Tensors whose
-// rows are not 16-byte aligned take k_gated_any: the same tiles with element loads through registers.  Matrix instructions:
+// k_gated_mma serves all three products: tiles of BM x BN, slices of the contraction in an LDS ring filled by LDS-DMA (see there).  Rows that are
+// not whole 16-byte chunks are copied into the workspace first (k_gated_pack); tensors that only start in the middle of a chunk, and calls without
+// a workspace, take k_gated_any: the same tiles with element loads through registers.  Matrix instructions:
 // v_mfma_f32_32x32x16 (bf16, fp16) or four v_mfma_f32_32x32x2 (float) per pair of 16-byte fragments; which k a lane half holds is the same on
 // both sides and does not matter.
 //
@@ -38,6 +39,7 @@ struct Args {
   float *slab;                     // [ksplit][2][F][D] when ksplit > 1
   int ksplit, kper;                // DW: slices of the rows and their length (a multiple of the K slice)
   int tiles_m, tiles_n;
+  int Dk, ldw;                     // length of x's and the weights' rows as they are multiplied (D, or up to whole chunks with zeros behind), of the weights' as they lie
 };
 
 __device__ __forceinline__ int swz(int n) { return (n ^ (n >> 3)) & 7; }
@@ -419,7 +421,7 @@ __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
   const T *x = reinterpret_cast<const T *>(p.x), *wg = reinterpret_cast<const T *>(p.w_gate), *wu = reinterpret_cast<const T *>(p.w_up);
   const T *dd = reinterpret_cast<const T *>(a.d) + which * (PARTS ? a.parts : 1) * M * a.Fp;
   // contraction [kbeg, K) of one pass
-  const int64_t kbeg = MODE == DW ? (int64_t)ks * a.kper : 0, K = MODE == FWD ? D : MODE == DX ? a.Fp : min(M, kbeg + a.kper);
+  const int64_t kbeg = MODE == DW ? (int64_t)ks * a.kper : 0, K = MODE == FWD ? a.Dk : MODE == DX ? a.Fp : min(M, kbeg + a.kper);
   const int half = (int)((K - kbeg + KS - 1) / KS), steps = passes_of<MODE, PARTS>(a) * half;
 
   // where this lane's chunks come from: an element offset from the operand's start for slice 0, and the chunk's place in the contraction
@@ -449,12 +451,12 @@ __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
       kb[q] = Rows::chunk(o) * E;
       const int64_t f = f0 + (n >> 6) * 32 + (n & 31);
       inb[q] = f < F;
-      ob[q] = f * D + kb[q];
+      ob[q] = f * a.ldw + kb[q];
     } else {
       kb[q] = BCols::row(o);
       const int64_t c = n0 + BCols::chunk(o) * E;
       inb[q] = c < D;
-      ob[q] = (int64_t)kb[q] * (MODE == DX ? D : p.x_sr) + c;
+      ob[q] = (int64_t)kb[q] * (MODE == DX ? a.ldw : p.x_sr) + c;
     }
   }
   // piece `piece` of `pieces` of a slice's DMA (a wave is held up while its requests are taken: in one go, with the other waves', that left the
@@ -464,7 +466,7 @@ __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
     const int64_t k0 = kbeg + (int64_t)(step - pass * half) * KS;
     const unsigned la = lds_addr(lds) + buf * (ABYTES + BBYTES) + wave * NA * 1024, lb = lds_addr(lds) + buf * (ABYTES + BBYTES) + ABYTES + wave * NB * 1024;
     const T *pa = MODE == FWD ? x + k0 : MODE == DX ? dd + pass * M * a.Fp + k0 : dd + pass * M * a.Fp + k0 * a.Fp;
-    const int64_t kx = k0 * (MODE == DX ? D : p.x_sr);
+    const int64_t kx = k0 * (MODE == DX ? a.ldw : p.x_sr);
 #pragma unroll
     for (int q = 0; q < NA + NB; ++q) {
       if (q * pieces / (NA + NB) != piece) continue;
@@ -643,7 +645,7 @@ __device__ __forceinline__ T rest_of(float v, T part) {
   const float p = to_f(part);
   return from_f<T>(fabsf(p) < INFINITY ? v - p : 0.f);
 }
-// dg, du of 64 columns x RB rows and their sums over those rows.
+// dg, du of 64 columns x RB rows and their sums over those rows.  Memory bounds it: bf16 8192 x 4096 105 us = 4.5 TB/s.
 constexpr int RB = 128;
 template <typename T>
 __global__ __launch_bounds__(256) void k_gated_grad(Args a) {
@@ -714,12 +716,35 @@ __global__ __launch_bounds__(256) void k_gated_sum(Args a, int64_t rblocks) {
   }
 }
 
+// Rows of whole chunks from rows that are not: x [M], then Wg and Wu [F], each of Dp elements with zeros behind D.  A thread copies one chunk.
+struct Pack {
+  const void *src[3];
+  int64_t sr[3], first[4];         // row strides; rows in front of each tensor's
+  void *dst;
+  int D, Dp;
+};
+template <typename T>
+__global__ __launch_bounds__(256) void k_gated_pack(Pack a) {
+  constexpr int E = 16 / sizeof(T);
+  const int64_t per = a.Dp / E, n = a.first[3] * per;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per, c = i % per * E;
+    const int w = (row >= a.first[1]) + (row >= a.first[2]);
+    const T *src = reinterpret_cast<const T *>(a.src[w]) + (row - a.first[w]) * a.sr[w] + c;
+    typedef T vec __attribute__((ext_vector_type(E)));
+    vec v;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = c + e < a.D ? src[e] : T(0.f);
+    reinterpret_cast<vec *>(a.dst)[i] = v;
+  }
+}
+
+constexpr int CUS = 256;
 // Tile shape of a product: rows x columns of tiles, and for the weight gradients the slices of the rows that fill the card.
 struct Shape {
   int bm, bn;
   int64_t tiles_m, tiles_n;
 };
-constexpr int CUS = 256;
 enum Choice { SMALL, WIDE, FLOAT };        // which tiles there are: 64 x 128 alone; and 128, 256 x 256 of 16-bit types; and 128 x 128 of float
 Shape shape_of(Choice choice, int64_t rows, int64_t cols, int tile_of_256, int copies) {     // tile_of_256: columns that a 256-wide tile covers
   const auto tiles = [&](int bm, int bn) { return (rows + bm - 1) / bm * ((cols + tile_of_256 * bn / 256 - 1) / (tile_of_256 * bn / 256)); };
@@ -767,6 +792,39 @@ Plan plan_of(const fdql_gated_t &p) {
 int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 bool al16(const void *q) { return ((uintptr_t)q & 15) == 0; }
 
+// Rows that are not whole 16-byte chunks are copied into some that are, whatever the size; the same work with element loads (k_gated_any) took, for
+// forward and backward of bf16 4097 x 1001 x 2730, 1120 us against 272, 1000 x 301 x 203 79 against 49, 64 x 101 x 99 49 against 32, float 12800 x 511 x
+// 256 363 against 269, and only where rows are a few dozen elements long up to 2 us less (forward of 10000 x 17 x 61 6.6 against 7.6).
+bool packs(const fdql_gated_t &p) {
+  const int E = p.dtype == FDQL_F32 ? 4 : 8;
+  return p.M > 32 && (p.D % E != 0 || p.x_sr % E != 0);
+}
+int64_t pack_bytes(const fdql_gated_t &p) {
+  const int E = p.dtype == FDQL_F32 ? 4 : 8;
+  return packs(p) ? (p.M + (p.D % E ? 2ll * p.F : 0)) * ((p.D + E - 1) / E * 16ll) : 0;
+}
+// a.p's x and weights become their packed copies at the workspace's start; without a workspace they stay as they are
+template <typename T>
+hipError_t pack(Args &a, hipStream_t s) {
+  constexpr int E = 16 / sizeof(T);
+  fdql_gated_t &p = a.p;
+  a.Dk = a.ldw = p.D;
+  if (!packs(p) || !p.workspace) return hipSuccess;
+  const bool w = p.D % E != 0;
+  const int Dp = (p.D + E - 1) / E * E;
+  Pack k = {{p.x, p.w_gate, p.w_up}, {p.x_sr, p.D, p.D}, {0, p.M, p.M + (w ? p.F : 0), p.M + (w ? 2ll * p.F : 0)}, p.workspace, p.D, Dp};
+  hipLaunchKernelGGL((k_gated_pack<T>), dim3((unsigned)std::min<int64_t>((k.first[3] * (Dp / E) + 255) / 256, 8 * CUS)), dim3(256), 0, s, k);
+  const T *at = reinterpret_cast<const T *>(p.workspace);
+  p.x = at;
+  p.x_sr = Dp;
+  if (w) {
+    p.w_gate = at + k.first[1] * Dp;
+    p.w_up = at + k.first[2] * Dp;
+    a.Dk = a.ldw = Dp;
+  }
+  return hipGetLastError();
+}
+
 template <typename T, int MODE>
 Choice choice_of(const Args &a, bool aligned) {
   if (!aligned || a.parts == 2) return SMALL;
@@ -809,7 +867,9 @@ hipError_t fwd(const fdql_gated_t &p, hipStream_t s) {
   Args a = {};
   a.p = p;
   constexpr int E = 16 / sizeof(T);
-  const bool vec = p.D % E == 0 && p.x_sr % E == 0 && al16(p.x) && al16(p.w_gate) && al16(p.w_up);
+  const hipError_t e = pack<T>(a, s);
+  if (e != hipSuccess) return e;
+  const bool vec = a.ldw % E == 0 && a.p.x_sr % E == 0 && al16(a.p.x) && al16(a.p.w_gate) && al16(a.p.w_up);
   if (p.M > 32) return product<T, FWD>(a, p.M, p.F, vec, s);
   const dim3 grid((unsigned)((p.F + 15) / 16));
   if (vec) hipLaunchKernelGGL((k_gated_rows<T, true>), grid, dim3(NW * 64), 0, s, a);
@@ -825,7 +885,9 @@ hipError_t bwd(const fdql_gated_t &p, hipStream_t s) {
   a.p = p;
   a.Fp = q.Fp;
   a.parts = q.parts;
-  char *ws = reinterpret_cast<char *>(p.workspace);
+  hipError_t e = pack<T>(a, s);
+  if (e != hipSuccess) return e;
+  char *ws = reinterpret_cast<char *>(p.workspace) + pack_bytes(p);
   a.d = ws;
   ws += up16(2 * q.parts * p.M * q.Fp * (int64_t)sizeof(T));
   a.colsum = reinterpret_cast<float *>(ws);
@@ -834,9 +896,9 @@ hipError_t bwd(const fdql_gated_t &p, hipStream_t s) {
   a.ksplit = q.ksplit;
   a.kper = q.kper;
   hipLaunchKernelGGL((k_gated_grad<T>), dim3((unsigned)((q.Fp + 63) / 64), (unsigned)q.rblocks), dim3(256), 0, s, a);
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess && p.dx) e = product<T, DX>(a, p.M, p.D, p.D % E == 0 && al16(p.w_gate) && al16(p.w_up), s);
-  const bool w = p.dw_gate && p.dw_up, vec = p.D % E == 0 && p.x_sr % E == 0 && al16(p.x);
+  e = hipGetLastError();
+  if (e == hipSuccess && p.dx) e = product<T, DX>(a, p.M, p.D, a.ldw % E == 0 && al16(a.p.w_gate) && al16(a.p.w_up), s);
+  const bool w = p.dw_gate && p.dw_up, vec = a.ldw % E == 0 && a.p.x_sr % E == 0 && al16(a.p.x);
   if (w && shape_of(choice_of<T, DW>(a, vec), p.F, p.D, 256, 2).bn == 256) a.ksplit = 1;
   if (e == hipSuccess && w) e = product<T, DW>(a, p.F, p.D, vec, s);
   const bool sum_w = w && a.ksplit > 1;
@@ -851,10 +913,10 @@ hipError_t bwd(const fdql_gated_t &p, hipStream_t s) {
 }  // namespace
 
 int64_t gated_workspace_bytes(const fdql_gated_t &p, bool backward) {
-  if (!backward) return 0;
+  if (!backward) return pack_bytes(p);
   const Plan q = plan_of(p);
   const int64_t esz = p.dtype == FDQL_F32 ? 4 : 2;
-  return up16(2 * q.parts * p.M * q.Fp * esz) + up16(q.rblocks * 2 * p.F * 4) + (q.ksplit > 1 ? (int64_t)q.ksplit * 2 * p.F * p.D * 4 : 0);
+  return pack_bytes(p) + up16(2 * q.parts * p.M * q.Fp * esz) + up16(q.rblocks * 2 * p.F * 4) + (q.ksplit > 1 ? (int64_t)q.ksplit * 2 * p.F * p.D * 4 : 0);
 }
 hipError_t gated_fwd_launch(const fdql_gated_t &p, hipStream_t s) {
   return p.dtype == FDQL_F32 ? fwd<float>(p, s) : p.dtype == FDQL_BF16 ? fwd<bf16_t>(p, s) : fwd<f16_t>(p, s);

@@ -693,7 +693,7 @@ __global__ __launch_bounds__(1024) void k_scan_par_finish(Args a) {
 // ------------------------------------------------------------------------------------------------------------ single steps
 // One step for every row: the state is read and written once, V = 4 states (16 bytes) per lane where the state's rows allow it.  A wave
 // owns 64 channels of one row: lane = channel for delta, x and the gate; then LPC lanes share a channel and the wave passes over
-// its state in LPC turns, consecutive lanes on consecutive addresses.
+// its state in LPC turns, consecutive lanes on consecutive addresses.  Memory bounds it: bf16 512 x 2048 x 64 117 us = 4.7 TB/s.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void k_scan_step(fdql_scan_t p, int Dg, int tpg, int lpc) {
   typedef float vec __attribute__((ext_vector_type(V)));

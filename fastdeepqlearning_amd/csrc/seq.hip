@@ -173,6 +173,7 @@ extern "C" int fdql_gated(const fdql_gated_t *p, void *stream) {
   if (p->M == 0) return FDQL_OK;
   FDQL_REQUIRE(p->x && p->w_gate && p->w_up && p->y, "gated: x, both weights and y are needed");
   FDQL_REQUIRE(!p->b_gate == !p->b_up, "gated: both biases or neither");
+  FDQL_TRY(check_workspace("gated", p->workspace, p->workspace_bytes, gated_workspace_bytes(*p, false)));
   FDQL_HIP(gated_fwd_launch(*p, (hipStream_t)stream));
   return FDQL_OK;
 }

@@ -665,3 +665,36 @@ def test_capturing_beside_an_eager_graph_of_the_same_leaves_is_refused(dev, seq,
 def test_scan_steps_of_many_rows(dev, seq, R, D, N, G, dtype):
     """Both sides of the rule that gives few rows a kernel of their own."""
     test_scan_steps_follow_the_definition(dev, seq, R, D, N, G, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("M,D,F", [(70, 64, 40), (200, 136, 72), (40, 24, 130), (33, 101, 99), (300, 37, 61)])
+@pytest.mark.parametrize("off", ["x", "weights", "both"])
+def test_gated_tensors_that_start_inside_a_chunk(dev, seq, M, D, F, dtype, off):
+    """Whole rows whose first element is not 16-byte aligned, and rows that are not whole chunks: outputs and gradients against the definition.  With u
+    half a step of the type and e = 2^-24: a product of n float terms is off by (2 n + 32) e of its terms, what D roundings move in the gate and the
+    up side enters through e_*, a 16-bit d (dg, du) by u of its terms (twice u^2 where it is kept in two parts: not more), the result by u."""
+    g = _gen(M + D)
+
+    def place(t, shifted):
+        t = t.to(dtype)
+        buf = torch.zeros(t.numel() + 1, dtype=dtype, device=dev)
+        out = buf[1:] if shifted else torch.zeros(t.numel(), dtype=dtype, device=dev)
+        return out.copy_(t.reshape(-1)).view(t.shape)
+    x, wg, wu = torch.randn(M, D, generator=g), torch.randn(F, D, generator=g) * D ** -0.5, torch.randn(F, D, generator=g) * D ** -0.5
+    dy = torch.randn(M, F, generator=g).to(dtype)
+    leaves = [place(x, off != "weights").requires_grad_()] + [place(w, off != "x").requires_grad_() for w in (wg, wu)]
+    assert off == "weights" or leaves[0].data_ptr() % 16
+    y = seq.gated_linear(*leaves)
+    got = torch.autograd.grad(y, leaves, dy.to(dev))
+    o = osq.gated_linear(*(t.to(dtype) for t in (x, wg, wu)), None, None, "silu", dy)
+    u, e = (0.0 if dtype == torch.float32 else torch.finfo(dtype).eps / 2), 2.0 ** -24
+    out_u = torch.finfo(dtype).eps / 2
+    tiny = 2.0 ** -24 if dtype == torch.float16 else 0.0
+    checks = [("y", y.detach(), o["m_y"] * (2 * D + 32) * e)]
+    for name, have, n in (("dx", got[0], 2 * F), ("dw_gate", got[1], M), ("dw_up", got[2], M)):
+        checks.append((name, have, o["r_" + name] * (1.01 * u + (2 * n + 32) * e) + o["e_" + name] * (2 * D + 32) * e + tiny * n))
+    for name, have, exact in checks:
+        bound = (o[name].abs() + exact) * out_u * 1.01 + exact + tiny
+        off_by = (have.cpu().double() - o[name]).abs()
+        assert (off_by <= bound).all(), (name, float((off_by / bound.clamp_min(1e-300)).max()))

@@ -513,6 +513,7 @@ int fdql_scan_backward(const fdql_scan_t *p, void *stream);
 
 /* y = f(x Wg^T + bg) * (x Wu^T + bu), f = SiLU, GELU (the erf form) or sigmoid; x [M, D] (row stride x_sr), weights [F, D] dense, y [M, F] dense.
  * pre: [2, M, F] float32 (or NULL) that the forward call fills with both products for the backward call.
+ * Rows of x or of the weights that are not whole 16-byte chunks are copied into the workspace first (both directions ask for one then).
  * Backward: dy [M, F] (row stride dy_sr) -> dx [M, D], dw_gate, dw_up [F, D], db_gate, db_up [F] (each or NULL), all of the type dtype.            */
 #define FDQL_ACT_SILU 0
 #define FDQL_ACT_GELU 1

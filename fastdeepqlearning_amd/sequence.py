@@ -10,7 +10,8 @@ Each is differentiable (once); ``causal_conv_step`` and ``selective_scan_step`` 
 may be float32, bfloat16 or float16 and any strided view (a copy is made only where the last dimension is not dense); states of the scan,
 its A / skip / dt_bias and the convolution's weights are float32.  ``reset`` [T, rows] (bool or uint8) marks the steps at which a new sequence
 begins: several sequences can share a row, and left padding is dropped by a reset at the first real step.  Calls run on the current
-stream of the tensors' device, never synchronise, and can be captured into a graph.  Wrong types, shapes or devices raise ValueError, a failed
+stream of the tensors' device, never synchronise, and can be captured into a graph (a captured backward pass raises while an eager graph of the same
+leaves is alive on the default stream).  Wrong types, shapes or devices raise ValueError, a failed
 launch FdqlError.  All compute is in libfdql_hip.so; there is no CPU path."""
 import ctypes as C
 
@@ -65,7 +66,8 @@ def selective_scan(x, dt, A, B, C, *, skip=None, z=None, dt_bias=None, dt_softpl
 
 def selective_scan_step(x, dt, A, B, C, state, *, skip=None, z=None, dt_bias=None, dt_softplus=True, reset=None, out_state=None):
     """One step of selective_scan for every row: x, dt, z [rows, D], B, C [rows, (groups,) n], state [rows, D, n], reset [rows].  Returns
-    (y, new state); the new state is written to out_state (rows dense, any distance apart; `state` itself updates it in place, other overlaps are not allowed) or to a new tensor."""
+    (y, new state); the new state is written to out_state (rows dense, any distance apart; `state` itself
+    updates it in place, other overlaps are not allowed) or to a new tensor."""
     return (_bound or _ops()).selective_scan_step(x, dt, A, B, C, state, skip, z, dt_bias, dt_softplus, reset, out_state)
 
 

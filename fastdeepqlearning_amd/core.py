@@ -359,6 +359,8 @@ class NativeAgent:
                     b.obs_2d_slots = sl.data_ptr()
                 continue
             assert t.is_cuda and t.dtype == torch.float32, f"batch[{k}] must be a float32 device tensor"
+            if k == "agent_state" and self.cfg.joiner_ssm and (t.shape[-1] != self.state_floats() or t.numel() < self.cfg.B * t.shape[-1]):
+                raise ValueError(f"batch[agent_state] must be [T, {self.cfg.B}, {self.state_floats()}], got {tuple(t.shape)}")
             t = t.contiguous()
             keep.append(t)
             setattr(b, k, t.data_ptr())

@@ -46,7 +46,7 @@ int check_conv(const fdql_causal_conv_t *p) {
 int check_scan(const fdql_scan_t *p) {
   FDQL_REQUIRE(p && p->size == (int32_t)sizeof(*p), "scan: struct size %d, this library has %d", p ? p->size : 0, (int)sizeof(*p));
   FDQL_REQUIRE(type_ok(p->dtype), "scan: dtype %d (float32, bf16 or fp16)", p->dtype);
-  FDQL_REQUIRE(p->T >= 0 && p->R >= 0 && p->D >= 1, "scan: T %d, R %d, D %d", p->T, p->R, p->D);
+  FDQL_REQUIRE(p->T >= 0 && p->T <= 1 << 30 && p->R >= 0 && p->D >= 1, "scan: T %d (up to 2^30), R %d, D %d", p->T, p->R, p->D);
   FDQL_REQUIRE(p->N >= 1 && p->N <= 64, "scan: %d states (1 to 64)", p->N);
   FDQL_REQUIRE(p->G >= 1 && p->D % p->G == 0, "scan: %d groups do not divide %d channels", p->G, p->D);
   // waves of 16 channels (a time axis cut into segments: 10240 of them at most), 16 of the joining kernel's each; 18 finish workgroups of 1024 threads

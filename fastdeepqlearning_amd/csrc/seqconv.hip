@@ -326,7 +326,7 @@ Plan plan_of(const fdql_causal_conv_t &p, int V) {
   q.V = V;
   q.blocks = (p.D + 64 * V - 1) / (64 * V);
   // Chunks of 64 steps, halved down to 8 while there are fewer than 2048 waves: each reads K - 1 steps of its neighbour again.  bf16 forward, 4099
-  // steps of 3 x 1000: 16.7 us against 18.0 at 1024 waves and 16.8 at 3072; 16384 steps of 1 x 1024: 19.5 against 21.8 and 21.4.
+  // steps of 3 x 1000: 16.7 us against 18.0 at 1024 waves and 16.7 at 4096; 16384 steps of 1 x 1024: 19.5 against 21.8 and 21.3.
   q.len = 64;
   while (q.len > 8 && (int64_t)q.blocks * p.R * ((p.T + q.len - 1) / q.len) < 2048) q.len >>= 1;
   q.chunks = std::max(1, (p.T + q.len - 1) / q.len);

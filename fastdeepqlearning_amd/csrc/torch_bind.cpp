@@ -107,7 +107,11 @@ void written(const Tensor &t) {
 void capturable(const char *what, const Tensor &x) {
   const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index());
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) {
+    (void)hipGetLastError();                // (no stream that could be captured: the next launch must not find this error)
+    return;
+  }
+  if (status == hipStreamCaptureStatusNone) return;
   const c10::Stream here = stream.unwrap(), eager = c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(x.device().index()).unwrap();
   const auto node = torch::autograd::get_current_node();
   const auto *runs = torch::autograd::get_current_graph_task_exec_info();       // empty: every node does

@@ -95,7 +95,7 @@ def test_graph_mode_equals_eager(dev, mode):
     assert torch.equal(out[0], out[1])
 
 
-@pytest.mark.parametrize("rows,kw", [(1, {}), (5, {}), (33, {}), (300, {}), (9, dict(ssm_inner=37, ssm_state=5)), (17, dict(discrete=True, act=5)),
+@pytest.mark.parametrize("rows,kw", [(1, {}), (5, {}), (33, {}), (300, {}), (9, dict(ssm_inner=37, ssm_state=5)), (40, dict(ssm_inner=37, ssm_state=5)), (17, dict(discrete=True, act=5)),
                                      (3, dict(ssm_inner=600, ssm_state=64, latent=256))])
 def test_act_matches_oracle(dev, rows, kw):
     from oracle import update as oup
@@ -201,3 +201,18 @@ def test_agent_life_cycle(dev):
         ec.joiner_mode = ec.JoinerModeEnum.feedforward      # EncoderConf attributes are class-level defaults
         ec.ssm_inner_dim, ec.ssm_state_dim = 0, 16
         ec.rnn_latent_state_training_mode = ec.RnnLatentStateTrainMode.zero
+
+
+def test_stored_states_of_another_width_are_refused(dev):
+    from oracle import update as oup
+    spec = oup.Spec(obs=9, act=3, C=2, Q=3, T=4, B=8, ssm="store", **NETS)
+    ag = _agent(spec, dev)
+    ag.load_tensors(oup.init_params(spec, seed=1))
+    xp, nt, na = _batch(spec, torch.Generator().manual_seed(1))
+    xp = {k: v.to(dev) for k, v in xp.items()}
+    for bad in (torch.zeros(4, 8, spec.latent, device=dev), xp["agent_state"][:, :3].contiguous()[:1]):
+        with pytest.raises(ValueError, match="agent_state"):
+            ag.update(dict(xp, agent_state=bad), nt.to(dev), na.to(dev))
+    del xp["agent_state"]
+    with pytest.raises(Exception, match="agent_state"):
+        ag.update(xp, nt.to(dev), na.to(dev))

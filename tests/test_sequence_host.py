@@ -165,3 +165,10 @@ def test_more_channels_than_the_finish_kernels_take_are_refused():
     assert lib.fdql_scan_workspace_bytes(C.byref(_scan(R=1, D=1 << 22)), 1) == nat.FDQL_EINVAL
     assert "one launch" in lib.fdql_last_error().decode()
     assert lib.fdql_scan_workspace_bytes(C.byref(_scan(R=1, D=1 << 21)), 1) > 0
+
+
+def test_windows_longer_than_the_step_index_are_refused():
+    lib = nat.load()
+    assert lib.fdql_scan_workspace_bytes(C.byref(_scan(T=2**31 - 1, R=1, D=1, N=1)), 0) == nat.FDQL_EINVAL
+    assert "2^30" in lib.fdql_last_error().decode()
+    assert lib.fdql_scan_workspace_bytes(C.byref(_scan(T=2**30, R=1, D=1, N=1)), 0) > 0

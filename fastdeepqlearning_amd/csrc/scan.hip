@@ -21,7 +21,7 @@
 // walks the tile in reverse with g_t = carry + C_t dy_t, carry <- e^(delta A) g_t.  dB and dC sum over channels, 4 values per step, lane and
 // pass: permlane swaps halve the values while they add (v_permlane32_swap exchanges half of one register's lanes with half of another's),
 // two DPP rotations finish - a channel's parts are neighbouring lanes so that these steps need no selects; then the workgroup's waves meet in
-// LDS, the workgroups in a slab that k_scan_bc_finish adds up.  No atomics: results repeat bit by bit.  (One-hot v_mfma_f32_16x16x4 products
+// LDS, the workgroups in a slab that k_scan_finish adds up.  No atomics: results repeat bit by bit.  (One-hot v_mfma_f32_16x16x4 products
 // for these sums measured slower, 190 us against 126 at 50 x 256 x 512 x 16: float32 matrix instructions and vector arithmetic do not overlap.)
 #include "seq.h"
 
@@ -649,28 +649,30 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
   a.part_s[o / NL * 2 + 64 + lane] = dbias;
 }
 
-// dB / dC: the workgroups' slabs added in order, rounded once to the tensor's type.
-template <typename T>
-__global__ __launch_bounds__(256) void k_scan_bc_finish(Args a) {
-  const int64_t n = (int64_t)a.p.T * a.p.R * a.p.G * a.p.N;
-  const float *slab = blockIdx.y ? a.slab_c : a.slab_b;
-  T *out = reinterpret_cast<T *>(blockIdx.y ? a.p.dC : a.p.dB);
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
-    float v = 0.f;
-    for (int k = 0; k < a.wgt; ++k) v += slab[k * n + i];
-    out[i] = from_f<T>(v);
-  }
-}
-
-// dA, dskip, ddt_bias: partials of the (segment, row) pairs added up; a workgroup per 64 lanes of one state, 16 slices of the pairs.
-template <int NL>
-__global__ __launch_bounds__(1024) void k_scan_par_finish(Args a) {
+// Joins the workgroups' parts.  blockIdx.x < nbc: dB / dC, the slabs added in order, rounded once to the tensor's type.  Behind them: dA, dskip, ddt_bias,
+// partials of the (segment, row) pairs added up, a workgroup per 64 lanes of one state, 16 slices of the pairs.  (One launch: as two, one behind the
+// other, 5 + 7.5 us at 50 x 256 x 512.)
+template <typename T, int NL>
+__global__ __launch_bounds__(1024) void k_scan_finish(Args a, int nbc) {
   __shared__ float red[16][64];
   const fdql_scan_t &p = a.p;
-  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6;
-  const int j = blockIdx.x % (NL + 2), blk = blockIdx.x / (NL + 2);
+  if ((int)blockIdx.x < nbc) {
+    const int64_t n = (int64_t)p.T * p.R * p.G * p.N;
+    for (int64_t k = (int64_t)blockIdx.x * 1024 + threadIdx.x; k < 2 * n; k += (int64_t)nbc * 1024) {
+      const int64_t i = k < n ? k : k - n;
+      const float *slab = k < n ? a.slab_b : a.slab_c;
+      float v = 0.f;
+#pragma unroll 8
+      for (int q = 0; q < a.wgt; ++q) v += slab[q * n + i];
+      reinterpret_cast<T *>(k < n ? p.dB : p.dC)[i] = from_f<T>(v);
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 63, slice = threadIdx.x >> 6, u = blockIdx.x - nbc;
+  const int j = u % (NL + 2), blk = u / (NL + 2);
   const int64_t pairs = (int64_t)a.nseg * p.R, blocks = (int64_t)p.G * a.tpg;
   float v = 0.f;
+#pragma unroll 8
   for (int64_t k = slice; k < pairs; k += 16)
     v += j < NL ? a.part_a[((k * blocks + blk) * NL + j) * 64 + lane] : a.part_s[((k * blocks + blk) * 2 + j - NL) * 64 + lane];
   red[slice][lane] = v;
@@ -881,9 +883,9 @@ hipError_t bwd(const fdql_scan_t &p, hipStream_t s) {
       hipLaunchKernelGGL((k_scan_combine<NL, 1>), dim3((unsigned)(per * NL)), dim3(64), 0, s, a);
     }
     hipLaunchKernelGGL((k_scan_bwd<T, NL>), dim3((unsigned)((int64_t)q.nseg * p.R * p.G * q.wgt)), dim3(q.wpw * 64), 0, s, a);
-    const int64_t bc = (int64_t)p.T * p.R * p.G * p.N;
-    hipLaunchKernelGGL((k_scan_bc_finish<T>), dim3((unsigned)std::min<int64_t>((bc + 255) / 256, 8 * CUS), 2), dim3(256), 0, s, a);
-    hipLaunchKernelGGL((k_scan_par_finish<NL>), dim3((unsigned)(p.G * q.tpg * (NL + 2))), dim3(1024), 0, s, a);
+    const int64_t bc = 2ll * p.T * p.R * p.G * p.N;
+    const int nbc = (int)std::min<int64_t>((bc + 1023) / 1024, 4 * CUS);
+    hipLaunchKernelGGL((k_scan_finish<T, NL>), dim3((unsigned)(nbc + p.G * q.tpg * (NL + 2))), dim3(1024), 0, s, a, nbc);
     return hipGetLastError();
   });
 }

@@ -51,7 +51,7 @@ int check_scan(const fdql_scan_t *p) {
   FDQL_REQUIRE(p->G >= 1 && p->D % p->G == 0, "scan: %d groups do not divide %d channels", p->G, p->D);
   // waves of 16 channels (a time axis cut into segments: 10240 of them at most), 16 of the joining kernel's each; 18 finish workgroups of 1024 threads
   const int64_t tiles = (int64_t)p->G * ((p->D / p->G + 15) / 16);
-  FDQL_REQUIRE((p->R * tiles + 10240) * 64 * 16 < MAX_THREADS && tiles * 18 * 1024 < MAX_THREADS, "scan: R %d x D %d is more than one launch", p->R, p->D);
+  FDQL_REQUIRE((p->R * tiles + 10240) * 64 * 16 < MAX_THREADS && (tiles * 18 + 1024) * 1024 < MAX_THREADS, "scan: R %d x D %d is more than one launch", p->R, p->D);
   return FDQL_OK;
 }
 int check_gated(const fdql_gated_t *p) {

@@ -3,8 +3,8 @@
 // Forward: one matrix product against both weights, with the activation, the product and the biases in its epilogue - a wave's accumulators
 // hold the gate and the up column of the same 32 outputs, so both meet in one lane and neither is stored (training keeps them in
 // float32 for the backward pass: rounded to 16 bits they would cost the gradients a bit more than their own rounding does).
-// Backward: an elementwise pass forms dg = dy u f'(g), du = dy f(g) (rounded to the operand type the matrix instructions take) and
-// their column sums; then dx = dg Wg + du Wu is one product over 2 F, and dWg = dg^T x, dWu = du^T x are one launch with the rows
+// Backward: an elementwise pass forms dg = dy u f'(g), du = dy f(g) in the operand type the matrix instructions take (16-bit types: in two parts
+// whose sum has twice the digits, see Plan) and their column sums; then dx = dg Wg + du Wu is one product over 2 F, and dWg = dg^T x, dWu = du^T x are one launch with the rows
 // split over workgroups where the weights alone leave the card idle (float32 slabs, added in order).
 //
 // k_gated_mma serves all three products: tiles of BM x BN, slices of the contraction in an LDS ring filled by LDS-DMA (see there).  Rows that are
@@ -229,17 +229,16 @@ __device__ __forceinline__ void clear(v16f (&acc)[MT][2]) {
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 }
 
-// The backward products pass over their contraction once for every part of d, DX for the gate's side, then the up side's.
-// PARTS: there may be two of them (the tiles of 256 columns are never given such a problem).
-template <int MODE, bool PARTS>
-__device__ __forceinline__ int passes_of(const Args &a) { return (MODE == DX ? 2 : 1) * (PARTS && MODE != FWD ? a.parts : 1); }
-template <int MODE, bool PARTS>
+// The backward products pass over their contraction once for each of d's PARTS, DX for the gate's side, then the up side's.
+template <int MODE, int PARTS>
+constexpr int passes_of() { return MODE == FWD ? 1 : MODE == DX ? 2 * PARTS : PARTS; }
+template <int MODE, int PARTS>
 __device__ __forceinline__ int pass_of(int step, int len) {
-  if (PARTS && MODE != FWD) return (step >= len) + (step >= 2 * len) + (step >= 3 * len);
-  return MODE == DX && step >= len;
+  constexpr int N = passes_of<MODE, PARTS>();
+  return N == 1 ? 0 : N == 2 ? step >= len : (step >= len) + (step >= 2 * len) + (step >= 3 * len);
 }
-template <int MODE, bool PARTS>
-__device__ __forceinline__ int side_of(const Args &a, int pass) { return MODE != DX ? 0 : PARTS && a.parts == 2 ? pass >> 1 : pass; }
+template <int MODE, int PARTS>
+__device__ __forceinline__ int side_of(int pass) { return MODE == DX ? pass / PARTS : 0; }
 
 // Float sums over a long contraction: RUN slices (512 products) at a time, the runs added up apart, so that the rounding error grows with the run's
 // length and their number instead of the whole length (dx at F 2000: 1.2e-6 of its norm in one chain).  16-bit results round at 2^-12
@@ -278,10 +277,9 @@ struct Runs {
 
 // 64 x 128 tiles for any alignment: slices of 128 bytes through registers into two LDS buffers, operands that lie across the contraction
 // transposed on the way.
-template <typename T, int MODE>
+template <typename T, int MODE, int PARTS>
 __global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
   constexpr int BM = 64, BN = 128, BK = 128 / sizeof(T);
-  constexpr bool PARTS = sizeof(T) == 2;
   __shared__ __align__(16) char lds[2][(BM + BN) * 128];
   const fdql_gated_t &p = a.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 1, wn = wave & 1;
@@ -290,9 +288,9 @@ __global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
   const int64_t M = p.M, D = p.D, F = p.F, m0 = (int64_t)tm * BM, f0 = (int64_t)tn * (BN / 2), n0 = (int64_t)tn * BN;
   const int which = MODE == DW ? blockIdx.y : 0, ks = MODE == DW ? blockIdx.z : 0;
   const T *x = reinterpret_cast<const T *>(p.x), *wg = reinterpret_cast<const T *>(p.w_gate), *wu = reinterpret_cast<const T *>(p.w_up);
-  const T *dd = reinterpret_cast<const T *>(a.d) + (MODE == DW ? which * a.parts * M * a.Fp : 0);
+  const T *dd = reinterpret_cast<const T *>(a.d) + (MODE == DW ? which * PARTS * M * a.Fp : 0);
   const int64_t kbeg = MODE == DW ? (int64_t)ks * a.kper : 0, kend = MODE == FWD ? D : MODE == DX ? F : min(M, kbeg + a.kper);
-  const int half = (int)((kend - kbeg + BK - 1) / BK), steps = passes_of<MODE, PARTS>(a) * half;
+  const int half = (int)((kend - kbeg + BK - 1) / BK), steps = passes_of<MODE, PARTS>() * half;
 
   Flight<2> fa;
   Flight<4> fb;
@@ -305,7 +303,7 @@ __global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
         return f < F ? (n & 32 ? wu : wg) + f * D : (const T *)nullptr;
       }, k0, D);
     } else if constexpr (MODE == DX) {
-      const int pass = pass_of<MODE, PARTS>(step, half), up = side_of<MODE, PARTS>(a, pass);
+      const int pass = pass_of<MODE, PARTS>(step, half), up = side_of<MODE, PARTS>(pass);
       const int64_t k0 = (int64_t)(step - pass * half) * BK;
       const T *src = dd + pass * M * a.Fp;
       fetch_rows<T>(fa, [&](int n) { return m0 + n < M ? src + (m0 + n) * a.Fp : (const T *)nullptr; }, k0, F);
@@ -402,10 +400,9 @@ __device__ __forceinline__ int2 tr_read(const char *p) {
   return __builtin_bit_cast(int2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4s *)p));
 }
 
-template <typename T, int MODE, int BM, int BN>
+template <typename T, int MODE, int BM, int BN, int PARTS>
 __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
   typedef Ring<T, BM, BN> R;
-  constexpr bool PARTS = sizeof(T) == 2 && BN == 128;
   constexpr int KS = R::KS, NBUF = R::NBUF, ABYTES = R::ABYTES, BBYTES = R::BBYTES, E = 16 / sizeof(T), RB = KS * sizeof(T), WAVES = BN / 32;
   constexpr int MT = BM / 64, NT = 2, NA = ABYTES / (WAVES * 1024), NB = BBYTES / (WAVES * 1024), KSTEPS = RB / 32;
   typedef RowTile<RB> Rows;
@@ -419,10 +416,10 @@ __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
   const int64_t M = p.M, D = p.D, F = p.F, m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN, f0 = (int64_t)tn * (BN / 2);
   const int which = MODE == DW ? blockIdx.y : 0, ks = MODE == DW ? blockIdx.z : 0;
   const T *x = reinterpret_cast<const T *>(p.x), *wg = reinterpret_cast<const T *>(p.w_gate), *wu = reinterpret_cast<const T *>(p.w_up);
-  const T *dd = reinterpret_cast<const T *>(a.d) + which * (PARTS ? a.parts : 1) * M * a.Fp;
+  const T *dd = reinterpret_cast<const T *>(a.d) + which * PARTS * M * a.Fp;
   // contraction [kbeg, K) of one pass
   const int64_t kbeg = MODE == DW ? (int64_t)ks * a.kper : 0, K = MODE == FWD ? a.Dk : MODE == DX ? a.Fp : min(M, kbeg + a.kper);
-  const int half = (int)((K - kbeg + KS - 1) / KS), steps = passes_of<MODE, PARTS>(a) * half;
+  const int half = (int)((K - kbeg + KS - 1) / KS), steps = passes_of<MODE, PARTS>() * half;
 
   // where this lane's chunks come from: an element offset from the operand's start for slice 0, and the chunk's place in the contraction
   int64_t oa[NA], ob[NB];
@@ -462,7 +459,7 @@ __global__ __launch_bounds__(BN * 2, 2) void k_gated_mma(Args a) {
   // piece `piece` of `pieces` of a slice's DMA (a wave is held up while its requests are taken: in one go, with the other waves', that left the
   // matrix unit idle for a quarter of a step)
   const auto fetch = [&](int step, int buf, int piece, int pieces) {
-    const int pass = pass_of<MODE, PARTS>(step, half), up = side_of<MODE, PARTS>(a, pass);
+    const int pass = pass_of<MODE, PARTS>(step, half), up = side_of<MODE, PARTS>(pass);
     const int64_t k0 = kbeg + (int64_t)(step - pass * half) * KS;
     const unsigned la = lds_addr(lds) + buf * (ABYTES + BBYTES) + wave * NA * 1024, lb = lds_addr(lds) + buf * (ABYTES + BBYTES) + ABYTES + wave * NB * 1024;
     const T *pa = MODE == FWD ? x + k0 : MODE == DX ? dd + pass * M * a.Fp + k0 : dd + pass * M * a.Fp + k0 * a.Fp;
@@ -766,9 +763,9 @@ Shape shape_of(Choice choice, int64_t rows, int64_t cols, int tile_of_256, int c
   return s;
 }
 
-// Rounding d to 16 bits adds as much to the gradients' error as rounding the results does: sqrt(2) of it over many elements, more by chance over few.
-// So small problems keep d in two parts, which puts a second pass into products that their launches dominate; large ones would
-// pay for it (8192 x 1024 x 4096: twice 350 us).
+// Rounding d to 16 bits once would add as much to the gradients' error as rounding the results does (8192 x 1024 x 4096, bf16: 0.0023 of their norm
+// instead of 0.0017), so it is kept in two parts, whatever the size, and each part has its pass in the products: 896 us a training pass there against 564.
+// A caller who would rather have the time asks for one part (FDQL_GATED_ROUND_GRADS).
 struct Plan {
   int Fp, parts, ksplit, kper;
   int64_t rblocks;
@@ -776,8 +773,7 @@ struct Plan {
 Plan plan_of(const fdql_gated_t &p) {
   Plan q;
   q.Fp = (p.F + 7) / 8 * 8;
-  const int64_t few = std::min((int64_t)p.F * p.D, std::min(p.M * p.F, p.M * p.D));
-  q.parts = p.dtype != FDQL_F32 && few < 8192 && p.M * p.F <= 1 << 20 ? 2 : 1;
+  q.parts = p.dtype == FDQL_F32 || (p.act & FDQL_GATED_ROUND_GRADS) ? 1 : 2;
   q.rblocks = (p.M + RB - 1) / RB;
   // rows split for the 64 x 128 tiles of the weight gradients (larger tiles are chosen where there are enough of them): slices of 256 rows and
   // more, up to three workgroups per CU of float (backward of 4096 x 1024 x 1024 324 us, with two 330, one 369) and two of 16 bits, whose
@@ -826,46 +822,54 @@ hipError_t pack(Args &a, hipStream_t s) {
 }
 
 template <typename T, int MODE>
-Choice choice_of(const Args &a, bool aligned) {
-  if (!aligned || a.parts == 2) return SMALL;
+Choice choice_of(bool aligned) {
+  if (!aligned) return SMALL;
   return sizeof(T) == 2 ? WIDE : MODE == DW ? SMALL : FLOAT;
 }
 
-template <typename T, int MODE, int BM, int BN>
+template <typename T, int MODE, int BM, int BN, int PARTS>
 hipError_t launch_mma(const Args &a, dim3 grid, hipStream_t s) {
   constexpr int bytes = Ring<T, BM, BN>::BYTES;
-  const hipError_t e = hipFuncSetAttribute((const void *)k_gated_mma<T, MODE, BM, BN>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  const hipError_t e = hipFuncSetAttribute((const void *)k_gated_mma<T, MODE, BM, BN, PARTS>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((k_gated_mma<T, MODE, BM, BN>), grid, dim3(BN * 2), bytes, s, a);
+  hipLaunchKernelGGL((k_gated_mma<T, MODE, BM, BN, PARTS>), grid, dim3(BN * 2), bytes, s, a);
   return hipGetLastError();
+}
+template <typename T, int MODE, int PARTS>
+hipError_t launch_tiles(const Args &a, const Shape &q, bool aligned, dim3 grid, hipStream_t s) {
+  if (!aligned) {
+    hipLaunchKernelGGL((k_gated_any<T, MODE, PARTS>), grid, dim3(256), 0, s, a);
+    return hipGetLastError();
+  }
+  if constexpr (sizeof(T) == 2) {
+    if (q.bm == 256) return launch_mma<T, MODE, 256, 256, PARTS>(a, grid, s);
+    if (q.bm == 128) return launch_mma<T, MODE, 128, 256, PARTS>(a, grid, s);
+  }
+  if constexpr (sizeof(T) == 4 && MODE != DW) {
+    if (q.bm == 128) return launch_mma<T, MODE, 128, 128, PARTS>(a, grid, s);
+  }
+  return launch_mma<T, MODE, 64, 128, PARTS>(a, grid, s);
 }
 // rows x cols of the product's result; aligned: every operand row is made of whole 16-byte chunks
 template <typename T, int MODE>
 hipError_t product(Args a, int64_t rows, int64_t cols, bool aligned, hipStream_t s) {
   const int copies = MODE == DW ? 2 : 1;
-  const Shape q = shape_of(choice_of<T, MODE>(a, aligned), rows, cols, MODE == FWD ? 128 : 256, copies);
+  const Shape q = shape_of(choice_of<T, MODE>(aligned), rows, cols, MODE == FWD ? 128 : 256, copies);
   a.tiles_m = (int)q.tiles_m;
   a.tiles_n = (int)q.tiles_n;
   if (MODE == DW && q.bn == 256) a.ksplit = 1, a.kper = (int)((a.p.M + 63) / 64 * 64);
   const dim3 grid((unsigned)(q.tiles_m * q.tiles_n), copies, MODE == DW ? (unsigned)a.ksplit : 1);
-  if (!aligned) {
-    hipLaunchKernelGGL((k_gated_any<T, MODE>), grid, dim3(256), 0, s, a);
-    return hipGetLastError();
+  if constexpr (sizeof(T) == 2 && MODE != FWD) {
+    if (a.parts == 2) return launch_tiles<T, MODE, 2>(a, q, aligned, grid, s);
   }
-  if constexpr (sizeof(T) == 2) {
-    if (q.bm == 256) return launch_mma<T, MODE, 256, 256>(a, grid, s);
-    if (q.bm == 128) return launch_mma<T, MODE, 128, 256>(a, grid, s);
-  }
-  if constexpr (sizeof(T) == 4 && MODE != DW) {
-    if (q.bm == 128) return launch_mma<T, MODE, 128, 128>(a, grid, s);
-  }
-  return launch_mma<T, MODE, 64, 128>(a, grid, s);
+  return launch_tiles<T, MODE, 1>(a, q, aligned, grid, s);
 }
 
 template <typename T>
 hipError_t fwd(const fdql_gated_t &p, hipStream_t s) {
   Args a = {};
   a.p = p;
+  a.p.act &= ~FDQL_GATED_ROUND_GRADS;
   constexpr int E = 16 / sizeof(T);
   const hipError_t e = pack<T>(a, s);
   if (e != hipSuccess) return e;
@@ -883,6 +887,7 @@ hipError_t bwd(const fdql_gated_t &p, hipStream_t s) {
   const Plan q = plan_of(p);
   Args a = {};
   a.p = p;
+  a.p.act &= ~FDQL_GATED_ROUND_GRADS;
   a.Fp = q.Fp;
   a.parts = q.parts;
   hipError_t e = pack<T>(a, s);
@@ -899,7 +904,7 @@ hipError_t bwd(const fdql_gated_t &p, hipStream_t s) {
   e = hipGetLastError();
   if (e == hipSuccess && p.dx) e = product<T, DX>(a, p.M, p.D, a.ldw % E == 0 && al16(a.p.w_gate) && al16(a.p.w_up), s);
   const bool w = p.dw_gate && p.dw_up, vec = a.ldw % E == 0 && a.p.x_sr % E == 0 && al16(a.p.x);
-  if (w && shape_of(choice_of<T, DW>(a, vec), p.F, p.D, 256, 2).bn == 256) a.ksplit = 1;
+  if (w && shape_of(choice_of<T, DW>(vec), p.F, p.D, 256, 2).bn == 256) a.ksplit = 1;
   if (e == hipSuccess && w) e = product<T, DW>(a, p.F, p.D, vec, s);
   const bool sum_w = w && a.ksplit > 1;
   if (e == hipSuccess && (sum_w || p.db_gate || p.db_up)) {

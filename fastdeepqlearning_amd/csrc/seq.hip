@@ -58,7 +58,8 @@ int check_gated(const fdql_gated_t *p) {
   FDQL_REQUIRE(p && p->size == (int32_t)sizeof(*p), "gated: struct size %d, this library has %d", p ? p->size : 0, (int)sizeof(*p));
   FDQL_REQUIRE(type_ok(p->dtype), "gated: dtype %d (float32, bf16 or fp16)", p->dtype);
   FDQL_REQUIRE(p->M >= 0 && p->D >= 1 && p->F >= 1 && p->D <= 1 << 24 && p->F <= 1 << 24, "gated: M %lld, D %d, F %d (D and F up to 2^24)", (long long)p->M, p->D, p->F);
-  FDQL_REQUIRE(p->act >= FDQL_ACT_SILU && p->act <= FDQL_ACT_SIGMOID, "gated: activation %d", p->act);
+  const int32_t act = p->act & ~FDQL_GATED_ROUND_GRADS;
+  FDQL_REQUIRE(act >= FDQL_ACT_SILU && act <= FDQL_ACT_SIGMOID, "gated: activation %d", p->act);
   FDQL_REQUIRE(p->M <= 128ll * 65535 && (p->M / 64 + 1) * ((int64_t)(p->F > p->D ? p->F : p->D) / 64 + 1) * 256 < MAX_THREADS,
                "gated: M %lld x (D %d, F %d) is more than one launch", (long long)p->M, p->D, p->F);
   FDQL_REQUIRE(((int64_t)p->F / 128 + 1) * (p->D / 128 + 1) * 256 * 2 < MAX_THREADS / 16, "gated: weights %d x %d are more than one launch", p->F, p->D);

@@ -20,6 +20,7 @@ from . import _native as N
 __all__ = ["causal_conv", "causal_conv_step", "selective_scan", "selective_scan_step", "gated_linear"]
 
 _ACTS = {"silu": 0, "gelu": 1, "sigmoid": 2}
+_ROUND_GRADS = 0x100
 _bound = None
 
 
@@ -71,12 +72,14 @@ def selective_scan_step(x, dt, A, B, C, state, *, skip=None, z=None, dt_bias=Non
     return (_bound or _ops()).selective_scan_step(x, dt, A, B, C, state, skip, z, dt_bias, dt_softplus, reset, out_state)
 
 
-def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, *, activation="silu"):
+def gated_linear(x, w_gate, w_up, b_gate=None, b_up=None, *, activation="silu", rounded_grads=False):
     """f(x w_gate^T + b_gate) * (x w_up^T + b_up), f = "silu", "gelu" (erf form) or "sigmoid".
 
-    x [..., D], weights [F, D], biases [F] (both or neither), all of one type; returns [..., F].  Sums are float32; the backward pass rounds
-    the two pre-activation gradients once to the type before its products."""
+    x [..., D], weights [F, D], biases [F] (both or neither), all of one type; returns [..., F].  Sums are float32.  The backward pass of
+    the 16-bit types keeps the two pre-activation gradients in two parts of the type, so that the gradients are rounded once, at the end;
+    rounded_grads=True rounds them before its products too, which halves the products' work and makes the gradients' error about sqrt(2) times as
+    large.  In float16 a pre-activation gradient beyond 65504 counts as infinite (choose the loss scale for it)."""
     act = _ACTS.get(activation)
     if act is None:
         raise ValueError(f"gated_linear: activation must be one of {sorted(_ACTS)}, got {activation!r}")
-    return (_bound or _ops()).gated_linear(x, w_gate, w_up, b_gate, b_up, act)
+    return (_bound or _ops()).gated_linear(x, w_gate, w_up, b_gate, b_up, act | (_ROUND_GRADS if rounded_grads else 0))

@@ -514,10 +514,15 @@ int fdql_scan_backward(const fdql_scan_t *p, void *stream);
 /* y = f(x Wg^T + bg) * (x Wu^T + bu), f = SiLU, GELU (the erf form) or sigmoid; x [M, D] (row stride x_sr), weights [F, D] dense, y [M, F] dense.
  * pre: [2, M, F] float32 (or NULL) that the forward call fills with both products for the backward call.
  * Rows of x or of the weights that are not whole 16-byte chunks are copied into the workspace first (both directions ask for one then).
- * Backward: dy [M, F] (row stride dy_sr) -> dx [M, D], dw_gate, dw_up [F, D], db_gate, db_up [F] (each or NULL), all of the type dtype.            */
+ * Backward: dy [M, F] (row stride dy_sr) -> dx [M, D], dw_gate, dw_up [F, D], db_gate, db_up [F] (each or NULL), all of the type dtype.
+ * The matrix instructions of the 16-bit types take the gradients of the two products' results, dg and du, in 16 bits: they are kept in two parts whose
+ * sum has twice the digits, for every size.  FDQL_GATED_ROUND_GRADS added to act in the backward call (and its workspace query) rounds them once
+ * instead: half the matrix work of the backward pass, and gradients whose error is about sqrt(2) times as large.  In fp16 either way a dg or du beyond
+ * 65504 counts as infinite (choose the loss scale for it).                                                                             */
 #define FDQL_ACT_SILU 0
 #define FDQL_ACT_GELU 1
 #define FDQL_ACT_SIGMOID 2
+#define FDQL_GATED_ROUND_GRADS 0x100
 typedef struct {
   int32_t size, dtype;
   int64_t M;

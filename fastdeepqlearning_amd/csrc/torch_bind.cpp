@@ -135,10 +135,14 @@ void capturable(const char *what, const Tensor &x) {
     }
   }
 }
-// Gradients of a backward pass that itself is recorded (create_graph): differentiating them again is an error, not a silent zero.
-variable_list once(const char *what, variable_list grads) {
+// Gradients of a backward pass that itself is recorded (create_graph) depend on everything in `from`: differentiating them again is an error, not a silent
+// zero.
+variable_list once(const char *what, variable_list grads, const variable_list &from, const variable_list &incoming) {
   if (!at::GradMode::is_enabled()) return grads;
-  return (*std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is differentiable once", (int64_t)grads.size()))(std::move(grads));
+  const auto error = std::make_shared<torch::autograd::Error>(std::string(what) + " is differentiable once", torch::autograd::collect_next_edges(from, incoming));
+  for (Tensor &g : grads)
+    if (g.defined()) torch::autograd::create_gradient_edge(g, error);
+  return grads;
 }
 
 // Which of a node's tensor arguments want a gradient: the node numbers those that are there.
@@ -219,7 +223,7 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
     p.workspace = ptr(ws);
     p.workspace_bytes = ws.defined() ? ws.numel() : 0;
     check(api.conv_bwd(&p, stream_of(x)));
-    return once("causal_conv", {dx, dw, db, ds, Tensor(), Tensor(), Tensor()});
+    return once("causal_conv", {dx, dw, db, ds, Tensor(), Tensor(), Tensor()}, s, g);
   }
 };
 void conv_check(const char *what, const Tensor &x, const Tensor &weight, const Tensor &bias, const Tensor &state) {
@@ -344,7 +348,7 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
     for (int k = 0; k < 9; ++k)
       if (!need.on[k]) d[k] = Tensor();
     d.resize(12);
-    return once("selective_scan", std::move(d));
+    return once("selective_scan", std::move(d), s, g);
   }
 };
 // checks everything; B and C come back with their group dimension
@@ -455,7 +459,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
     for (int k = 1; k < 5; ++k)
       if (!need.on[k]) d[k] = Tensor();
     d.resize(6);
-    return once("gated_linear", std::move(d));
+    return once("gated_linear", std::move(d), s, g);
   }
 };
 Tensor gated_linear(const Tensor &x, const Tensor &wg, const Tensor &wu, const Opt &bg_, const Opt &bu_, int64_t act) {

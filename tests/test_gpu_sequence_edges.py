@@ -32,3 +32,28 @@ def test_gated_gradients_round_once_at_every_size(dev, seq, M, D, F, dtype):
     print(M, D, F, dtype, ratio)
     assert max(ratio[False]) <= 1.05, ratio
     assert max(ratio[True]) <= 1.6 and min(ratio[True]) > 1.1, ratio
+
+
+def _graded_calls(dev, seq):
+    """(operator, output, leaves) of the three operators on small inputs."""
+    g = _gen(3)
+    r = lambda *s: torch.randn(*s, generator=g).to(dev).requires_grad_()  # noqa: E731
+    x, w, b, st = r(5, 2, 8), r(8, 4), r(8), r(2, 3, 8)
+    yield "causal_conv", seq.causal_conv(x, w, b, initial_state=st), [x, w, b, st]
+    x, dt, A, B, C, h = r(5, 2, 8), r(5, 2, 8), (-torch.rand(8, 4, generator=g)).to(dev).requires_grad_(), r(5, 2, 4), r(5, 2, 4), r(2, 8, 4)
+    yield "selective_scan", seq.selective_scan(x, dt, A, B, C, initial_state=h), [x, dt, A, B, C, h]
+    x, wg, wu = r(6, 8), r(5, 8), r(5, 8)
+    yield "gated_linear", seq.gated_linear(x, wg, wu), [x, wg, wu]
+
+
+def test_differentiating_a_gradient_raises(dev, seq):
+    """A gradient taken with create_graph carries an error, by itself and beside the output in one loss; its values are the ordinary ones."""
+    for name, y, leaves in _graded_calls(dev, seq):
+        plain = torch.autograd.grad(y.sum(), leaves, retain_graph=True)
+        grads = torch.autograd.grad(y.sum(), leaves, create_graph=True)
+        for g, p in zip(grads, plain):
+            assert g.requires_grad and not p.requires_grad and torch.equal(g.detach(), p)
+            with pytest.raises(RuntimeError, match=f"{name} is differentiable once"):
+                (y.sum() + g.pow(2).sum()).backward(retain_graph=True)
+            with pytest.raises(RuntimeError, match=f"{name} is differentiable once"):
+                torch.autograd.grad(g.sum(), leaves, retain_graph=True, allow_unused=True)

@@ -97,6 +97,10 @@ bool graded(std::initializer_list<Tensor> ts) {
 void no_grad(const char *what, std::initializer_list<Tensor> ts) {
   TORCH_CHECK_VALUE(!graded(ts), what, " has no gradient: call it under torch.no_grad(), or the windowed form with T = 1");
 }
+// The operators have no forward-mode derivative: a tangent would be dropped without a word.
+void no_tangent(const char *what, std::initializer_list<Tensor> ts) {
+  for (const Tensor &t : ts) TORCH_CHECK_VALUE(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative: a tensor carries a tangent");
+}
 // A tensor that a kernel writes in place counts as changed: a backward pass that saved it refuses, as behind torch's own in-place operators.
 void written(const Tensor &t) {
   if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
@@ -236,6 +240,7 @@ void conv_check(const char *what, const Tensor &x, const Tensor &weight, const T
 std::pair<Tensor, Opt> causal_conv(const Tensor &x, const Tensor &weight, const Opt &bias_, const Opt &reset_, const Opt &state_, bool silu, bool want) {
   const char *what = "causal_conv";
   const Tensor bias = val(bias_), reset = val(reset_), state = val(state_);
+  no_tangent(what, {x, weight, bias, state});
   head(what, x, 3);
   conv_check(what, x, weight, bias, state);
   check_reset(what, x, reset);
@@ -249,6 +254,7 @@ std::pair<Tensor, Opt> causal_conv(const Tensor &x, const Tensor &weight, const 
 std::pair<Tensor, Tensor> causal_conv_step(const Tensor &x, const Opt &state_, const Tensor &weight, const Opt &bias_, const Opt &reset_, bool silu, const Opt &out_) {
   const char *what = "causal_conv_step";
   const Tensor bias = val(bias_), reset = val(reset_), state = val(state_), out = val(out_);
+  no_tangent(what, {x, state, weight, bias, out});
   head(what, x, 2);
   TORCH_CHECK_VALUE(state.defined(), what, ": a state is needed");
   conv_check(what, x, weight, bias, state);
@@ -378,6 +384,7 @@ ScanIn scan_check(const char *what, const Tensor &x, const Tensor &dt, const Ten
 std::pair<Tensor, Opt> selective_scan(const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Opt &skip, const Opt &z, const Opt &dt_bias,
                                       bool softplus, const Opt &reset, const Opt &state, bool want) {
   const char *what = "selective_scan";
+  no_tangent(what, {x, dt, A, B, C, val(skip), val(z), val(dt_bias), val(state)});
   head(what, x, 3);
   const ScanIn i = scan_check(what, x, dt, A, B, C, val(skip), val(z), val(dt_bias), val(state), val(reset), softplus);
   if (graded({i.x, i.dt, i.A, i.B, i.C, i.skip, i.z, i.dt_bias, i.state})) {
@@ -391,6 +398,7 @@ std::pair<Tensor, Tensor> selective_scan_step(const Tensor &x, const Tensor &dt,
                                               const Opt &z, const Opt &dt_bias, bool softplus, const Opt &reset, const Opt &out_) {
   const char *what = "selective_scan_step";
   const Tensor state = val(state_), out = val(out_);
+  no_tangent(what, {x, dt, A, B, C, state, val(skip), val(z), val(dt_bias), out});
   head(what, x, 2);
   TORCH_CHECK_VALUE(state.defined(), what, ": a state is needed");
   const ScanIn i = scan_check(what, x, dt, A, B, C, val(skip), val(z), val(dt_bias), state, val(reset), softplus);
@@ -465,6 +473,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
 Tensor gated_linear(const Tensor &x, const Tensor &wg, const Tensor &wu, const Opt &bg_, const Opt &bu_, int64_t act) {
   const char *what = "gated_linear";
   const Tensor bg = val(bg_), bu = val(bu_);
+  no_tangent(what, {x, wg, wu, bg, bu});
   TORCH_CHECK_VALUE(x.dim() >= 1, what, ": x must be [..., channels]");
   head(what, x, x.dim());
   TORCH_CHECK_VALUE(wg.dim() == 2 && wg.size(0) >= 1, what, ": w_gate must be [features, channels], got ", wg.sizes());

@@ -6,7 +6,7 @@
     y = seq.selective_scan(x, dt, A, B, C, skip=d, z=z, dt_bias=bias, reset=reset)
     h = seq.gated_linear(y, w_gate, w_up, b_gate, b_up)           # SiLU(y Wg^T + bg) * (y Wu^T + bu)
 
-Each is differentiable (once); ``causal_conv_step`` and ``selective_scan_step`` advance every acting row by one step.  Activations
+Each is differentiable (once, in reverse mode: a second derivative and a forward-mode tangent raise); ``causal_conv_step`` and ``selective_scan_step`` advance every acting row by one step.  Activations
 may be float32, bfloat16 or float16 and any strided view (a copy is made only where the last dimension is not dense); states of the scan,
 its A / skip / dt_bias and the convolution's weights are float32.  ``reset`` [T, rows] (bool or uint8) marks the steps at which a new sequence
 begins: several sequences can share a row, and left padding is dropped by a reset at the first real step.  Calls run on the current

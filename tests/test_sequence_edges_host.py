@@ -2,9 +2,10 @@
 import ctypes as C
 
 import pytest
-import torch  # noqa: F401
+import torch
 
 from fastdeepqlearning_amd import _native as nat
+from fastdeepqlearning_amd import sequence as seq
 from test_sequence_host import P, _gated
 
 ROUND = 0x100      # FDQL_GATED_ROUND_GRADS
@@ -21,3 +22,31 @@ def test_gated_gradient_parts_are_the_callers_choice():
     for act in (ROUND | 3, ROUND << 1, -1):
         assert lib.fdql_gated(C.byref(_gated(act=act, x=P, w_gate=P, w_up=P, y=P)), None) == nat.FDQL_EINVAL
         assert "activation" in lib.fdql_last_error().decode()
+
+
+def _calls(seq, lift=lambda t: t):
+    """name -> the five calls on small CPU tensors, every floating-point argument in turn passed through `lift`."""
+    z = lambda *s: torch.ones(*s)  # noqa: E731
+    forms = {
+        "causal_conv": ([z(2, 1, 4), z(4, 2), z(4)], lambda a: seq.causal_conv(*a)),
+        "causal_conv with a state": ([z(2, 1, 4), z(4, 2), z(1, 1, 4)], lambda a: seq.causal_conv(a[0], a[1], initial_state=a[2])),
+        "causal_conv_step": ([z(1, 4), z(1, 1, 4), z(4, 2), z(4), z(1, 1, 4)], lambda a: seq.causal_conv_step(*a[:4], out_state=a[4])),
+        "selective_scan": ([z(2, 1, 4), z(2, 1, 4), z(4, 2), z(2, 1, 2), z(2, 1, 2), z(4), z(2, 1, 4), z(4), z(1, 4, 2)],
+                           lambda a: seq.selective_scan(*a[:5], skip=a[5], z=a[6], dt_bias=a[7], initial_state=a[8])),
+        "selective_scan_step": ([z(1, 4), z(1, 4), z(4, 2), z(1, 2), z(1, 2), z(1, 4, 2), z(4), z(1, 4), z(4), z(1, 4, 2)],
+                                lambda a: seq.selective_scan_step(*a[:6], skip=a[6], z=a[7], dt_bias=a[8], out_state=a[9])),
+        "gated_linear": ([z(2, 4), z(3, 4), z(3, 4), z(3), z(3)], lambda a: seq.gated_linear(*a)),
+    }
+    for name, (args, call) in forms.items():
+        for k in range(len(args)):
+            yield f"{name}, argument {k}", lambda: call([lift(t) if j == k else t for j, t in enumerate(args)])  # noqa: B023
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor in any place raises; the result would have no tangent."""
+    import torch.autograd.forward_ad as fwad
+    with fwad.dual_level():
+        for name, call in _calls(seq, lambda t: fwad.make_dual(t, torch.ones_like(t))):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+                pytest.fail(name)

@@ -5,9 +5,11 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <unordered_set>
@@ -96,6 +98,15 @@ bool graded(std::initializer_list<Tensor> ts) {
 }
 void no_grad(const char *what, std::initializer_list<Tensor> ts) {
   TORCH_CHECK_VALUE(!graded(ts), what, " has no gradient: call it under torch.no_grad(), or the windowed form with T = 1");
+}
+// The calls go past torch's dispatcher: a trace would hold the allocation of their results and nothing that fills them.
+void not_traced(const char *what) {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  bool traced = torch::jit::tracer::isTracing();
+  for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+    traced = traced || TorchDispatchModeTLS::get_mode(mode).has_value();
+  TORCH_CHECK(!traced, what, " cannot be traced: its kernels would be missing from the trace (capture the call into a graph instead)");
 }
 // The operators have no forward-mode derivative: a tangent would be dropped without a word.
 void no_tangent(const char *what, std::initializer_list<Tensor> ts) {
@@ -207,6 +218,7 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
+    not_traced("causal_conv");
     capturable("causal_conv", s[0]);
     const Tensor &x = s[0], &weight = s[1], &bias = s[2], &state = s[3];
     c10::DeviceGuard guard(x.device());
@@ -240,6 +252,7 @@ void conv_check(const char *what, const Tensor &x, const Tensor &weight, const T
 std::pair<Tensor, Opt> causal_conv(const Tensor &x, const Tensor &weight, const Opt &bias_, const Opt &reset_, const Opt &state_, bool silu, bool want) {
   const char *what = "causal_conv";
   const Tensor bias = val(bias_), reset = val(reset_), state = val(state_);
+  not_traced(what);
   no_tangent(what, {x, weight, bias, state});
   head(what, x, 3);
   conv_check(what, x, weight, bias, state);
@@ -254,6 +267,7 @@ std::pair<Tensor, Opt> causal_conv(const Tensor &x, const Tensor &weight, const 
 std::pair<Tensor, Tensor> causal_conv_step(const Tensor &x, const Opt &state_, const Tensor &weight, const Opt &bias_, const Opt &reset_, bool silu, const Opt &out_) {
   const char *what = "causal_conv_step";
   const Tensor bias = val(bias_), reset = val(reset_), state = val(state_), out = val(out_);
+  not_traced(what);
   no_tangent(what, {x, state, weight, bias, out});
   head(what, x, 2);
   TORCH_CHECK_VALUE(state.defined(), what, ": a state is needed");
@@ -331,6 +345,7 @@ struct ScanNode : torch::autograd::Function<ScanNode> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
+    not_traced("selective_scan");
     capturable("selective_scan", s[0]);
     const ScanIn i = {s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9], ctx->saved_data["softplus"].toBool()};
     c10::DeviceGuard guard(i.x.device());
@@ -384,6 +399,7 @@ ScanIn scan_check(const char *what, const Tensor &x, const Tensor &dt, const Ten
 std::pair<Tensor, Opt> selective_scan(const Tensor &x, const Tensor &dt, const Tensor &A, const Tensor &B, const Tensor &C, const Opt &skip, const Opt &z, const Opt &dt_bias,
                                       bool softplus, const Opt &reset, const Opt &state, bool want) {
   const char *what = "selective_scan";
+  not_traced(what);
   no_tangent(what, {x, dt, A, B, C, val(skip), val(z), val(dt_bias), val(state)});
   head(what, x, 3);
   const ScanIn i = scan_check(what, x, dt, A, B, C, val(skip), val(z), val(dt_bias), val(state), val(reset), softplus);
@@ -398,6 +414,7 @@ std::pair<Tensor, Tensor> selective_scan_step(const Tensor &x, const Tensor &dt,
                                               const Opt &z, const Opt &dt_bias, bool softplus, const Opt &reset, const Opt &out_) {
   const char *what = "selective_scan_step";
   const Tensor state = val(state_), out = val(out_);
+  not_traced(what);
   no_tangent(what, {x, dt, A, B, C, state, val(skip), val(z), val(dt_bias), out});
   head(what, x, 2);
   TORCH_CHECK_VALUE(state.defined(), what, ": a state is needed");
@@ -447,6 +464,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
   }
   static variable_list backward(AutogradContext *ctx, variable_list g) {
     const variable_list s = ctx->get_saved_variables();
+    not_traced("gated_linear");
     capturable("gated_linear", s[0]);
     const Tensor &x = s[0];
     c10::DeviceGuard guard(x.device());
@@ -473,6 +491,7 @@ struct GatedNode : torch::autograd::Function<GatedNode> {
 Tensor gated_linear(const Tensor &x, const Tensor &wg, const Tensor &wu, const Opt &bg_, const Opt &bu_, int64_t act) {
   const char *what = "gated_linear";
   const Tensor bg = val(bg_), bu = val(bu_);
+  not_traced(what);
   no_tangent(what, {x, wg, wu, bg, bu});
   TORCH_CHECK_VALUE(x.dim() >= 1, what, ": x must be [..., channels]");
   head(what, x, x.dim());

@@ -11,7 +11,7 @@ may be float32, bfloat16 or float16 and any strided view (a copy is made only wh
 its A / skip / dt_bias and the convolution's weights are float32.  ``reset`` [T, rows] (bool or uint8) marks the steps at which a new sequence
 begins: several sequences can share a row, and left padding is dropped by a reset at the first real step.  Calls run on the current
 stream of the tensors' device, never synchronise, and can be captured into a graph (a captured backward pass raises while an eager graph of the same
-leaves is alive on the default stream).  Wrong types, shapes or devices raise ValueError, a failed
+leaves is alive on the default stream); tracers (torch.jit.trace, make_fx, fake tensors) cannot see them, and the calls raise there.  Wrong types, shapes or devices raise ValueError, a failed
 launch FdqlError.  All compute is in libfdql_hip.so; there is no CPU path."""
 import ctypes as C
 

@@ -50,3 +50,21 @@ def test_forward_mode_tangents_are_refused():
             with pytest.raises(ValueError, match="forward-mode"):
                 call()
                 pytest.fail(name)
+
+
+def test_tracing_is_refused():
+    """A trace would hold uninitialised results: jit and fx tracers and fake tensors raise."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    seen = set()
+    for name, call in _calls(seq):
+        if name.split(",")[0] in seen:
+            continue
+        seen.add(name.split(",")[0])
+        for trace in (lambda f: torch.jit.trace(f, torch.ones(1), check_trace=False), lambda f: make_fx(f)(torch.ones(1)),
+                      lambda f: make_fx(f, tracing_mode="fake")(torch.ones(1))):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                trace(lambda a: call())  # noqa: B023
+        with FakeTensorMode(), pytest.raises(RuntimeError, match="cannot be traced"):
+            call()
+    assert len(seen) == 6

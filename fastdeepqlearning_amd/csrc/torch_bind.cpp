@@ -45,7 +45,12 @@ void check(int64_t rc) {
   if (rc < 0) throw FdqlException(rc, api.last_error());
 }
 
-void *ptr(const Tensor &t) { return t.defined() ? const_cast<void *>(t.const_data_ptr()) : nullptr; }
+void *ptr(const Tensor &t) {
+  if (!t.defined()) return nullptr;
+  void *const p = const_cast<void *>(t.const_data_ptr());
+  TORCH_CHECK(p || t.numel() == 0, "sequence operators: a tensor of ", t.sizes(), " has no memory");
+  return p;
+}
 float *fptr(const Tensor &t) { return static_cast<float *>(ptr(t)); }
 uint8_t *bptr(const Tensor &t) { return static_cast<uint8_t *>(ptr(t)); }
 Tensor val(const Opt &t) { return t.has_value() ? *t : Tensor(); }
@@ -56,10 +61,20 @@ Tensor scratch(int64_t bytes, const Tensor &like) {
   return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
 }
 Tensor like(const Tensor &t) { return t.defined() ? at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous)) : Tensor(); }
+// The values as memory holds them: a view that torch negates on reading is written out, a gradient that is a symbolic zero becomes zeros.
+Tensor stored(const Tensor &t) { return t._is_zerotensor() ? at::zeros(t.sizes(), t.options()) : t.is_neg() ? t.resolve_neg() : t; }
 // the last dimension dense / everything dense / everything behind the first dimension dense
-Tensor dense(const Tensor &t) { return !t.defined() || t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous(); }
-Tensor whole(const Tensor &t) { return t.defined() ? t.contiguous() : t; }
-Tensor rows_dense(const Tensor &t) { return !t.defined() || t.size(0) == 0 || t.select(0, 0).is_contiguous() ? t : t.contiguous(); }
+Tensor dense(const Tensor &u) {
+  if (!u.defined()) return u;
+  const Tensor t = stored(u);
+  return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+}
+Tensor whole(const Tensor &t) { return t.defined() ? stored(t).contiguous() : t; }
+Tensor rows_dense(const Tensor &u) {
+  if (!u.defined()) return u;
+  const Tensor t = stored(u);
+  return t.size(0) == 0 || t.select(0, 0).is_contiguous() ? t : t.contiguous();
+}
 
 int32_t type_of(const Tensor &t) {
   switch (t.scalar_type()) {
@@ -108,9 +123,16 @@ void not_traced(const char *what) {
     traced = traced || TorchDispatchModeTLS::get_mode(mode).has_value();
   TORCH_CHECK(!traced, what, " cannot be traced: its kernels would be missing from the trace (capture the call into a graph instead)");
 }
-// The operators have no forward-mode derivative: a tangent would be dropped without a word.
-void no_tangent(const char *what, std::initializer_list<Tensor> ts) {
-  for (const Tensor &t : ts) TORCH_CHECK_VALUE(!t.defined() || !t._fw_grad(0).defined(), what, " has no forward-mode derivative: a tensor carries a tangent");
+// Tensors whose memory holds their values: a subclass that dispatches by itself or a functional transform's wrapper has none of its own, and the operators
+// have no forward-mode derivative, a tangent would be dropped without a word.
+void plain(const char *what, std::initializer_list<Tensor> ts) {
+  constexpr c10::DispatchKeySet foreign({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Batched,
+                                         c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::ZeroTensor});
+  for (const Tensor &t : ts) {
+    if (!t.defined()) continue;
+    TORCH_CHECK_VALUE(!t.key_set().has_any(foreign), what, ": plain tensors only, one is a wrapper without memory of its own");
+    TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), what, " has no forward-mode derivative: a tensor carries a tangent");
+  }
 }
 // A tensor that a kernel writes in place counts as changed: a backward pass that saved it refuses, as behind torch's own in-place operators.
 void written(const Tensor &t) {
@@ -253,7 +275,7 @@ std::pair<Tensor, Opt> causal_conv(const Tensor &x, const Tensor &weight, const 
   const char *what = "causal_conv";
   const Tensor bias = val(bias_), reset = val(reset_), state = val(state_);
   not_traced(what);
-  no_tangent(what, {x, weight, bias, state});
+  plain(what, {x, weight, bias, state, reset});
   head(what, x, 3);
   conv_check(what, x, weight, bias, state);
   check_reset(what, x, reset);
@@ -268,14 +290,14 @@ std::pair<Tensor, Tensor> causal_conv_step(const Tensor &x, const Opt &state_, c
   const char *what = "causal_conv_step";
   const Tensor bias = val(bias_), reset = val(reset_), state = val(state_), out = val(out_);
   not_traced(what);
-  no_tangent(what, {x, state, weight, bias, out});
+  plain(what, {x, state, weight, bias, out, reset});
   head(what, x, 2);
   TORCH_CHECK_VALUE(state.defined(), what, ": a state is needed");
   conv_check(what, x, weight, bias, state);
   check_reset(what, x, reset);
   no_grad(what, {x, state, weight, bias, out});
   same(what, "out_state", x, out, state.sizes(), x.scalar_type());
-  TORCH_CHECK_VALUE(!out.defined() || out.size(0) == 0 || out.select(0, 0).is_contiguous(), what, ": rows of out_state must be dense");
+  TORCH_CHECK_VALUE(!out.defined() || (!out.is_neg() && (out.size(0) == 0 || out.select(0, 0).is_contiguous())), what, ": rows of out_state must be dense");
   auto r = conv_run(dense(x), whole(weight), whole(bias), rows_dense(state), reset, silu, true, out);
   written(out);
   return r;
@@ -400,7 +422,7 @@ std::pair<Tensor, Opt> selective_scan(const Tensor &x, const Tensor &dt, const T
                                       bool softplus, const Opt &reset, const Opt &state, bool want) {
   const char *what = "selective_scan";
   not_traced(what);
-  no_tangent(what, {x, dt, A, B, C, val(skip), val(z), val(dt_bias), val(state)});
+  plain(what, {x, dt, A, B, C, val(skip), val(z), val(dt_bias), val(state), val(reset)});
   head(what, x, 3);
   const ScanIn i = scan_check(what, x, dt, A, B, C, val(skip), val(z), val(dt_bias), val(state), val(reset), softplus);
   if (graded({i.x, i.dt, i.A, i.B, i.C, i.skip, i.z, i.dt_bias, i.state})) {
@@ -415,13 +437,13 @@ std::pair<Tensor, Tensor> selective_scan_step(const Tensor &x, const Tensor &dt,
   const char *what = "selective_scan_step";
   const Tensor state = val(state_), out = val(out_);
   not_traced(what);
-  no_tangent(what, {x, dt, A, B, C, state, val(skip), val(z), val(dt_bias), out});
+  plain(what, {x, dt, A, B, C, state, val(skip), val(z), val(dt_bias), out, val(reset)});
   head(what, x, 2);
   TORCH_CHECK_VALUE(state.defined(), what, ": a state is needed");
   const ScanIn i = scan_check(what, x, dt, A, B, C, val(skip), val(z), val(dt_bias), state, val(reset), softplus);
   no_grad(what, {x, dt, A, B, C, i.skip, i.z, i.dt_bias, state, out});
   same(what, "out_state", x, out, state.sizes(), at::kFloat);
-  TORCH_CHECK_VALUE(!out.defined() || out.size(0) == 0 || out.select(0, 0).is_contiguous(), what, ": rows of out_state must be dense");
+  TORCH_CHECK_VALUE(!out.defined() || (!out.is_neg() && (out.size(0) == 0 || out.select(0, 0).is_contiguous())), what, ": rows of out_state must be dense");
   auto r = scan_run(i, true, false, out);
   written(out);
   return {std::get<0>(r), std::get<1>(r)};
@@ -492,7 +514,7 @@ Tensor gated_linear(const Tensor &x, const Tensor &wg, const Tensor &wu, const O
   const char *what = "gated_linear";
   const Tensor bg = val(bg_), bu = val(bu_);
   not_traced(what);
-  no_tangent(what, {x, wg, wu, bg, bu});
+  plain(what, {x, wg, wu, bg, bu});
   TORCH_CHECK_VALUE(x.dim() >= 1, what, ": x must be [..., channels]");
   head(what, x, x.dim());
   TORCH_CHECK_VALUE(wg.dim() == 2 && wg.size(0) >= 1, what, ": w_gate must be [features, channels], got ", wg.sizes());

@@ -57,3 +57,28 @@ def test_differentiating_a_gradient_raises(dev, seq):
                 (y.sum() + g.pow(2).sum()).backward(retain_graph=True)
             with pytest.raises(RuntimeError, match=f"{name} is differentiable once"):
                 torch.autograd.grad(g.sum(), leaves, retain_graph=True, allow_unused=True)
+
+
+def test_views_that_torch_negates_on_reading(dev, seq):
+    """The imaginary part of a conjugate view is stored with the other sign: inputs, gradients and states of that kind count with their values."""
+    neg = lambda t: torch.complex(torch.zeros_like(t), -t).conj().imag  # noqa: E731
+    g = _gen(12)
+    r = lambda *s: torch.randn(*s, generator=g).to(dev)  # noqa: E731
+    x, w, b, st, dt, A, B, h, wg, wu = r(5, 2, 8), r(8, 4), r(8), r(2, 3, 8), r(5, 2, 8), -r(8, 4).abs(), r(5, 2, 4), r(2, 8, 4), r(6, 8), r(6, 8)
+    assert neg(x).is_neg() and torch.equal(neg(x), x)
+    calls = [([x, w, b, st], lambda a: seq.causal_conv(a[0], a[1], a[2], initial_state=a[3])), ([x, dt, A, B, h], lambda a: seq.selective_scan(a[0], a[1], a[2], a[3], a[3], initial_state=a[4])),
+             ([x, wg, wu], lambda a: seq.gated_linear(*a))]
+    for args, call in calls:
+        want = call(args)
+        assert torch.equal(call([neg(t) for t in args]), want)
+        leaves, dy = [t.clone().requires_grad_() for t in args], torch.randn(want.shape, generator=g).to(dev)
+        plain = torch.autograd.grad(call(leaves), leaves, dy)
+        for a, c in zip(plain, torch.autograd.grad(call([neg(t) for t in leaves]), leaves, neg(dy))):
+            assert torch.equal(a, c)
+    y, s = seq.causal_conv_step(x[0], st, w, b)
+    y2, s2 = seq.causal_conv_step(neg(x[0]), neg(st), w, b)
+    assert torch.equal(y, y2) and torch.equal(s, s2)
+    with pytest.raises(ValueError, match="out_state"):
+        seq.causal_conv_step(x[0], st, w, b, out_state=neg(st))
+    with pytest.raises(ValueError, match="out_state"):
+        seq.selective_scan_step(x[0], dt[0], A, B[0], B[0], h, out_state=neg(h))

@@ -68,3 +68,32 @@ def test_tracing_is_refused():
         with FakeTensorMode(), pytest.raises(RuntimeError, match="cannot be traced"):
             call()
     assert len(seen) == 6
+
+
+class _Wrapped(torch.Tensor):
+    """A tensor without memory of its own, as distributed and quantised tensors are."""
+
+    @staticmethod
+    def __new__(cls, inner):
+        return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(f"{func} was called")
+
+
+def test_wrapper_tensors_are_refused():
+    """In any place: their data pointer is null.  A plain subclass, which has memory, gets as far as every other tensor."""
+    for name, call in _calls(seq, _Wrapped):
+        with pytest.raises(ValueError, match="plain tensors"):
+            call()
+            pytest.fail(name)
+    with pytest.raises(ValueError, match="GPU"):
+        seq.gated_linear(torch.nn.Parameter(torch.ones(2, 4)), torch.ones(3, 4), torch.ones(3, 4))
+
+
+def test_functional_transforms_are_refused():
+    w = torch.ones(3, 4)
+    for transform in (torch.vmap, torch.func.grad):
+        with pytest.raises(ValueError, match="plain tensors"):
+            transform(lambda a: seq.gated_linear(a, w, w).sum())(torch.ones(2, 2, 4))

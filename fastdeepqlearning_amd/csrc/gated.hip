@@ -74,21 +74,38 @@ template <> struct Mma<float> {
   }
 };
 
+// GELU's two pieces: e^(-g^2 / 2), the square's rounding undone, and the normal distribution P(g) = erfc(-g / sqrt 2) / 2.  The argument's rounding
+// is off by up to g^2 steps of a small P: a float result adds its first order, -rest erfc'(x) / 2 = rest e^(-x^2) / sqrt pi (a 16-bit one does not see it:
+// P is below float's range from g = -13 on, 2^-16 before).
+__device__ __forceinline__ float gauss(float g) {
+  const float sq = g * g, rest = fmaf(g, g, -sq);
+  return exp_acc(-0.5f * sq) * (sq < 1e4f ? fmaf(-0.5f, rest, 1.f) : 1.f);
+}
+template <typename T>
+__device__ __forceinline__ float normal_cdf(float g, float gauss_g) {
+  constexpr float C = 0.70710678118654752f, C_REST = (float)(0.70710678118654752440 - (double)C);
+  const float x = -C * g;
+  float p = 0.5f * erfcf(x);
+  if (sizeof(T) == 4 && fabsf(g) < 100.f) p = fmaf(fmaf(C, g, x) + C_REST * g, 0.56418958354775628f * gauss_g, p);
+  return p;
+}
 // f(g) and f'(g)
+template <typename T>
 __device__ __forceinline__ float act_f(int act, float g) {
-  if (act == FDQL_ACT_GELU) return 0.5f * g * erfcf(-0.70710678118654752f * g);
-  const float s = sigmoid_f(g);
+  if (act == FDQL_ACT_GELU) return g * normal_cdf<T>(g, sizeof(T) == 4 ? gauss(g) : 0.f);
+  const float s = sigmoid_f<T>(g).s;
   return act == FDQL_ACT_SILU ? g * s : s;
 }
+template <typename T>
 __device__ __forceinline__ void act_df(int act, float g, float &f, float &df) {
   if (act == FDQL_ACT_GELU) {
-    const float cdf = 0.5f * erfcf(-0.70710678118654752f * g);
+    const float e = gauss(g), cdf = normal_cdf<T>(g, e);
     f = g * cdf;
-    df = fmaf(g * 0.39894228040143268f, exp_acc(-0.5f * g * g), cdf);
+    df = fmaf(g * 0.39894228040143268f, e, cdf);
   } else {
-    const float s = sigmoid_f(g), r = s * (1.f - s);
-    f = act == FDQL_ACT_SILU ? g * s : s;
-    df = act == FDQL_ACT_SILU ? fmaf(g, r, s) : r;
+    const Sigmoid v = sigmoid_f<T>(g);
+    f = act == FDQL_ACT_SILU ? g * v.s : v.s;
+    df = act == FDQL_ACT_SILU ? fmaf(g * v.s, v.c, v.s) : v.s * v.c;
   }
 }
 
@@ -196,7 +213,7 @@ __device__ __forceinline__ void store_part(const Args &a, const v16f (&acc)[MT][
         if (WHOLE || (col && row < left)) {
           if constexpr (MODE == FWD) {
             const float g = acc[i][0][r] + bg, u = acc[i][1][r] + bu;
-            (out + o)[at] = from_f<T>(act_f(p.act, g) * u);
+            (out + o)[at] = from_f<T>(act_f<T>(p.act, g) * u);
             if (p.pre) {
               (p.pre + o)[at] = g;
               (p.pre + p.M * ld + o)[at] = u;
@@ -626,7 +643,7 @@ __global__ __launch_bounds__(NW * 64) void k_gated_rows(Args a) {
       if (o < F) {
         const float g = acc[m][0][r] + bg[r];
         const float u = acc[m][1][r] + bu[r];
-        reinterpret_cast<T *>(p.y)[row * F + o] = from_f<T>(act_f(p.act, g) * u);
+        reinterpret_cast<T *>(p.y)[row * F + o] = from_f<T>(act_f<T>(p.act, g) * u);
         if (p.pre) {
           p.pre[row * F + o] = g;
           p.pre[(p.M + row) * F + o] = u;
@@ -660,7 +677,7 @@ __global__ __launch_bounds__(256) void k_gated_grad(Args a) {
         const float g = p.pre[m * F + f], u = p.pre[MF + m * F + f];
         const float dy = to_f(reinterpret_cast<const T *>(p.dy)[m * p.dy_sr + f]);
         float v, dv;
-        act_df(p.act, g, v, dv);
+        act_df<T>(p.act, g, v, dv);
         dg = dy * u * dv;
         du = dy * v;
       }

@@ -265,7 +265,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
       for (int q = 0; q < OWN; ++q) {
         const int i = q * S + s;
         float y = fmaf(skip, x[q], own[q]);
-        if (p.z) y *= z[q] * sigmoid_f(z[q]);
+        if (p.z) y *= z[q] * sigmoid_f<T>(z[q]).s;
         if (live && i < nt) yp[(int64_t)(t + q * S) * y_st] = from_f<T>(y);
       }
     }
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
       v[q] = to_f(yn[q]);
       if (p.z) {
         const float z = to_f(zn[q]);
-        v[q] *= z * sigmoid_f(z);
+        v[q] *= z * sigmoid_f<T>(z).s;
       }
       del[q] = to_f(dn[q]) + bias;
       if (p.dt_softplus) del[q] = softplus_f(del[q]);
@@ -514,9 +514,10 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
       x[q] = live ? to_f(xn[q]) : 0.f;
       dy[q] = live ? to_f(yn[q]) : 0.f;
       if (p.z) {
-        const float z = to_f(zn[q]), sg = sigmoid_f(z);
-        zf[q] = dy[q] * sg * fmaf(z, 1.f - sg, 1.f);
-        dy[q] *= z * sg;
+        const float z = to_f(zn[q]);
+        const Sigmoid g = sigmoid_f<T>(z);
+        zf[q] = dy[q] * g.s * fmaf(z, g.c, 1.f);
+        dy[q] *= z * g.s;
       }
       del[q] = to_f(dn[q]) + bias;
       slope[q] = 1.f;
@@ -743,7 +744,7 @@ __global__ __launch_bounds__(256) void k_scan_step(fdql_scan_t p, int Dg, int tp
   y = fmaf(p.skip ? p.skip[d] : 0.f, x, y);
   if (p.z) {
     const float z = to_f(reinterpret_cast<const T *>(p.z)[(int64_t)r * p.z_sr + d]);
-    y *= z * sigmoid_f(z);
+    y *= z * sigmoid_f<T>(z).s;
   }
   if (dc < Dg) reinterpret_cast<T *>(p.y)[(int64_t)r * p.D + d] = from_f<T>(y);
 }
@@ -782,7 +783,7 @@ __global__ __launch_bounds__(256) void k_scan_step_few(fdql_scan_t p, int Dg, in
   }
   for (int m = 1; m < lpc; m <<= 1) acc += __shfl_xor(acc, m);
   float y = fmaf(skip, x, acc);
-  if (p.z) y *= z * sigmoid_f(z);
+  if (p.z) y *= z * sigmoid_f<T>(z).s;
   if (sub == 0 && live) reinterpret_cast<T *>(p.y)[(int64_t)r * p.D + d] = from_f<T>(y);
 }
 

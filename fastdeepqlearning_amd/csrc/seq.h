@@ -38,8 +38,16 @@ __device__ __forceinline__ float exp_acc(float v) {
   const float e = __builtin_amdgcn_exp2f(hi);
   return fabsf(hi) < 126.f ? fmaf(e, lo * LN2, e) : e;   // (infinite or vanishing: nothing to correct)
 }
-// 1 / (1 + e^-v); the power's error, |v| float steps of it, is at most 0.3 steps of the sum
-__device__ __forceinline__ float sigmoid_f(float v) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E * v)); }
+// s = 1 / (1 + e^-v) and c = 1 - s = 1 / (1 + e^v), each from the power w = e^-|v| that keeps its own digits where it is small (s of a negative v is
+// w / (1 + w): as 1 / (1 + e^|v|) it would carry the power's error whole, c as 1 - s would have none of its digits left from v = 17 on).
+// One product for the exponent is off by up to |v| float steps, 2^-17.5 of the result at most: enough for a result of 16 bits (half a step is 2^-12
+// or 2^-9), not for a float one.
+struct Sigmoid { float s, c; };
+template <typename T>
+__device__ __forceinline__ Sigmoid sigmoid_f(float v) {
+  const float w = sizeof(T) == 4 ? exp_acc(-fabsf(v)) : __builtin_amdgcn_exp2f(-LOG2E * fabsf(v)), r = __builtin_amdgcn_rcpf(1.f + w), q = w * r;
+  return v >= 0.f ? Sigmoid{r, q} : Sigmoid{q, r};
+}
 // log(1 + e^v) = max(v, 0) + log1p(w), w = e^-|v| in (0, 1]: log1p(w) = 2 atanh(w / (2 + w)), the odd series to the eighth term
 // (argument at most 1/3: the first term left out is below 2e-9 of the sum).  Keeps its relative precision for small steps.
 __device__ __forceinline__ float softplus_w(float v, float w) {

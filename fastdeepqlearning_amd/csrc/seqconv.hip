@@ -149,7 +149,7 @@ __global__ __launch_bounds__(WPB * 64) void k_seqconv_fwd(Args a) {
           float pre = b[v];
 #pragma unroll
           for (int k = 0; k < K; ++k) pre = fmaf(w[k][v], win[k][v], pre);
-          y[v] = p.silu ? pre * sigmoid_f(pre) : pre;
+          y[v] = p.silu ? pre * sigmoid_f<T>(pre).s : pre;
         }
         store_v<T, V>(reinterpret_cast<T *>(p.y) + ((int64_t)(t + i) * p.R + r) * p.D + d, y);
       }
@@ -233,8 +233,8 @@ __global__ __launch_bounds__(WPB * 64) void k_seqconv_bwd(Args a) {
         for (int k = 0; k < K; ++k) pre = fmaf(w[k][v], win[k][v], pre);
         dp[v] = dy[v];
         if (p.silu) {
-          const float sg = sigmoid_f(pre);
-          dp[v] *= sg * fmaf(pre, 1.f - sg, 1.f);
+          const Sigmoid g = sigmoid_f<T>(pre);
+          dp[v] *= g.s * fmaf(pre, g.c, 1.f);
         }
         if (t >= p.T) dp[v] = 0.f;                   // past the end only the pending gradients leave
         if (t < t1) {

@@ -82,3 +82,62 @@ def test_views_that_torch_negates_on_reading(dev, seq):
         seq.causal_conv_step(x[0], st, w, b, out_state=neg(st))
     with pytest.raises(ValueError, match="out_state"):
         seq.selective_scan_step(x[0], dt[0], A, B[0], B[0], h, out_state=neg(h))
+
+
+def _relative(name, got, want, steps):
+    """Every value within `steps` roundings of float, 2^-24 each, of its own size."""
+    off = (got.detach().cpu().double() - want).abs() / want.abs()
+    assert off.max() <= steps * U32, f"{name}: {float(off.max() / U32):.1f} roundings at {int(off.argmax())}"
+
+
+def _sig(v):
+    """1 / (1 + e^-v) and 1 / (1 + e^v) in 64 bits, both with all their digits"""
+    return torch.where(v >= 0, 1 / (1 + torch.exp(-v)), torch.exp(v) / (1 + torch.exp(v))), torch.where(v >= 0, torch.exp(-v) / (1 + torch.exp(-v)), 1 / (1 + torch.exp(v)))
+
+
+# float activations far from zero, relative to their own size.  e^-|v| to one step (2 roundings of 2^-24) and its correction's 2, 1 + w 1, the reciprocal 2, the
+# product with w 1, two or three more products: 11; the slope's 1 + v c another 2 and the cancellation left at v <= -10 (1 + v c is at least 9 |c| of terms 11 |c|) 1.3 of
+# those.  16 holds them.  GELU adds the complementary error function's own error, up to 4 steps = 8 roundings: 24.
+@pytest.mark.parametrize("T", [1, 40])
+def test_small_conv_outputs_keep_their_digits(dev, seq, T):
+    v = -torch.logspace(1, 1.92, T * 3 * 64).view(T, 3, 64)
+    x = v.to(dev).requires_grad_()
+    w = torch.tensor([[0.0, 1.0]]).expand(64, 2).to(dev)
+    y = seq.causal_conv(x, w)
+    s, c = _sig(v.double())
+    _relative("y", y, v.double() * s, 16)
+    _relative("dx", torch.autograd.grad(y, x, torch.ones_like(y))[0], s * (1 + v.double() * c), 16)
+    _relative("step", seq.causal_conv_step(x[0].detach(), torch.zeros(3, 1, 64, device=dev), w)[0], (v.double() * s)[0], 16)
+
+
+@pytest.mark.parametrize("T", [1, 40, 200])
+def test_small_scan_gates_keep_their_digits(dev, seq, T):
+    v = -torch.logspace(1, 1.92, T * 64).view(T, 1, 64)
+    z, one = v.to(dev).requires_grad_(), torch.ones(T, 1, 64, device=dev)
+    A, B, skip = -torch.ones(64, 4, device=dev), torch.zeros(T, 1, 4, device=dev), torch.ones(64, device=dev)
+    y = seq.selective_scan(one, one, A, B, B, skip=skip, z=z)
+    s, c = _sig(v.double())
+    _relative("y", y, v.double() * s, 16)
+    dz, dx = torch.autograd.grad(seq.selective_scan(one.requires_grad_(), one, A, B, B, skip=skip, z=z), [z, one], torch.ones_like(y))
+    _relative("dz", dz, s * (1 + v.double() * c), 16)
+    _relative("dx", dx, v.double() * s, 16)
+    state = torch.zeros(1, 64, 4, device=dev)
+    _relative("step", seq.selective_scan_step(one[0].detach(), one[0].detach(), A, B[0], B[0], state, skip=skip, z=v[0].to(dev))[0], (v.double() * s)[0], 16)
+
+
+@pytest.mark.parametrize("M", [5, 32, 33, 4000])
+@pytest.mark.parametrize("kind", ["silu", "sigmoid", "gelu"])
+def test_small_gated_outputs_keep_their_digits(dev, seq, M, kind):
+    """One channel is the gate's value, another the constant 1 that the up side reads; sigmoid's slope on both sides."""
+    v = -torch.logspace(0.3 if kind == "gelu" else 1, 1.08 if kind == "gelu" else 1.92, M)
+    if kind == "sigmoid":
+        v[::2] *= -1
+    x = torch.stack([v, torch.ones(M), torch.zeros(M), torch.zeros(M)], 1).to(dev).requires_grad_()
+    wg, wu = torch.tensor([[1.0, 0, 0, 0]]).to(dev), torch.tensor([[0.0, 1, 0, 0]]).to(dev)
+    y = seq.gated_linear(x, wg, wu, activation=kind)
+    g = v.double()
+    s, c = _sig(g)
+    cdf, pdf = 0.5 * torch.erfc(-g / 2 ** 0.5), torch.exp(-g * g / 2) / (2 * torch.pi) ** 0.5
+    f, df = {"silu": (g * s, s * (1 + g * c)), "sigmoid": (s, s * c), "gelu": (g * cdf, cdf + g * pdf)}[kind]
+    _relative("y", y[:, 0], f, 24 if kind == "gelu" else 16)
+    _relative("dx", torch.autograd.grad(y, x, torch.ones_like(y))[0][:, 0], df, 24 if kind == "gelu" else 16)

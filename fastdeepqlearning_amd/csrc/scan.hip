@@ -12,6 +12,9 @@
 // some 150 per tile for the rest; backward 18).  Measured: float 50 x 256 x 512, N 16: forward 47 us (213 MB with the checkpoints would take 41),
 // backward 130; bf16 prompt 16383 x 1 x 1024: carries 65, join 14, outputs 89 us.
 //
+// Lanes without a channel and states behind the last one compute on zeros.  Zero times a step that is infinite or NaN would not stay zero: a
+// tile that holds one (looked at only where there are such states) takes the form that selects, as a tile with a reset does.
+//
 // Few rows and a long time axis leave most of the card idle, so the axis is cut into segments: k_scan_fwd<CARRY> gets each segment's
 // final state from a zero start and the sum of its steps (the product of the decays is e^(A sum delta)), k_scan_combine joins
 // them in order, and the main kernel runs every segment from its true start.  Backward does the same from the right.
@@ -72,6 +75,15 @@ __device__ __forceinline__ void pass_edge() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
+
+// How many of the N states lie at or behind a lane's first one, worked out where it is asked for (held through the loop it takes a mask for every state).
+__device__ __forceinline__ int states_left(int N, int first) {
+  int left = N - first;
+  asm volatile("" : "+v"(left));
+  return left;
+}
+
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < INFINITY; }
 
 // The value is computed by here (an accumulation put off to the end would keep every one of its terms in a register).
 __device__ __forceinline__ void settle(float &v) { asm volatile("" : "+v"(v)); }
@@ -178,7 +190,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
     A[j] = n < p.N ? p.A[(int64_t)d * p.N + n] * LOG2E : 0.f;
     if (CARRY) h[j] = 0.f;
     else if (a.nseg > 1) h[j] = a.seg_h[lane_slot<NL>(a, w.seg, w) + j * 64 + lane];
-    else h[j] = p.state_in && n < p.N ? p.state_in[(int64_t)w.r * p.state_in_sr + (int64_t)d * p.N + n] : 0.f;
+    else h[j] = p.state_in && live && n < p.N ? p.state_in[(int64_t)w.r * p.state_in_sr + (int64_t)d * p.N + n] : 0.f;
   }
   const int64_t y_st = (int64_t)p.R * p.D;
   T *yp = reinterpret_cast<T *>(p.y) + (int64_t)w.r * p.D + s * y_st + d;
@@ -211,7 +223,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
     float x[OWN], del[OWN], z[OWN];
 #pragma unroll
     for (int q = 0; q < OWN; ++q) {
-      x[q] = to_f(xn[q]);
+      x[q] = live ? to_f(xn[q]) : 0.f;
       del[q] = to_f(dn[q]) + bias;
       if (!CARRY) z[q] = to_f(zn[q]);
     }
@@ -221,14 +233,18 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
 #pragma unroll
       for (int j = 0; j < NL; ++j) ck[j * 64] = h[j];
     }
+    bool plain = true;
 #pragma unroll
     for (int q = 0; q < OWN; ++q) {
       if (p.dt_softplus) del[q] = softplus_f(del[q]);
+      if (!live) del[q] = 0.f;
       lds_d[wave][q * S + s][c] = make_float2(del[q], del[q] * x[q]);
+      plain = plain && finite(del[q]) && finite(del[q] * x[q]);
     }
+    const bool wild = p.N < NP && __any(!plain);
     wave_lds_fence();
     float acc[TS];
-    const auto tile = [&](auto whole) {              // whole: eight steps without a reset
+    const auto tile = [&](auto whole) {              // whole: eight finite steps without a reset
 #pragma unroll
       for (int i = 0; i < TS; ++i) {
         if (i % 2 == 0) pass_edge();
@@ -236,6 +252,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
         if (decltype(whole)::value || i < nt) {
           const float2 v = lds_d[wave][i][c];
           const float dl = v.x, dx = v.y;
+          const int left = decltype(whole)::value ? NL : states_left(p.N, s * NL);
           if (CARRY) sum += dl;
           if (!decltype(whole)::value && (rst >> i & 1)) {
 #pragma unroll
@@ -249,6 +266,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
 #pragma unroll
             for (int j = 0; j < VW; ++j) {
               h[j4 + j] = fmaf(__builtin_amdgcn_exp2f(dl * A[j4 + j]), h[j4 + j], dx * B[j]);
+              if (!decltype(whole)::value && j4 + j >= left) h[j4 + j] = 0.f;
               if (!CARRY) acc[i] = fmaf(h[j4 + j], C[j], acc[i]);
             }
           }
@@ -256,7 +274,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
         }
       }
     };
-    if (rst == 0 && nt == TS) tile(std::true_type());
+    if (rst == 0 && nt == TS && !wild) tile(std::true_type());
     else tile(std::false_type());
     if (!CARRY) {
       float own[OWN];
@@ -264,7 +282,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
 #pragma unroll
       for (int q = 0; q < OWN; ++q) {
         const int i = q * S + s;
-        float y = fmaf(skip, x[q], own[q]);
+        float y = p.skip ? fmaf(skip, x[q], own[q]) : own[q];
         if (p.z) y *= z[q] * sigmoid_f<T>(z[q]).s;
         if (live && i < nt) yp[(int64_t)(t + q * S) * y_st] = from_f<T>(y);
       }
@@ -336,6 +354,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
     any |= rst != 0;
     Cn.put(lC, lane);
     float v[OWN], del[OWN];
+    bool plain = true;
 #pragma unroll
     for (int q = 0; q < OWN; ++q) {
       v[q] = to_f(yn[q]);
@@ -346,7 +365,9 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
       del[q] = to_f(dn[q]) + bias;
       if (p.dt_softplus) del[q] = softplus_f(del[q]);
       lds_d[wave][q * S + s][c] = make_float2(del[q], v[q]);
+      plain = plain && finite(del[q]) && finite(v[q]);
     }
+    const bool wild = p.N < NP && __any(!plain);
     if (t > t0) fetch(t - TS);
     wave_lds_fence();
     const auto tile = [&](auto whole) {
@@ -355,6 +376,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
         if (decltype(whole)::value || i < nt) {
           const float2 q = lds_d[wave][i][c];
           const float dl = q.x, dy = q.y;
+          const int left = decltype(whole)::value ? NL : states_left(p.N, s * NL);
           sum += dl;
           const bool cut = !decltype(whole)::value && (rst >> i & 1);
 #pragma unroll
@@ -363,13 +385,13 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
 #pragma unroll
             for (int j = 0; j < VW; ++j) {
               const float g = __builtin_amdgcn_exp2f(dl * A[j4 + j]) * fmaf(dy, C[j], h[j4 + j]);
-              h[j4 + j] = cut ? 0.f : g;
+              h[j4 + j] = cut || (!decltype(whole)::value && j4 + j >= left) ? 0.f : g;
             }
           }
         }
       }
     };
-    if (rst == 0 && nt == TS) tile(std::true_type());
+    if (rst == 0 && nt == TS && !wild) tile(std::true_type());
     else tile(std::false_type());
     wave_lds_fence();
   }
@@ -380,6 +402,8 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
   if (lane == 0 && w.tile == 0 && w.g == 0) a.seg_f[(int64_t)w.seg * p.R + w.r] = any;
 }
 
+// A zero and an infinite state pass a segment as they are, whatever the product of its decays is, as they pass its steps one by one; others are
+// multiplied by its root twice, since the product may leave float's range where what it makes of a state does not.
 // seg_h becomes the state every segment starts from (REV = 0) / the carry that enters every segment from the right (REV = 1).
 template <int NL, int REV>
 __global__ __launch_bounds__(64) void k_scan_combine(Args a) {
@@ -420,7 +444,7 @@ __global__ __launch_bounds__(64) void k_scan_combine(Args a) {
 #pragma unroll
     for (int q = 0; q < AHEAD; ++q) {
       to[q] = own[q];
-      e[q] = __builtin_amdgcn_exp2f(sum[q] * A);
+      e[q] = __builtin_amdgcn_exp2f(0.5f * sum[q] * A);
       cut[q] = any[q] != 0;
     }
     if (k0 + AHEAD < a.nseg - 1) fetch(k0 + AHEAD);
@@ -428,7 +452,8 @@ __global__ __launch_bounds__(64) void k_scan_combine(Args a) {
     for (int q = 0; q < AHEAD; ++q) {
       if (k0 + q < a.nseg - 1) {
         a.seg_h[seg_of(k0 + q) * per + i] = cur;
-        cur = cut[q] ? to[q] : fmaf(e[q], cur, to[q]);
+        const float in = cur == 0.f || !finite(cur) ? cur : cur * e[q] * e[q];
+        cur = cut[q] ? to[q] : in + to[q];
       }
     }
   }
@@ -507,12 +532,13 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
   for (int t = last; t >= t0; t -= TS, buf ^= 1) {
     const int nt = min(TS, t1 - t);
     const unsigned rst = (unsigned)__ballot(lane < nt && rn != 0);
-    // steps of this lane (S = 1: all eight): delta, delta x, gated dy; slope of the softplus, what dz is of the ungated output
+    // this lane's own steps: delta, delta x, gated dy; slope of the softplus, what dz is of the ungated output
     float x[OWN], del[OWN], dx[OWN], dy[OWN], slope[OWN], zf[OWN];
+    bool plain = true;
 #pragma unroll
     for (int q = 0; q < OWN; ++q) {
       x[q] = live ? to_f(xn[q]) : 0.f;
-      dy[q] = live ? to_f(yn[q]) : 0.f;
+      dy[q] = to_f(yn[q]);
       if (p.z) {
         const float z = to_f(zn[q]);
         const Sigmoid g = sigmoid_f<T>(z);
@@ -522,9 +548,12 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
       del[q] = to_f(dn[q]) + bias;
       slope[q] = 1.f;
       if (p.dt_softplus) del[q] = softplus_f(del[q], slope[q]);
+      if (!live) del[q] = dy[q] = 0.f;             // (dy: behind its gate)
       dx[q] = del[q] * x[q];
       lds_d[wave][q * S + s][c] = v4f{del[q], dx[q], dy[q], 0.f};
+      plain = plain && finite(del[q]) && finite(dx[q]) && finite(dy[q]);
     }
+    const bool wild = p.N < NP && __any(!plain);
     wave_lds_fence();
     if (t > t0) fetch(t - TS);
     const float *ck = p.checkpoints + lane_slot<NL>(a, t / TS, w) + lane;
@@ -534,7 +563,7 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
 #pragma unroll
     for (int i = 0; i < TS; ++i) yc[i] = dd[i] = gx[i] = 0.f;
     const auto tile = [&](auto whole) {
-      constexpr bool W = decltype(whole)::value;   // eight steps without a reset
+      constexpr bool W = decltype(whole)::value;   // eight finite steps without a reset
       float h0 = ck[0], h1 = ck[64];
 #pragma unroll
       for (int m = 0; m < NL; m += 2) {
@@ -549,11 +578,13 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
             const float dl = st[0], dxi = st[1];
             const float2 B = *reinterpret_cast<const float2 *>(tB + i * NP + m), C = *reinterpret_cast<const float2 *>(tC + i * NP + m);
             const bool cut = !W && (rst >> i & 1);
+            const int left = W ? NL : states_left(p.N, s * NL);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               e[i][j] = __builtin_amdgcn_exp2f(dl * A[m + j]);
               const float in = dxi * (j ? B.y : B.x);
               h[i + 1][j] = cut ? in : fmaf(e[i][j], h[i][j], in);
+              if (!W && m + j >= left) e[i][j] = h[i + 1][j] = 0.f;
               yc[i] = fmaf(h[i + 1][j], j ? C.y : C.x, yc[i]);
             }
           } else {
@@ -571,10 +602,12 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
             const float dl = st[0], dxi = st[1], dyi = st[2];
             const float2 B = *reinterpret_cast<const float2 *>(tB + i * NP + m), C = *reinterpret_cast<const float2 *>(tC + i * NP + m);
             const bool cut = !W && (rst >> i & 1);
+            const int left = W ? NL : states_left(p.N, s * NL);
             float v[4];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const float g = fmaf(dyi, j ? C.y : C.x, carry[m + j]);
+              float g = fmaf(dyi, j ? C.y : C.x, carry[m + j]);
+              if (!W && m + j >= left) g = 0.f;
               float ga = g * e[i][j], q = ga * h[i][j];
               if (cut) ga = q = 0.f;
               dd[i] = fmaf(q, A[m + j], dd[i]);        // (A log2 e: undone at the end)
@@ -599,7 +632,7 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
         }
       }
     };
-    if (rst == 0 && nt == TS) tile(std::true_type());
+    if (rst == 0 && nt == TS && !wild) tile(std::true_type());
     else tile(std::false_type());
     if (t > t0) put(buf ^ 1);
     __syncthreads();                             // red of this tile and the rows of the next one are there
@@ -616,9 +649,9 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
           dskip = fmaf(dy[q], x[q], dskip);
           dbias += ddt;
           const int64_t o = o0 + (int64_t)(t + q * S) * o_st;
-          reinterpret_cast<T *>(p.dx)[o] = from_f<T>(fmaf(skip, dy[q], del[q] * go[q]));
+          reinterpret_cast<T *>(p.dx)[o] = from_f<T>(p.skip ? fmaf(skip, dy[q], del[q] * go[q]) : del[q] * go[q]);
           reinterpret_cast<T *>(p.ddt)[o] = from_f<T>(ddt);
-          if (p.z && p.dz) reinterpret_cast<T *>(p.dz)[o] = from_f<T>(zf[q] * fmaf(skip, x[q], yo[q]));
+          if (p.z && p.dz) reinterpret_cast<T *>(p.dz)[o] = from_f<T>(zf[q] * (p.skip ? fmaf(skip, x[q], yo[q]) : yo[q]));
         }
       }
     }
@@ -741,7 +774,7 @@ __global__ __launch_bounds__(256) void k_scan_step(fdql_scan_t p, int Dg, int tp
     const float back = __shfl(acc, (lane % cpt) * lpc);            // the sum of channel it * cpt + (lane % cpt)
     if (lane / cpt == it) y = back;
   }
-  y = fmaf(p.skip ? p.skip[d] : 0.f, x, y);
+  if (p.skip) y = fmaf(p.skip[d], x, y);
   if (p.z) {
     const float z = to_f(reinterpret_cast<const T *>(p.z)[(int64_t)r * p.z_sr + d]);
     y *= z * sigmoid_f<T>(z).s;
@@ -782,7 +815,7 @@ __global__ __launch_bounds__(256) void k_scan_step_few(fdql_scan_t p, int Dg, in
     if (p.state_out && live) *reinterpret_cast<vec *>(p.state_out + (int64_t)r * p.state_out_sr + at) = h;
   }
   for (int m = 1; m < lpc; m <<= 1) acc += __shfl_xor(acc, m);
-  float y = fmaf(skip, x, acc);
+  float y = p.skip ? fmaf(skip, x, acc) : acc;
   if (p.z) y *= z * sigmoid_f<T>(z).s;
   if (sub == 0 && live) reinterpret_cast<T *>(p.y)[(int64_t)r * p.D + d] = from_f<T>(y);
 }

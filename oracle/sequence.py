@@ -78,7 +78,6 @@ def selective_scan(x, dt, A, B, C, skip=None, z=None, dt_bias=None, softplus=Tru
     G, N = B.shape[-2:]
     h = torch.zeros(R, D, N, dtype=torch.float64) if state is None else _f64(state)
     rst = torch.zeros(T, R, dtype=torch.bool) if reset is None else reset.cpu().bool()
-    skip = torch.zeros(D, dtype=torch.float64) if skip is None else skip
     raw = dt if dt_bias is None else dt + dt_bias
     delta = torch.logaddexp(raw, torch.zeros((), dtype=torch.float64)) if softplus else raw
     slope = torch.sigmoid(raw) if softplus else torch.ones_like(raw)
@@ -86,6 +85,7 @@ def selective_scan(x, dt, A, B, C, skip=None, z=None, dt_bias=None, softplus=Tru
     gate = torch.ones_like(x) if z is None else z * sg
     decay = torch.exp(delta[..., None] * A)
     x, B, C, skip, gate, h = (_abs(t, mag) for t in (x, B, C, skip, gate, h))
+    direct = lambda m: 0.0 if skip is None else skip * m  # noqa: E731
     step = _abs(delta, mag)
     wide = lambda m: m.repeat_interleave(D // G, 1)  # noqa: E731
     fold = lambda m: m.view(R, G, D // G, N).sum(2)  # noqa: E731
@@ -94,7 +94,7 @@ def selective_scan(x, dt, A, B, C, skip=None, z=None, dt_bias=None, softplus=Tru
     for t in range(T):
         h = torch.where(rst[t][:, None, None], zero, decay[t] * h) + (step[t] * x[t])[..., None] * wide(B[t])
         hs.append(h)
-        core.append((h * wide(C[t])).sum(-1) + skip * x[t])
+        core.append((h * wide(C[t])).sum(-1) + direct(x[t]))
     core = torch.stack(core) if T else torch.zeros_like(x)
     out = {"y": core * gate, "state": h}
     if dy is None:
@@ -109,7 +109,7 @@ def selective_scan(x, dt, A, B, C, skip=None, z=None, dt_bias=None, softplus=Tru
         carry = torch.where(rst[t][:, None, None], zero, g * decay[t])
         past = torch.where(rst[t][:, None, None], zero, g * decay[t] * hs[t])
         gb = (g * wide(B[t])).sum(-1)
-        dx[t] = skip * g_core[t] + step[t] * gb
+        dx[t] = direct(g_core[t]) + step[t] * gb
         ddt[t] = ((past * Am).sum(-1) + gb * x[t]) * slope[t]
         dA += (past * step[t][..., None]).sum(0)
         dB[t] = fold(g * (step[t] * x[t])[..., None])

@@ -141,3 +141,55 @@ def test_small_gated_outputs_keep_their_digits(dev, seq, M, kind):
     f, df = {"silu": (g * s, s * (1 + g * c)), "sigmoid": (s, s * c), "gelu": (g * cdf, cdf + g * pdf)}[kind]
     _relative("y", y[:, 0], f, 24 if kind == "gelu" else 16)
     _relative("dx", torch.autograd.grad(y, x, torch.ones_like(y))[0][:, 0], df, 24 if kind == "gelu" else 16)
+
+
+def _same(name, got, want, rel=1e-3):
+    """Infinities and NaN where the definition has them, the rest near (a check of special values: errors are measured elsewhere)."""
+    got = got.detach().cpu().double()
+    assert torch.equal(got.isnan(), want.isnan()), f"{name}: NaN in {int((got.isnan() != want.isnan()).sum())} wrong places"
+    inf = want.isinf()
+    assert torch.equal(got[inf], want[inf]) and not got[~inf & ~want.isnan()].isinf().any(), f"{name}: infinities"
+    ok = want.isfinite()
+    assert torch.allclose(got[ok], want[ok], rtol=rel, atol=rel * float(want[ok].abs().max() if ok.any() else 1.0)), name
+
+
+@pytest.mark.parametrize("T,R,D,G", [(9, 2, 21, 1), (160, 2, 38, 2)])
+@pytest.mark.parametrize("N", [1, 3, 4, 5, 7, 8, 12, 16, 20, 32, 33, 64])
+@pytest.mark.parametrize("form", ["x", "dt", "dy", "carried", "bare", "nan"])
+def test_scan_infinite_values_stay_where_they_are(dev, seq, T, R, D, N, G, form):
+    """An infinite input, step, gradient or carried state gives the infinities of the definition and no NaN beside them, in windows (whole and cut into
+    segments) and in steps, for every number of states and with channels that leave a wave part empty; a NaN stays in its channel."""
+    i, _, dy, _ = _scan_inputs(dev, T, R, D, N, G, torch.float32, "dense", seed=N)
+    for k in ("x", "dt", "B", "C", "state"):
+        i[k] = i[k].abs() + 0.1
+    i["dt"], dy, inf = i["dt"] * 0.2, dy.abs() + 0.1, float("inf")
+    i["z"] = None
+    i["skip"] = None if form == "bare" else i["skip"].abs() + 0.1
+    at = T // 2
+    for d in (1, D - 1):         # the last channel is the one that lanes without a channel look at
+        if form in ("x", "bare"):
+            i["x"][at, 1, d] = inf
+        elif form == "dt":
+            i["dt"][at, 1, d] = inf
+        elif form == "dy":
+            dy[at, 1, d] = inf
+        elif form == "carried":
+            i["state"][1, d] = inf
+        else:
+            i["x"][at, 1, d] = float("nan")
+    o = osq.selective_scan(**i, dy=None if form == "dt" else dy)
+    with torch.no_grad():
+        y, st = _scan_call(seq, i, None, True, return_state=True)
+        h = i["state"]
+        for t in range(T if T < 20 else 0):
+            yt, h = seq.selective_scan_step(i["x"][t], i["dt"][t], i["A"], i["B"][t], i["C"][t], h, skip=i["skip"], dt_bias=i["dt_bias"])
+            _same("step y", yt, o["y"][t])
+        _same("y", y, o["y"])
+        _same("state", st, o["state"])
+        assert T >= 20 or torch.equal(h.isnan(), st.isnan())
+    if form == "dt":             # (0 * inf in the definition's own gradients)
+        return
+    leaves = {k: v.detach().requires_grad_() for k, v in i.items() if v is not None}
+    y = _scan_call(seq, {k: leaves.get(k) for k in i}, None, True)
+    for k, g in zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)):
+        _same("d" + k, g, o["d" + k])

@@ -254,10 +254,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
           const float dl = v.x, dx = v.y;
           const int left = decltype(whole)::value ? NL : states_left(p.N, s * NL);
           if (CARRY) sum += dl;
-          if (!decltype(whole)::value && (rst >> i & 1)) {
-#pragma unroll
-            for (int j = 0; j < NL; ++j) h[j] = 0.f;
-          }
+          const bool cut = !decltype(whole)::value && (rst >> i & 1);
 #pragma unroll
           for (int j4 = 0; j4 < NL; j4 += VW) {
             const vec B = *reinterpret_cast<const vec *>(lB + i * NP + s * NL + j4);
@@ -265,7 +262,8 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
             if (!CARRY) C = *reinterpret_cast<const vec *>(lC + i * NP + s * NL + j4);
 #pragma unroll
             for (int j = 0; j < VW; ++j) {
-              h[j4 + j] = fmaf(__builtin_amdgcn_exp2f(dl * A[j4 + j]), h[j4 + j], dx * B[j]);
+              const float in = dx * B[j], on = fmaf(__builtin_amdgcn_exp2f(dl * A[j4 + j]), h[j4 + j], in);
+              h[j4 + j] = cut ? in : on;        // (selected: a decay beyond float's range times zero would not be nothing)
               if (!decltype(whole)::value && j4 + j >= left) h[j4 + j] = 0.f;
               if (!CARRY) acc[i] = fmaf(h[j4 + j], C[j], acc[i]);
             }

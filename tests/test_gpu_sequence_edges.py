@@ -193,3 +193,49 @@ def test_scan_infinite_values_stay_where_they_are(dev, seq, T, R, D, N, G, form)
     y = _scan_call(seq, {k: leaves.get(k) for k in i}, None, True)
     for k, g in zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)):
         _same("d" + k, g, o["d" + k])
+
+
+@pytest.mark.parametrize("T,N", [(6, 4), (6, 5), (9, 16), (170, 4), (170, 16), (170, 33)])
+@pytest.mark.parametrize("form", ["positive A", "negative step"])
+def test_scan_growth_beyond_floats_range_ends_at_a_reset(dev, seq, T, N, form):
+    """A decay that overflows (positive A, or negative steps without the softplus) is dropped with the state it would multiply: the step that begins a sequence
+    has its own input alone, in windows, their segments and backward, and in single steps."""
+    R, D = 2, 20
+    i, _, dy, _ = _scan_inputs(dev, T, R, D, N, 1, torch.float32, "dense", seed=4)
+    i.update(state=None, dt_bias=None, dt=torch.full((T, R, D), 1e-3, device=dev), A=-torch.ones(D, N, device=dev))
+    at = [3, T - 2] if T < 20 else [3, 60, T - 2]
+    rst = torch.zeros(T, R, dtype=torch.bool, device=dev)
+    for t in at:                             # e^(delta A) = e^200 there
+        rst[t, 1] = True
+        i["dt"][t, 1] = 200.0 if form == "positive A" else -200.0
+    if form == "positive A":
+        i["A"] = -i["A"]
+    args = dict(i, softplus=False, reset=rst, dy=dy)
+    o = osq.selective_scan(**args)
+    assert all(v.isfinite().all() for v in o.values())
+    leaves = {k: v.detach().requires_grad_() for k, v in i.items() if v is not None}
+    li = {k: leaves.get(k) for k in i}
+    y, st = _scan_call(seq, li, rst, False, return_state=True)
+    _same("y", y, o["y"])
+    _same("state", st, o["state"])
+    for k, g in zip(leaves, torch.autograd.grad(y, list(leaves.values()), dy)):
+        _same("d" + k, g, o["d" + k])
+    with torch.no_grad():
+        h = torch.zeros(R, D, N, device=dev)
+        for t in range(T if T < 20 else 0):
+            yt, h = seq.selective_scan_step(i["x"][t], i["dt"][t], i["A"], i["B"][t], i["C"][t], h, skip=i["skip"], z=i["z"][t], dt_softplus=False, reset=rst[t])
+            _same("step", yt, o["y"][t])
+
+
+def test_join_of_segments_whose_decays_leave_floats_range(dev, seq):
+    """32 steps of e^3.125: e^100 in one piece is beyond float's range, a state of 2e-38 reaches 5e5 by it and one of zeros stays zeros."""
+    T, D, N = 192, 4, 4
+    dt = torch.zeros(T, 2, D, device=dev)
+    dt[:32] = 3.125
+    h0 = torch.full((2, D, N), 2e-38, device=dev)
+    h0[1] = 0.0
+    x, B, C = torch.zeros(T, 2, D, device=dev), torch.zeros(T, 2, N, device=dev), torch.ones(T, 2, N, device=dev)
+    y, st = seq.selective_scan(x, dt, torch.ones(D, N, device=dev), B, C, dt_softplus=False, initial_state=h0, return_state=True)
+    o = osq.selective_scan(x, dt, torch.ones(D, N), B[:, :, None], C[:, :, None], softplus=False, state=h0)
+    _same("y", y, o["y"])
+    _same("state", st, o["state"])

@@ -138,18 +138,10 @@ void plain(const char *what, std::initializer_list<Tensor> ts) {
 void written(const Tensor &t) {
   if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
-// A backward pass under capture that reaches a node which eager code has made on the default stream - a leaf's accumulator that an eager graph keeps
-// alive, or such a graph itself - would have that stream wait for the capture, which is not allowed and ends the process.  So every node in
-// front of this one that the pass will run is looked at, and the call refuses instead.  (Costs nothing outside a capture.)
-void capturable(const char *what, const Tensor &x) {
-  const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index());
-  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) {
-    (void)hipGetLastError();                // (no stream that could be captured: the next launch must not find this error)
-    return;
-  }
-  if (status == hipStreamCaptureStatusNone) return;
-  const c10::Stream here = stream.unwrap(), eager = c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(x.device().index()).unwrap();
+// Every node that the running backward pass will run behind (in its order) the node that runs now, once each, until `stop` says so: that node, or null.
+// A pass for chosen inputs runs part of a graph only.
+template <typename F>
+torch::autograd::Node *nodes_ahead(F stop) {
   const auto node = torch::autograd::get_current_node();
   const auto *runs = torch::autograd::get_current_graph_task_exec_info();       // empty: every node does
   std::vector<torch::autograd::Node *> todo;
@@ -165,12 +157,30 @@ void capturable(const char *what, const Tensor &x) {
         const auto it = runs->find(f);
         if (it == runs->end() || !it->second.should_execute()) continue;
       }
-      const auto at = f->stream();
-      TORCH_CHECK(!at || *at == here || *at != eager, what, ": this backward pass is being captured and reaches an eager graph on the default stream (", f->name(),
-                  "); delete what holds that graph (its outputs, its loss) before the capture");
+      if (stop(f)) return f;
       todo.push_back(f);
     }
   }
+  return nullptr;
+}
+// A backward pass under capture that reaches a node which eager code has made on the default stream - a leaf's accumulator that an eager graph keeps
+// alive, or such a graph itself - would have that stream wait for the capture, which is not allowed and ends the process.  The call refuses
+// instead.  (Costs nothing outside a capture.)
+void capturable(const char *what, const Tensor &x) {
+  const auto stream = c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &status) != hipSuccess) {
+    (void)hipGetLastError();                // (no stream that could be captured: the next launch must not find this error)
+    return;
+  }
+  if (status == hipStreamCaptureStatusNone) return;
+  const c10::Stream here = stream.unwrap(), eager = c10::hip::getDefaultHIPStreamMasqueradingAsCUDA(x.device().index()).unwrap();
+  const torch::autograd::Node *bad = nodes_ahead([&](torch::autograd::Node *f) {
+    const auto at = f->stream();
+    return at && *at != here && *at == eager;
+  });
+  TORCH_CHECK(!bad, what, ": this backward pass is being captured and reaches an eager graph on the default stream (", bad->name(),
+              "); delete what holds that graph (its outputs, its loss) before the capture");
 }
 // Gradients of a backward pass that itself is recorded (create_graph) depend on everything in `from`: differentiating them again is an error, not a silent
 // zero.
@@ -569,4 +579,9 @@ PYBIND11_MODULE(_seq_torch, m) {
   m.def("selective_scan", &selective_scan, free_gil());
   m.def("selective_scan_step", &selective_scan_step, free_gil());
   m.def("gated_linear", &gated_linear, free_gil());
+  m.def("nodes_ahead", [] {            // names of the nodes that a captured backward pass is checked against, for the tests of that check
+    std::vector<std::string> names;
+    nodes_ahead([&](torch::autograd::Node *f) { return names.push_back(f->name()), false; });
+    return names;
+  });
 }

@@ -239,3 +239,39 @@ def test_join_of_segments_whose_decays_leave_floats_range(dev, seq):
     o = osq.selective_scan(x, dt, torch.ones(D, N), B[:, :, None], C[:, :, None], softplus=False, state=h0)
     _same("y", y, o["y"])
     _same("state", st, o["state"])
+
+
+@pytest.mark.parametrize("form", ["view", "operators"])
+def test_capturing_beside_an_eager_graph_further_ahead_is_refused(dev, seq, form):
+    """The leaf whose accumulator an eager graph keeps on the default stream lies behind a view (gated_linear of a 3-dimensional x), or behind two more
+    operators: the call raises, and works once the eager graph is gone.  (What the check walks over is tested without a GPU: nodes_ahead.)"""
+    g = _gen(7)
+    leaf = torch.randn(6, 2, 8, generator=g).to(dev).requires_grad_()
+    w, B, wg, A = torch.randn(8, 4, generator=g).to(dev), torch.randn(6, 2, 4, generator=g).to(dev), torch.randn(5, 8, generator=g).to(dev), -torch.rand(8, 4, generator=g).to(dev)
+
+    def call():
+        x = leaf
+        if form == "operators":
+            x = seq.causal_conv(x, w)
+            x = seq.selective_scan(x, torch.ones_like(x), A, B, B)
+        return seq.gated_linear(x, wg, wg)
+    step = lambda: torch.autograd.grad(call().sum(), [leaf])[0]  # noqa: E731
+    want = step()
+    side = torch.cuda.Stream(dev)
+    side.wait_stream(torch.cuda.current_stream(dev))
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream(dev).wait_stream(side)
+    alive = call()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            step()
+    del alive
+    torch.cuda.synchronize(dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize(dev)
+        assert torch.equal(got, want) and torch.equal(step(), want)

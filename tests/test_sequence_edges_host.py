@@ -97,3 +97,40 @@ def test_functional_transforms_are_refused():
     for transform in (torch.vmap, torch.func.grad):
         with pytest.raises(ValueError, match="plain tensors"):
             transform(lambda a: seq.gated_linear(a, w, w).sum())(torch.ones(2, 2, 4))
+
+
+class _Looks(torch.autograd.Function):
+    """Identity whose backward pass notes what the binding sees ahead of it."""
+    seen = []
+
+    @staticmethod
+    def forward(ctx, *xs):
+        return sum(x.sum() for x in xs)
+
+    @staticmethod
+    def backward(ctx, g):
+        _Looks.seen.append(sorted(seq._ops().nodes_ahead()))
+        return tuple(g.expand(6) for _ in ctx.needs_input_grad)
+
+
+def _ahead(run):
+    _Looks.seen = []
+    run()
+    return _Looks.seen[0]
+
+
+def test_nodes_that_a_backward_pass_will_run():
+    """What a captured backward pass is checked against: leaves behind views and behind other operators, each once, nothing that the pass leaves out."""
+    leaf, other = torch.ones(2, 3, requires_grad=True), torch.ones(6, requires_grad=True)
+    acc = "torch::autograd::AccumulateGrad"
+    assert _ahead(lambda: _Looks.apply(other).backward()) == [acc]                                                            # a leaf itself
+    assert _ahead(lambda: _Looks.apply(leaf.view(6)).backward()) == sorted(["ViewBackward0", acc])                            # a leaf behind a view
+    deep = (leaf * 2).view(6).exp()
+    assert _ahead(lambda: _Looks.apply(deep, deep).backward()) == sorted(["ExpBackward0", "ViewBackward0", "MulBackward0", acc])      # node -> node -> leaf, met twice
+    both = lambda: _Looks.apply(leaf.view(6), other.exp())  # noqa: E731
+    assert _ahead(lambda: both().backward()) == sorted(["ViewBackward0", "ExpBackward0", acc, acc])
+    assert _ahead(lambda: torch.autograd.grad(both(), [leaf])) == sorted(["ViewBackward0", acc])                              # chosen inputs: their way only
+    assert _ahead(lambda: torch.autograd.grad(both(), [other])) == sorted(["ExpBackward0", acc])
+    middle = leaf.view(6)
+    assert _ahead(lambda: torch.autograd.grad(_Looks.apply(middle.exp()), [middle])) == ["ExpBackward0", "ViewBackward0"]     # (stops at the input's own node)
+    assert seq._ops().nodes_ahead() == []                                                                                     # outside a pass

@@ -17,6 +17,7 @@ LIB_PATH = os.environ.get("FDQL_LIB_PATH") or os.path.join(_HERE, "libfdql_hip.s
 FDQL_OK, FDQL_EINVAL, FDQL_EHIP, FDQL_EOVERSAMPLE, FDQL_ESTATE, FDQL_ENOMEM = 0, -1, -2, -3, -4, -5
 PHASE_ALL, PHASE_GRAD, PHASE_APPLY, PHASE_GRAD_CRITICS, PHASE_GRAD_REST = 0, 1, 2, 3, 4
 MAX_HIDDEN = 4
+VERSION = 2     # FDQL_VERSION of the header that this file mirrors
 MAX_CONV = 3
 
 
@@ -209,6 +210,8 @@ def load():
         fn = getattr(lib, name)  # AttributeError if the library does not export it
         fn.restype = res
         fn.argtypes = args
+    if lib.fdql_version() != VERSION:
+        raise ImportError(f"_native.py mirrors version {VERSION} of include/fdql.h, libfdql_hip.so has {lib.fdql_version()}")
     sizes = (C.c_int32 * 6)()
     lib.fdql_abi_sizes(sizes)
     mine = [C.sizeof(x) for x in (AgentConfig, Batch, AgentStats, KernelTime, RewardFn, EpisodeSpec)]

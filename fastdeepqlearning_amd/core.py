@@ -259,7 +259,7 @@ def make_config(obs_dim, act_dim, T, B, goal_dim=0, discrete=False, n_critics=2,
             arr[i] = v
     c.distributional, c.use_lowerbound, c.use_max_entropy = int(distributional), int(use_lowerbound), int(use_max_entropy)
     c.hard_updates, c.keep_frozen_copy = int(hard_updates), int(keep_frozen_copy)
-    c.bootstrap_nstep = int(bootstrap_nstep)
+    c.bootstrap_nstep = int(bool(bootstrap_nstep))
     c.burn_in_steps = int(burn_in_steps)
     c.obs_2d_u8 = int(bool(obs_2d_u8) and bool(img))
     if img:      # pixel encoder (a design of this build: the reference has none)

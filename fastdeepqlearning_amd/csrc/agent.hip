@@ -168,7 +168,7 @@ int prepare_update(fdql_agent *a, const fdql_batch_t *batch, const float *noise_
 extern "C" {
 
 const char *fdql_last_error(void) { return g_err; }
-int fdql_version(void) { return 1; }
+int fdql_version(void) { return FDQL_VERSION; }
 void fdql_abi_sizes(int32_t *out6) {
   out6[0] = (int32_t)sizeof(fdql_agent_config_t);
   out6[1] = (int32_t)sizeof(fdql_batch_t);
@@ -181,6 +181,10 @@ void fdql_abi_sizes(int32_t *out6) {
 int fdql_agent_create(fdql_agent_t **out, const fdql_agent_config_t *cfg) {
   FDQL_REQUIRE(out && cfg, "null argument");
   const fdql_agent_config_t &c = *cfg;
+  // the struct of version 1 puts T (at least 2) and B where these two stand
+  FDQL_REQUIRE((c.bootstrap_nstep & ~1) == 0 && (c.obs_2d_u8 & ~1) == 0,
+               "bootstrap_nstep %d and obs_2d_u8 %d must be 0 or 1 (a client built with a header before version %d? see fdql_version)", c.bootstrap_nstep, c.obs_2d_u8,
+               FDQL_VERSION);
   FDQL_REQUIRE(c.obs_dim >= 0 && c.act_dim > 0 && c.goal_dim >= 0 && c.img_c >= 0 && (c.obs_dim > 0 || c.img_c > 0),
                "bad obs/act/goal dims");
   if (c.img_c > 0) {

@@ -42,6 +42,9 @@ extern "C" {
 #define FDQL_ENOMEM (-5)
 
 const char *fdql_last_error(void);
+/* 1 up to the GRU joiner; 2: fdql_agent_config_t has joiner_ssm, ssm_inner and ssm_state behind gru_state_mode.  Compare it with FDQL_VERSION: a client
+ * that was built with another header hands in structs of another layout. */
+#define FDQL_VERSION 2
 int fdql_version(void);
 /* sizeof() of the structs below as this library was compiled, so a binding can verify its
  * own mirror: out[0]=fdql_agent_config_t, [1]=fdql_batch_t, [2]=fdql_agent_stats_t,

@@ -70,6 +70,16 @@ int check_workspace(const char *what, const void *ws, int64_t have, int64_t need
                (long long)need);
   return FDQL_OK;
 }
+// Do two sets of R rows of `len` bytes, sa and sb bytes apart, share memory?  Rows equally far apart may lie between each other (columns of one wider
+// row); of others the whole ranges count.
+bool rows_meet(const void *a, int64_t sa, const void *b, int64_t sb, int64_t R, int64_t len) {
+  const auto lo = [&](const void *p, int64_t s) { return (int64_t)(intptr_t)p + (s < 0 ? s * (R - 1) : 0); };
+  const auto hi = [&](const void *p, int64_t s) { return (int64_t)(intptr_t)p + (s > 0 ? s * (R - 1) : 0) + len; };
+  if (!a || !b || lo(a, sa) >= hi(b, sb) || lo(b, sb) >= hi(a, sa)) return false;
+  if (sa != sb || sa <= 0) return true;
+  const int64_t off = (((int64_t)(intptr_t)b - (int64_t)(intptr_t)a) % sa + sa) % sa;
+  return off < len || off > sa - len;
+}
 #define FDQL_TRY(call)              \
   do {                              \
     const int _rc = (call);         \
@@ -107,10 +117,13 @@ hipError_t ssm_dalog_launch(const float *dA, const float *A, int n, float *out, 
 extern "C" int fdql_causal_conv(const fdql_causal_conv_t *p, void *stream) {
   FDQL_TRY(check_conv(p));
   if (p->R == 0) return FDQL_OK;
-  FDQL_REQUIRE(p->weight && (p->T == 0 || (p->x && p->y)), "causal_conv: x, weight and y are needed");
   FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1), "causal_conv: the state is updated in place only in a single step");
   FDQL_REQUIRE(!p->state_out || p->R == 1 || p->state_out_sr >= (p->K - 1ll) * p->D, "causal_conv: rows of state_out %lld apart overlap", (long long)p->state_out_sr);
   FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || p->state_in_sr == p->state_out_sr, "causal_conv: a state updated in place has one row stride");
+  const int64_t esz = p->dtype == FDQL_F32 ? 4 : 2;
+  FDQL_REQUIRE(p->state_out == p->state_in || !rows_meet(p->state_in, p->state_in_sr * esz, p->state_out, p->state_out_sr * esz, p->R, (p->K - 1ll) * p->D * esz),
+               "causal_conv: state_out overlaps state_in in other places");
+  FDQL_REQUIRE(p->weight && (p->T == 0 || (p->x && p->y)), "causal_conv: x, weight and y are needed");
   FDQL_HIP(seqconv_fwd_launch(*p, (hipStream_t)stream));
   return FDQL_OK;
 }
@@ -138,6 +151,8 @@ extern "C" int fdql_scan(const fdql_scan_t *p, void *stream) {
   FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || (p->T == 1 && !p->checkpoints), "scan: the state is updated in place only in a single step");
   FDQL_REQUIRE(!p->state_out || p->R == 1 || p->state_out_sr >= (int64_t)p->D * p->N, "scan: rows of state_out %lld apart overlap", (long long)p->state_out_sr);
   FDQL_REQUIRE(!p->state_out || p->state_out != p->state_in || p->state_in_sr == p->state_out_sr, "scan: a state updated in place has one row stride");
+  FDQL_REQUIRE(p->state_out == p->state_in || !rows_meet(p->state_in, p->state_in_sr * 4, p->state_out, p->state_out_sr * 4, p->R, (int64_t)p->D * p->N * 4),
+               "scan: state_out overlaps state_in in other places");
   if (p->T == 0) return copy_rows(p->state_in, p->state_in_sr, p->state_out, p->state_out_sr, p->R, (int64_t)p->D * p->N, s);
   FDQL_REQUIRE(p->x && p->dt && p->A && p->B && p->C && p->y, "scan: x, dt, A, B, C and y are needed");
   FDQL_TRY(check_workspace("scan", p->workspace, p->workspace_bytes, scan_workspace_bytes(*p, false)));

@@ -51,7 +51,8 @@ def causal_conv(x, weight, bias=None, *, reset=None, initial_state=None, silu=Tr
 
 def causal_conv_step(x, state, weight, bias=None, *, reset=None, silu=True, out_state=None):
     """One step of causal_conv for every row: x [rows, D], state [rows, K-1, D], reset [rows].  Returns (y, new state); the new state is
-    written to out_state (rows dense, any distance apart; `state` itself updates it in place, other overlaps are not allowed) or to a new tensor."""
+    written to out_state (rows dense, any distance apart; `state` itself updates it in place, rows that overlap in another way are
+    refused) or to a new tensor."""
     return (_bound or _ops()).causal_conv_step(x, state, weight, bias, reset, silu, out_state)
 
 
@@ -68,7 +69,7 @@ def selective_scan(x, dt, A, B, C, *, skip=None, z=None, dt_bias=None, dt_softpl
 def selective_scan_step(x, dt, A, B, C, state, *, skip=None, z=None, dt_bias=None, dt_softplus=True, reset=None, out_state=None):
     """One step of selective_scan for every row: x, dt, z [rows, D], B, C [rows, (groups,) n], state [rows, D, n], reset [rows].  Returns
     (y, new state); the new state is written to out_state (rows dense, any distance apart; `state` itself
-    updates it in place, other overlaps are not allowed) or to a new tensor."""
+    updates it in place, rows that overlap in another way are refused) or to a new tensor."""
     return (_bound or _ops()).selective_scan_step(x, dt, A, B, C, state, skip, z, dt_bias, dt_softplus, reset, out_state)
 
 

@@ -447,7 +447,7 @@ int32_t fdql_agent_profile_update(fdql_agent_t *agent, const fdql_batch_t *batch
 /* y_t = f(bias + sum_{j<K} weight[:, K-1-j] * x_{t-j}), f = SiLU or identity, channel by channel; x_{t-j} counts as zero when a
  * reset lies in (t-j, t].  Inputs before step 0 come from state_in [R, K-1, D] (row stride state_in_sr, oldest first; NULL: zeros); state_out
  * [R, K-1, D] (row stride state_out_sr >= (K-1) D; or NULL) receives the last K-1 inputs (zeros for those before the last reset).  state_out may be
- * state_in, with the same stride, when T == 1.
+ * state_in, with the same stride, when T == 1; rows that overlap in another way are refused.
  * Backward: dy [T, R, D] (strides dy_st, dy_sr) and dstate_out (or NULL) -> dx, dweight [D, K], dbias [D], dstate_in (each or NULL).                  */
 typedef struct {
   int32_t size, dtype;
@@ -479,7 +479,7 @@ int fdql_causal_conv_backward(const fdql_causal_conv_t *p, void *stream);
  *   h     = exp(delta * A[d]) * h + delta * x_t * B_t[g]      (the first term dropped at a reset)
  *   y_t   = (C_t[g] . h + skip[d] * x_t) * SiLU(z_t)          (factors that are NULL left out)
  * state_in [R, D, N] (row stride state_in_sr, NULL: zeros), state_out [R, D, N] (row stride state_out_sr >= D N; or NULL; may be state_in,
- * with the same stride, when T == 1).
+ * with the same stride, when T == 1; rows that overlap in another way are refused).
  * checkpoints: fdql_scan_checkpoint_floats() floats that the forward call fills for the backward call of the same inputs (NULL
  * when there is none).  Backward: dy (strides dy_st, dy_sr) and dstate_out (or NULL) -> every gradient; those of optional inputs that are NULL may be NULL,
  * dstate_in always.                                                                                              */

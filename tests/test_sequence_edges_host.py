@@ -6,7 +6,7 @@ import torch
 
 from fastdeepqlearning_amd import _native as nat
 from fastdeepqlearning_amd import sequence as seq
-from test_sequence_host import P, _gated
+from test_sequence_host import P, _conv, _gated, _scan
 
 ROUND = 0x100      # FDQL_GATED_ROUND_GRADS
 
@@ -134,3 +134,25 @@ def test_nodes_that_a_backward_pass_will_run():
     middle = leaf.view(6)
     assert _ahead(lambda: torch.autograd.grad(_Looks.apply(middle.exp()), [middle])) == ["ExpBackward0", "ViewBackward0"]     # (stops at the input's own node)
     assert seq._ops().nodes_ahead() == []                                                                                     # outside a pass
+
+
+@pytest.mark.parametrize("entry,make,kw,row", [("fdql_causal_conv", _conv, dict(x=P, weight=P, y=P), 24 * 4), ("fdql_causal_conv", _conv, dict(x=P, weight=P, y=P, dtype=2), 24 * 2),
+                                               ("fdql_scan", _scan, dict(x=P, dt=P, A=P, B=P, C=P, y=P), 32 * 4)])
+def test_states_that_share_memory_are_refused(entry, make, kw, row):
+    """Rows of the new state on top of other rows or of parts of rows of the old one; columns side by side in one buffer get past this check (and are
+    refused for what else this struct lacks, before anything is launched)."""
+    lib, esz = nat.load(), 2 if kw.get("dtype") else 4
+    base = 1 << 20
+
+    def call(off, so, si, T=1, **more):
+        s = make(state_in=base, state_in_sr=si // esz, state_out=base + off, state_out_sr=so // esz, T=T, **{**kw, **more})
+        assert getattr(lib, entry)(C.byref(s), None) == nat.FDQL_EINVAL
+        return lib.fdql_last_error().decode()
+    for off, so, si in ((esz, row, row), (-esz, row, row), (row, row, row), (esz, 3 * row, 3 * row), (2 * row + esz, 3 * row, 3 * row), (row, 2 * row, row), (0, row, 0), (row - esz, row, 0)):
+        if off == 0 and so != si:
+            assert "row stride" in call(off, so, si)
+        else:
+            assert "overlaps" in call(off, so, si) and "overlaps" in call(off, so, si, T=4), (off, so, si)
+    missing = {"fdql_causal_conv": dict(x=None), "fdql_scan": dict(x=None)}[entry]
+    for off, so, si in ((2 * row, row, row), (row, 3 * row, 3 * row), (-row, 3 * row, 3 * row), (2 * row, 3 * row, 3 * row), (row, row, 0)):
+        assert "overlap" not in call(off, so, si, **missing), (off, so, si)

@@ -275,3 +275,26 @@ def test_capturing_beside_an_eager_graph_further_ahead_is_refused(dev, seq, form
         graph.replay()
         torch.cuda.synchronize(dev)
         assert torch.equal(got, want) and torch.equal(step(), want)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("T,R,D,N,G", [(50, 16, 512, 16, 1), (50, 2, 128, 16, 2), (16, 4, 200, 64, 1), (9, 30, 65, 5, 1), (300, 2, 72, 33, 2), (1100, 1, 96, 8, 1)])
+def test_scan_errors_are_a_few_roundings(dev, seq, T, R, D, N, G, dtype):
+    """Error norms.  A step adds about five roundings of the state's size (the decay's exponent and power, the input, the sum), each of variance u^2 / 3, u =
+    2^-24; a state of m remembered steps is itself a sum of m terms, so against its own size they add up to u sqrt(5 m / 3), m at most T.  A's own
+    rounding is the same at every step, but a state forgets it by the rate that it is off by: it, the sum over states, the gate and the step size add a
+    few u, 4 here.  The whole is allowed twice (resets and decays shorten the memory: a lost digit shows below 100 steps); 16-bit results add one rounding of their own (5% for its scatter
+    over 500 values and more, as a norm)."""
+    i, rst, dy, ds = _scan_inputs(dev, T, R, D, N, G, dtype, "dense", seed=T + D)
+    leaves = {k: v.detach().requires_grad_() for k, v in i.items()}
+    y, state = _scan_call(seq, leaves, rst, True, return_state=True)
+    got = dict(zip(("d" + k for k in leaves), torch.autograd.grad([y, state], list(leaves.values()), [dy, ds])), y=y, state=state)
+    o = osq.selective_scan(**i, reset=rst, dy=dy, dstate=ds)
+    own = 2 * ((5 * T / 3) ** 0.5 + 4) * U32
+    worst = {}
+    for k, v in got.items():
+        once = float((o[k].to(v.dtype).double() - o[k]).norm())
+        off = float((v.detach().cpu().double() - o[k]).norm())
+        worst[k] = off / (own * float(o[k].norm()) + (1.05 * once if v.dtype != torch.float32 else 0.0))
+    print(T, R, D, N, dtype, {k: round(v, 3) for k, v in worst.items()})
+    assert max(worst.values()) <= 1.0, worst

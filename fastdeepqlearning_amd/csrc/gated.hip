@@ -408,9 +408,9 @@ struct ColTile {
 };
 __device__ __forceinline__ unsigned lds_addr(const char *p) { return (unsigned)(uintptr_t)(const __attribute__((address_space(3))) char *)p; }
 // LDS-DMA of 16 bytes per lane, lane l to lds + 16 l.  Written out because the compiler, which knows the builtin, would wait for every DMA in
-// flight in front of each transposing read; nothing comes back into a register, the kernel counts its own waits, and nothing else in it uses M0.
+// flight in front of each transposing read; nothing comes back into a register but M0, and the kernel counts its own waits.
 __device__ __forceinline__ void dma16(const void *src, unsigned lds) {
-  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
 typedef short v4s __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ int2 tr_read(const char *p) {

@@ -13,7 +13,8 @@
 // backward 130; bf16 prompt 16383 x 1 x 1024: carries 65, join 14, outputs 89 us.
 //
 // Lanes without a channel and states behind the last one compute on zeros.  Zero times a step that is infinite or NaN would not stay zero: a
-// tile that holds one (looked at only where there are such states) takes the form that selects, as a tile with a reset does.
+// tile that holds one takes the form that selects, as a tile with a reset does.  Only the kernels for other numbers of states than 8, 16, 32 and
+// 64 (PAD) look for it: the masks cost registers (float windows of 12 states 161 us -> 170, of 16, without them, 168.5 against 166.5).
 //
 // Few rows and a long time axis leave most of the card idle, so the axis is cut into segments: k_scan_fwd<CARRY> gets each segment's
 // final state from a zero start and the sum of its steps (the product of the decays is e^(A sum delta)), k_scan_combine joins
@@ -162,7 +163,7 @@ __device__ __forceinline__ void own_sums(const float v[TS], float out[OWN], int 
 // CARRY: a segment's state at its end from a zero start and the sum of its steps, for segments [0, nseg - 1); no outputs.
 // The S lanes of a channel share the work of a step that does not depend on the state (loads, softplus, gate, store): part s takes the
 // steps S q + s of a tile and hands delta and delta x to the others through LDS.
-template <typename T, int NL, bool CARRY>
+template <typename T, int NL, bool CARRY, bool PAD>
 __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
   constexpr int NP = NL * S, VW = NL < 4 ? NL : 4;         // VW: states read from LDS at once
   typedef float vec __attribute__((ext_vector_type(VW)));
@@ -241,7 +242,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
       lds_d[wave][q * S + s][c] = make_float2(del[q], del[q] * x[q]);
       plain = plain && finite(del[q]) && finite(del[q] * x[q]);
     }
-    const bool wild = p.N < NP && __any(!plain);
+    const bool wild = PAD && __any(!plain);
     wave_lds_fence();
     float acc[TS];
     const auto tile = [&](auto whole) {              // whole: eight finite steps without a reset
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
         if (decltype(whole)::value || i < nt) {
           const float2 v = lds_d[wave][i][c];
           const float dl = v.x, dx = v.y;
-          const int left = decltype(whole)::value ? NL : states_left(p.N, s * NL);
+          const int left = PAD && !decltype(whole)::value ? states_left(p.N, s * NL) : NL;
           if (CARRY) sum += dl;
           const bool cut = !decltype(whole)::value && (rst >> i & 1);
 #pragma unroll
@@ -264,7 +265,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
             for (int j = 0; j < VW; ++j) {
               const float in = dx * B[j], on = fmaf(__builtin_amdgcn_exp2f(dl * A[j4 + j]), h[j4 + j], in);
               h[j4 + j] = cut ? in : on;        // (selected: a decay beyond float's range times zero would not be nothing)
-              if (!decltype(whole)::value && j4 + j >= left) h[j4 + j] = 0.f;
+              if (j4 + j >= left) h[j4 + j] = 0.f;
               if (!CARRY) acc[i] = fmaf(h[j4 + j], C[j], acc[i]);
             }
           }
@@ -301,7 +302,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
 }
 
 // The backward pass's segments: the carry at a segment's start from a zero carry at its end, for segments [1, nseg).
-template <typename T, int NL>
+template <typename T, int NL, bool PAD>
 __global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
   constexpr int NP = NL * S, VW = NL < 4 ? NL : 4;
   typedef float vec __attribute__((ext_vector_type(VW)));
@@ -365,7 +366,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
       lds_d[wave][q * S + s][c] = make_float2(del[q], v[q]);
       plain = plain && finite(del[q]) && finite(v[q]);
     }
-    const bool wild = p.N < NP && __any(!plain);
+    const bool wild = PAD && __any(!plain);
     if (t > t0) fetch(t - TS);
     wave_lds_fence();
     const auto tile = [&](auto whole) {
@@ -374,7 +375,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
         if (decltype(whole)::value || i < nt) {
           const float2 q = lds_d[wave][i][c];
           const float dl = q.x, dy = q.y;
-          const int left = decltype(whole)::value ? NL : states_left(p.N, s * NL);
+          const int left = PAD && !decltype(whole)::value ? states_left(p.N, s * NL) : NL;
           sum += dl;
           const bool cut = !decltype(whole)::value && (rst >> i & 1);
 #pragma unroll
@@ -383,7 +384,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_carry_back(Args a) {
 #pragma unroll
             for (int j = 0; j < VW; ++j) {
               const float g = __builtin_amdgcn_exp2f(dl * A[j4 + j]) * fmaf(dy, C[j], h[j4 + j]);
-              h[j4 + j] = cut || (!decltype(whole)::value && j4 + j >= left) ? 0.f : g;
+              h[j4 + j] = cut || j4 + j >= left ? 0.f : g;
             }
           }
         }
@@ -459,7 +460,7 @@ __global__ __launch_bounds__(64) void k_scan_combine(Args a) {
 }
 
 // --------------------------------------------------------------------------------------------------------------- backward
-template <typename T, int NL>
+template <typename T, int NL, bool PAD>
 __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
   constexpr int NP = NL * S;
   __shared__ __align__(16) float lB[2][TS * NP], lC[2][TS * NP];
@@ -551,7 +552,7 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
       lds_d[wave][q * S + s][c] = v4f{del[q], dx[q], dy[q], 0.f};
       plain = plain && finite(del[q]) && finite(dx[q]) && finite(dy[q]);
     }
-    const bool wild = p.N < NP && __any(!plain);
+    const bool wild = PAD && __any(!plain);
     wave_lds_fence();
     if (t > t0) fetch(t - TS);
     const float *ck = p.checkpoints + lane_slot<NL>(a, t / TS, w) + lane;
@@ -576,13 +577,13 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
             const float dl = st[0], dxi = st[1];
             const float2 B = *reinterpret_cast<const float2 *>(tB + i * NP + m), C = *reinterpret_cast<const float2 *>(tC + i * NP + m);
             const bool cut = !W && (rst >> i & 1);
-            const int left = W ? NL : states_left(p.N, s * NL);
+            const int left = PAD && !W ? states_left(p.N, s * NL) : NL;
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               e[i][j] = __builtin_amdgcn_exp2f(dl * A[m + j]);
               const float in = dxi * (j ? B.y : B.x);
               h[i + 1][j] = cut ? in : fmaf(e[i][j], h[i][j], in);
-              if (!W && m + j >= left) e[i][j] = h[i + 1][j] = 0.f;
+              if (m + j >= left) e[i][j] = h[i + 1][j] = 0.f;
               yc[i] = fmaf(h[i + 1][j], j ? C.y : C.x, yc[i]);
             }
           } else {
@@ -600,12 +601,12 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
             const float dl = st[0], dxi = st[1], dyi = st[2];
             const float2 B = *reinterpret_cast<const float2 *>(tB + i * NP + m), C = *reinterpret_cast<const float2 *>(tC + i * NP + m);
             const bool cut = !W && (rst >> i & 1);
-            const int left = W ? NL : states_left(p.N, s * NL);
+            const int left = PAD && !W ? states_left(p.N, s * NL) : NL;
             float v[4];
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               float g = fmaf(dyi, j ? C.y : C.x, carry[m + j]);
-              if (!W && m + j >= left) g = 0.f;
+              if (m + j >= left) g = 0.f;
               float ga = g * e[i][j], q = ga * h[i][j];
               if (cut) ga = q = 0.f;
               dd[i] = fmaf(q, A[m + j], dd[i]);        // (A log2 e: undone at the end)
@@ -878,27 +879,29 @@ Args args_of(const fdql_scan_t &p, const Plan &q, bool backward) {
 }
 
 template <typename F>
-hipError_t with_states(int NL, F f) {
+hipError_t with_states(int NL, int N, F f) {
+  const auto pad = [&](auto nl) { return N < nl * S ? f(nl, std::true_type()) : f(nl, std::false_type()); };
   switch (NL) {
-    case 2: return f(std::integral_constant<int, 2>());
-    case 4: return f(std::integral_constant<int, 4>());
-    case 8: return f(std::integral_constant<int, 8>());
-    default: return f(std::integral_constant<int, 16>());
+    case 2: return pad(std::integral_constant<int, 2>());
+    case 4: return pad(std::integral_constant<int, 4>());
+    case 8: return pad(std::integral_constant<int, 8>());
+    default: return pad(std::integral_constant<int, 16>());
   }
 }
 
 template <typename T>
 hipError_t fwd(const fdql_scan_t &p, hipStream_t s) {
   const Plan q = plan_of(p);
-  return with_states(q.NL, [&](auto v) {
+  return with_states(q.NL, p.N, [&](auto v, auto padded) {
     constexpr int NL = decltype(v)::value;
+    constexpr bool PAD = decltype(padded)::value;
     const Args a = args_of(p, q, false);
     const int64_t per = (int64_t)p.R * p.G * q.tpg;
     if (q.nseg > 1) {
-      hipLaunchKernelGGL((k_scan_fwd<T, NL, true>), dim3((unsigned)(((q.nseg - 1) * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
+      hipLaunchKernelGGL((k_scan_fwd<T, NL, true, PAD>), dim3((unsigned)(((q.nseg - 1) * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
       hipLaunchKernelGGL((k_scan_combine<NL, 0>), dim3((unsigned)(per * NL)), dim3(64), 0, s, a);
     }
-    hipLaunchKernelGGL((k_scan_fwd<T, NL, false>), dim3((unsigned)((q.nseg * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
+    hipLaunchKernelGGL((k_scan_fwd<T, NL, false, PAD>), dim3((unsigned)((q.nseg * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
     return hipGetLastError();
   });
 }
@@ -906,15 +909,16 @@ hipError_t fwd(const fdql_scan_t &p, hipStream_t s) {
 template <typename T>
 hipError_t bwd(const fdql_scan_t &p, hipStream_t s) {
   const Plan q = plan_of(p);
-  return with_states(q.NL, [&](auto v) {
+  return with_states(q.NL, p.N, [&](auto v, auto padded) {
     constexpr int NL = decltype(v)::value;
+    constexpr bool PAD = decltype(padded)::value;
     const Args a = args_of(p, q, true);
     const int64_t per = (int64_t)p.R * p.G * q.tpg;
     if (q.nseg > 1) {
-      hipLaunchKernelGGL((k_scan_carry_back<T, NL>), dim3((unsigned)(((q.nseg - 1) * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
+      hipLaunchKernelGGL((k_scan_carry_back<T, NL, PAD>), dim3((unsigned)(((q.nseg - 1) * per + WPB - 1) / WPB)), dim3(WPB * 64), 0, s, a);
       hipLaunchKernelGGL((k_scan_combine<NL, 1>), dim3((unsigned)(per * NL)), dim3(64), 0, s, a);
     }
-    hipLaunchKernelGGL((k_scan_bwd<T, NL>), dim3((unsigned)((int64_t)q.nseg * p.R * p.G * q.wgt)), dim3(q.wpw * 64), 0, s, a);
+    hipLaunchKernelGGL((k_scan_bwd<T, NL, PAD>), dim3((unsigned)((int64_t)q.nseg * p.R * p.G * q.wgt)), dim3(q.wpw * 64), 0, s, a);
     const int64_t bc = 2ll * p.T * p.R * p.G * p.N;
     const int nbc = (int)std::min<int64_t>((bc + 1023) / 1024, 4 * CUS);
     hipLaunchKernelGGL((k_scan_finish<T, NL>), dim3((unsigned)(nbc + p.G * q.tpg * (NL + 2))), dim3(1024), 0, s, a, nbc);

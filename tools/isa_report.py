@@ -27,7 +27,7 @@ def kernels_of(path):
     """[(demangled name, {vgpr, agpr, sgpr, vgpr_spill, sgpr_spill, scratch, lds})] of one .hip file."""
     with tempfile.TemporaryDirectory() as td:
         out = os.path.join(td, "k.s")
-        subprocess.run([HIPCC, "-O3", "-std=c++17", "--offload-arch=gfx950", "--cuda-device-only", "-S", path, "-o", out,
+        subprocess.run([HIPCC, "-O3", "-std=c++17", "--offload-arch=gfx950", "--cuda-device-only", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops", "-S", path, "-o", out,
                         "-I", CSRC] + (["-fno-slp-vectorize"] if os.path.basename(path) == "wstat.hip" else []), check=True, capture_output=True)
         text = open(out).read()
     res = []

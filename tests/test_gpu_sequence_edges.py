@@ -298,3 +298,44 @@ def test_scan_errors_are_a_few_roundings(dev, seq, T, R, D, N, G, dtype):
         worst[k] = off / (own * float(o[k].norm()) + (1.05 * once if v.dtype != torch.float32 else 0.0))
     print(T, R, D, N, dtype, {k: round(v, 3) for k, v in worst.items()})
     assert max(worst.values()) <= 1.0, worst
+
+
+def test_offsets_past_32_bits(dev, seq):
+    """Tensors of more than 2^31 elements: the last steps, rows and channels against a call on those alone (the same kernels' bits where each value has its own
+    sums, the definition's neighbourhood for the weights' sums)."""
+    if torch.cuda.mem_get_info(dev)[0] < 60 << 30:
+        pytest.skip("needs 60 GB")
+    T, D, last = 66000, 32768, 40
+    bf, g = torch.bfloat16, torch.Generator(device=dev).manual_seed(1)
+    x = torch.empty(T, 1, D, dtype=bf, device=dev).normal_(generator=g)
+    assert x.numel() > 2 ** 31
+    w = torch.randn(D, 4, device=dev, generator=g) * 0.5
+    tail, state = x[-last:], x[-last - 3:-last].transpose(0, 1)
+    leaf, tail_leaf = x.requires_grad_(), tail.detach().clone().requires_grad_()
+    y, want = seq.causal_conv(leaf, w), seq.causal_conv(tail_leaf, w, initial_state=state.detach())
+    assert torch.equal(y[-last:], want)
+    dy = torch.empty_like(x).normal_(generator=g)
+    dx, = torch.autograd.grad(y, leaf, dy)
+    assert torch.equal(dx[-last:], torch.autograd.grad(want, tail_leaf, dy[-last:])[0])
+    del y, dx, leaf, tail_leaf, want
+    x = x.detach()
+    A, B = -torch.rand(D, 4, device=dev, generator=g) - 0.5, torch.randn(T, 1, 4, device=dev, generator=g).to(bf)
+    reset = torch.zeros(T, 1, dtype=torch.bool, device=dev)
+    reset[-last] = True
+    with torch.no_grad():
+        y, st = seq.selective_scan(x, dy, A, B, B, reset=reset, return_state=True)
+        want, wst = seq.selective_scan(x[-last:], dy[-last:], A, B[-last:], B[-last:], return_state=True)
+    assert torch.equal(y[-last:], want) and torch.allclose(st, wst, rtol=1e-5, atol=1e-6)
+    del y, dy
+    rows = x.view(-1, 512)                                    # 4.2 million rows
+    M, F, k = rows.shape[0], 40, 3000
+    wg, wu = (torch.randn(F, 512, device=dev, generator=g).mul(0.05).to(bf).requires_grad_() for _ in range(2))
+    leaf, tail_leaf = rows.requires_grad_(), rows[-k:].detach().clone().requires_grad_()
+    y, want = seq.gated_linear(leaf, wg, wu), seq.gated_linear(tail_leaf, wg, wu)
+    assert torch.allclose(y[-k:].float(), want.float(), rtol=2 ** -7, atol=1e-5)
+    dy = torch.zeros_like(y)
+    dy[-k:] = torch.randn(k, F, device=dev, generator=g).to(bf)          # only the last rows add to the weights' sums
+    got, ref = torch.autograd.grad(y, [leaf, wg, wu], dy), torch.autograd.grad(want, [tail_leaf, wg, wu], dy[-k:])
+    assert torch.allclose(got[0][-k:].float(), ref[0].float(), rtol=2 ** -7, atol=1e-5) and not got[0][:-k].any()
+    for a, b in zip(got[1:], ref[1:]):
+        assert torch.allclose(a.float(), b.float(), rtol=2 ** -6, atol=2 ** -8 * float(b.abs().max()))

@@ -376,11 +376,11 @@ __global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
 // Shapes: 256 x 256 (KS 32, 4 slices) and 128 x 256 (KS 64, 3 slices) with one workgroup per CU for 16-bit types and many tiles; 64 x 128 for
 // few tiles; 64 x 128 and 128 x 128 for float, whose matrix instructions take so long that the ring needs only two slices and three or two
 // workgroups share a CU.
-// Measured (bf16, 8192 rows, F 4096): forward 502 us at D 4096 = 1095 TFLOP/s, 165 at D 1024 (about 45 us of it outside the contraction: filling
-// the ring, activations, stores); float 12800 x 2048 x 1024 115 TFLOP/s.  What bounds the 16-bit loop is the way from L2 into LDS: with every
-// request at one address it takes 80% of the time, with none 76%, without LDS reads 97%; 128 x 256 tiles, which need half as much again per
-// product, lose a third to it.  Splitting each slice between two groups of four waves (a third fewer LDS reads) gave 172 us instead of 182 for dx
-// and lost as much on the weight gradients.
+// Measured (bf16, 8192 rows, F 4096): forward 508 us at D 4096 = 1082 TFLOP/s, 156 at D 1024 (about 45 us of it outside the contraction: filling
+// the ring, activations, stores); float 12800 x 2048 x 1024 115 TFLOP/s.  What bounds the 16-bit loop is the way from L2 into LDS (copies of the
+// kernel that left one thing out: with every request at one address 80% of the time, with none 76%, without LDS reads 97%); 128 x 256 tiles,
+// which need half as much again per product, lose a third to it.  Splitting each slice between two groups of four waves (a third fewer LDS reads)
+// gave 172 us instead of 182 for dx, of d in one part, and lost as much on the weight gradients.
 __device__ const v4i g_zeros = {0, 0, 0, 0};
 
 template <typename T, int BM, int BN>
@@ -659,7 +659,7 @@ __device__ __forceinline__ T rest_of(float v, T part) {
   const float p = to_f(part);
   return from_f<T>(fabsf(p) < INFINITY ? v - p : 0.f);
 }
-// dg, du of 64 columns x RB rows and their sums over those rows.  Memory bounds it: bf16 8192 x 4096 105 us = 4.5 TB/s.
+// dg, du of 64 columns x RB rows and their sums over those rows.  Memory bounds it: bf16 8192 x 4096 140 us = 4.3 TB/s with d in two parts, 110 = 4.3 in one.
 constexpr int RB = 128;
 template <typename T>
 __global__ __launch_bounds__(256) void k_gated_grad(Args a) {
@@ -765,8 +765,8 @@ Shape shape_of(Choice choice, int64_t rows, int64_t cols, int tile_of_256, int c
   Shape s = {64, 128, 0, 0};
   const auto rounds = [&](int64_t n) { return (n * copies + CUS - 1) / CUS; };      // tiles on the CU that has most
   // float: two workgroups of 128 x 128 on a CU or three of 64 x 128, both near the rate of the matrix units while they share it and slow when the
-  // last one is alone: the larger tile (fewer bytes through LDS) where it needs no more row-steps of the card.  Forward at D 512, F 256:
-  // 12800 rows 79 us -> 70 (800 tiles or 400), 8192 rows 42 either way; where it needs more, 20000 rows, it would take 113 us instead of 101.
+  // last one is alone: the larger tile (fewer bytes through LDS) where it needs no more row-steps of the card.  Forward without `pre` at D 512, F 256:
+  // 12800 rows 79 us -> 70 to 75 (800 tiles or 400), 8192 rows 43 either way; where it needs more, 20000 rows, it would take 113 us instead of 102.
   if (choice == FLOAT && tiles(128, 128) >= CUS && 2 * rounds(tiles(128, 128)) <= rounds(tiles(64, 128))) s.bm = 128;
   // 16 bits: up to half a tile of 128 x 256 per CU the small ones are faster (bf16, D 1024: 128 tiles 19.7 us, as 512 small ones 17.1; 136 tiles 19.2
   // against 24.5; 256 tiles 22.8 against 29.5)
@@ -781,8 +781,9 @@ Shape shape_of(Choice choice, int64_t rows, int64_t cols, int tile_of_256, int c
 }
 
 // Rounding d to 16 bits once would add as much to the gradients' error as rounding the results does (8192 x 1024 x 4096, bf16: 0.0023 of their norm
-// instead of 0.0017), so it is kept in two parts, whatever the size, and each part has its pass in the products: 896 us a training pass there against 564.
-// A caller who would rather have the time asks for one part (FDQL_GATED_ROUND_GRADS).
+// instead of 0.0017), so it is kept in two parts, whatever the size, and each part has its pass in the products: 890 us a training pass there
+// against 564, 12800 x 512 x 256 91 us of kernels against 71, 1024 x 512 x 512 66 against 53.  A caller who would rather have the time asks for one
+// part (FDQL_GATED_ROUND_GRADS).
 struct Plan {
   int Fp, parts, ksplit, kper;
   int64_t rblocks;
@@ -794,7 +795,7 @@ Plan plan_of(const fdql_gated_t &p) {
   q.rblocks = (p.M + RB - 1) / RB;
   // rows split for the 64 x 128 tiles of the weight gradients (larger tiles are chosen where there are enough of them): slices of 256 rows and
   // more, up to three workgroups per CU of float (backward of 4096 x 1024 x 1024 324 us, with two 330, one 369) and two of 16 bits, whose
-  // products are over sooner (12800 x 512 x 256 57 us, with three 61)
+  // products are over sooner (weight gradients of bf16 12800 x 512 x 256 27.9 us, with three 31.6, of 4096 x 1024 x 1024 53.1 and 58.5)
   const int64_t tiles = 2ll * ((p.F + 63) / 64) * ((p.D + 127) / 128);
   const int64_t ks = std::max<int64_t>(1, std::min<int64_t>((p.dtype == FDQL_F32 ? 3 : 2) * CUS / tiles, p.M / 256));
   q.kper = (int)(((p.M + ks - 1) / ks + 63) / 64 * 64);
@@ -806,8 +807,8 @@ int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 bool al16(const void *q) { return ((uintptr_t)q & 15) == 0; }
 
 // Rows that are not whole 16-byte chunks are copied into some that are, whatever the size; the same work with element loads (k_gated_any) took, for
-// forward and backward of bf16 4097 x 1001 x 2730, 1120 us against 272, 1000 x 301 x 203 79 against 49, 64 x 101 x 99 49 against 32, float 12800 x 511 x
-// 256 363 against 269, and only where rows are a few dozen elements long up to 2 us less (forward of 10000 x 17 x 61 6.6 against 7.6).
+// forward and backward of bf16 4097 x 1001 x 2730, 1906 us against 483, 1000 x 301 x 203 118 against 63, 64 x 101 x 99 50 against 34, float 12800 x 511 x
+// 256 365 against 273, and only where rows are a few dozen elements long up to 2 us less (forward of 10000 x 17 x 61 7.3 against 8.3).
 bool packs(const fdql_gated_t &p) {
   const int E = p.dtype == FDQL_F32 ? 4 : 8;
   return p.M > 32 && (p.D % E != 0 || p.x_sr % E != 0);

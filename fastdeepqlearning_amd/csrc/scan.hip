@@ -7,10 +7,11 @@
 // what a step has to do beside its states (loads, softplus, gate, store) is dealt to the quad, two of a tile's eight steps each.  B_t and
 // C_t are the same for the whole wave: they pass through a small LDS tile of eight steps and are read back as broadcasts.  The next tile's
 // reads are under way while one is computed.  Waves of the forward kernels share nothing, so there is no barrier in them.
-// Decays are e^(delta A) = exp2((delta log2 e) A): one multiply and one v_exp_f32 per state and step.  Vector instructions bound the kernels:
-// they are issued in 75 to 82% of all cycles (forward at N 16: five per state and step, of which the power takes four times as long, and
-// some 150 per tile for the rest; backward 18).  Measured: float 50 x 256 x 512, N 16: forward 47 us (213 MB with the checkpoints would take 41),
-// backward 130; bf16 prompt 16383 x 1 x 1024: carries 65, join 14, outputs 89 us.
+// Decays are e^(delta A) = exp2(delta (A log2 e)): one multiply and one v_exp_f32 per state and step; the rounding of A log2 e is one of A's own size.
+// Vector instructions bound the kernels (forward at N 16: five per state and step, of which the power takes four times as long, and some 150 per
+// tile for the rest; backward 18, which are about half of its time, the rest per-tile work and scalar registers held in vector lanes).
+// Measured: float 50 x 256 x 512, N 16: forward 42 us (its 213 MB with the checkpoints would take 41), backward 118; bf16 prompt 16383 x 1 x
+// 1024: carries 57, join 16, outputs 76 us.
 //
 // Lanes without a channel and states behind the last one compute on zeros.  Zero times a step that is infinite or NaN would not stay zero: a
 // tile that holds one takes the form that selects, as a tile with a reset does.  Only the kernels for other numbers of states than 8, 16, 32 and
@@ -77,7 +78,7 @@ __device__ __forceinline__ void pass_edge() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// How many of the N states lie at or behind a lane's first one, worked out where it is asked for (held through the loop it takes a mask for every state).
+// How many of the N states lie at or behind a lane's first one, worked out where it is asked for (the compiler would hold a mask per state through the loop).
 __device__ __forceinline__ int states_left(int N, int first) {
   int left = N - first;
   asm volatile("" : "+v"(left));
@@ -245,7 +246,7 @@ __global__ __launch_bounds__(WPB * 64) void k_scan_fwd(Args a) {
     const bool wild = PAD && __any(!plain);
     wave_lds_fence();
     float acc[TS];
-    const auto tile = [&](auto whole) {              // whole: eight finite steps without a reset
+    const auto tile = [&](auto whole) {              // whole: eight steps without a reset (PAD: and finite)
 #pragma unroll
       for (int i = 0; i < TS; ++i) {
         if (i % 2 == 0) pass_edge();
@@ -562,7 +563,7 @@ __global__ __launch_bounds__(WPB * 64, 2) void k_scan_bwd(Args a) {
 #pragma unroll
     for (int i = 0; i < TS; ++i) yc[i] = dd[i] = gx[i] = 0.f;
     const auto tile = [&](auto whole) {
-      constexpr bool W = decltype(whole)::value;   // eight finite steps without a reset
+      constexpr bool W = decltype(whole)::value;   // eight steps without a reset (PAD: and finite)
       float h0 = ck[0], h1 = ck[64];
 #pragma unroll
       for (int m = 0; m < NL; m += 2) {

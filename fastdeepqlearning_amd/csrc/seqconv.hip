@@ -4,8 +4,8 @@
 // Every value is used K times by the same channel, so a thread owns V neighbouring channels (16 bytes of x where the tensors'
 // alignment allows it, else one) of one row and walks a chunk of steps with the last K inputs in registers: x is read once but for the
 // K - 1 steps in front of a chunk, y written once, and memory bounds it.  A reset clears the window, which also decides the
-// taps in the backward pass.  The steps are read eight (backward: four) ahead of the arithmetic.  Measured, forward: float 50 x 1024 x 1024 90 us =
-// 4.7 TB/s, 50 x 256 x 512 12.3 us; a single step of 32 x 512 3.8 us, of which the launch is most.
+// taps in the backward pass.  The steps are read eight (backward: four) ahead of the arithmetic.  Measured, forward: float 50 x 1024 x 1024 94 us =
+// 4.5 TB/s, bf16 40 us = 5.2 TB/s; float 50 x 256 x 512 13.1 us; a single step of 32 x 512 4.2 us, of which the launch is most.
 //
 // Backward: dpre_t = dy_t SiLU'(pre_t), dx_t = sum_j w[K-1-j] dpre_{t+j} over the steps before the next reset, so a chunk runs K - 1
 // steps past its end.  The weights' sums stay in registers over all chunks that a thread visits, are joined over the four waves of a

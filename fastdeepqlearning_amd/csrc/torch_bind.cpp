@@ -119,20 +119,26 @@ void not_traced(const char *what) {
   using c10::impl::TorchDispatchModeKey;
   using c10::impl::TorchDispatchModeTLS;
   bool traced = torch::jit::tracer::isTracing();
-  for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
-    traced = traced || TorchDispatchModeTLS::get_mode(mode).has_value();
+  if (TorchDispatchModeTLS::any_modes_set())
+    for (const auto mode : {TorchDispatchModeKey::FAKE, TorchDispatchModeKey::PROXY, TorchDispatchModeKey::FUNCTIONAL})
+      traced = traced || TorchDispatchModeTLS::get_mode(mode).has_value();
   TORCH_CHECK(!traced, what, " cannot be traced: its kernels would be missing from the trace (capture the call into a graph instead)");
 }
 // Tensors whose memory holds their values: a subclass that dispatches by itself or a functional transform's wrapper has none of its own, and the operators
 // have no forward-mode derivative, a tangent would be dropped without a word.
-void plain(const char *what, std::initializer_list<Tensor> ts) {
+void plain_one(const char *what, const Tensor &t) {
   constexpr c10::DispatchKeySet foreign({c10::DispatchKey::Python, c10::DispatchKey::Functionalize, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::Batched,
                                          c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::ZeroTensor});
-  for (const Tensor &t : ts) {
-    if (!t.defined()) continue;
-    TORCH_CHECK_VALUE(!t.key_set().has_any(foreign), what, ": plain tensors only, one is a wrapper without memory of its own");
-    TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), what, " has no forward-mode derivative: a tensor carries a tangent");
-  }
+  if (!t.defined()) return;
+  TORCH_CHECK_VALUE(!t.key_set().has_any(foreign), what, ": plain tensors only, one is a wrapper without memory of its own");
+  TORCH_CHECK_VALUE(!t._fw_grad(0).defined(), what, " has no forward-mode derivative: a tensor carries a tangent");
+}
+void plain_one(const char *what, const Opt &t) {
+  if (t.has_value()) plain_one(what, *t);
+}
+template <typename... Ts>
+void plain(const char *what, const Ts &...ts) {
+  (plain_one(what, ts), ...);
 }
 // A tensor that a kernel writes in place counts as changed: a backward pass that saved it refuses, as behind torch's own in-place operators.
 void written(const Tensor &t) {
@@ -285,7 +291,7 @@ std::pair<Tensor, Opt> causal_conv(const Tensor &x, const Tensor &weight, const 
   const char *what = "causal_conv";
   const Tensor bias = val(bias_), reset = val(reset_), state = val(state_);
   not_traced(what);
-  plain(what, {x, weight, bias, state, reset});
+  plain(what, x, weight, bias, state, reset);
   head(what, x, 3);
   conv_check(what, x, weight, bias, state);
   check_reset(what, x, reset);
@@ -300,7 +306,7 @@ std::pair<Tensor, Tensor> causal_conv_step(const Tensor &x, const Opt &state_, c
   const char *what = "causal_conv_step";
   const Tensor bias = val(bias_), reset = val(reset_), state = val(state_), out = val(out_);
   not_traced(what);
-  plain(what, {x, state, weight, bias, out, reset});
+  plain(what, x, state, weight, bias, out, reset);
   head(what, x, 2);
   TORCH_CHECK_VALUE(state.defined(), what, ": a state is needed");
   conv_check(what, x, weight, bias, state);
@@ -432,7 +438,7 @@ std::pair<Tensor, Opt> selective_scan(const Tensor &x, const Tensor &dt, const T
                                       bool softplus, const Opt &reset, const Opt &state, bool want) {
   const char *what = "selective_scan";
   not_traced(what);
-  plain(what, {x, dt, A, B, C, val(skip), val(z), val(dt_bias), val(state), val(reset)});
+  plain(what, x, dt, A, B, C, skip, z, dt_bias, state, reset);
   head(what, x, 3);
   const ScanIn i = scan_check(what, x, dt, A, B, C, val(skip), val(z), val(dt_bias), val(state), val(reset), softplus);
   if (graded({i.x, i.dt, i.A, i.B, i.C, i.skip, i.z, i.dt_bias, i.state})) {
@@ -447,7 +453,7 @@ std::pair<Tensor, Tensor> selective_scan_step(const Tensor &x, const Tensor &dt,
   const char *what = "selective_scan_step";
   const Tensor state = val(state_), out = val(out_);
   not_traced(what);
-  plain(what, {x, dt, A, B, C, state, val(skip), val(z), val(dt_bias), out, val(reset)});
+  plain(what, x, dt, A, B, C, state, skip, z, dt_bias, out, reset);
   head(what, x, 2);
   TORCH_CHECK_VALUE(state.defined(), what, ": a state is needed");
   const ScanIn i = scan_check(what, x, dt, A, B, C, val(skip), val(z), val(dt_bias), state, val(reset), softplus);
@@ -524,7 +530,7 @@ Tensor gated_linear(const Tensor &x, const Tensor &wg, const Tensor &wu, const O
   const char *what = "gated_linear";
   const Tensor bg = val(bg_), bu = val(bu_);
   not_traced(what);
-  plain(what, {x, wg, wu, bg, bu});
+  plain(what, x, wg, wu, bg, bu);
   TORCH_CHECK_VALUE(x.dim() >= 1, what, ": x must be [..., channels]");
   head(what, x, x.dim());
   TORCH_CHECK_VALUE(wg.dim() == 2 && wg.size(0) >= 1, what, ": w_gate must be [features, channels], got ", wg.sizes());

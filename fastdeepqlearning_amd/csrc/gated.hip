@@ -378,7 +378,7 @@ __global__ __launch_bounds__(256, 2) void k_gated_any(Args a) {
 // workgroups share a CU.
 // Measured (bf16, 8192 rows, F 4096): forward 508 us at D 4096 = 1082 TFLOP/s, 156 at D 1024 (about 45 us of it outside the contraction: filling
 // the ring, activations, stores); float 12800 x 2048 x 1024 115 TFLOP/s.  What bounds the 16-bit loop is the way from L2 into LDS (copies of the
-// kernel that left one thing out: with every request at one address 80% of the time, with none 76%, without LDS reads 97%); 128 x 256 tiles,
+// kernel that left one thing out: with every request at one address 80% of the time, with none 76%, with one slice's LDS reads for all 97%); 128 x 256 tiles,
 // which need half as much again per product, lose a third to it.  Splitting each slice between two groups of four waves (a third fewer LDS reads)
 // gave 172 us instead of 182 for dx, of d in one part, and lost as much on the weight gradients.
 __device__ const v4i g_zeros = {0, 0, 0, 0};

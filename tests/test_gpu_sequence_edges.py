@@ -339,3 +339,19 @@ def test_offsets_past_32_bits(dev, seq):
     assert torch.allclose(got[0][-k:].float(), ref[0].float(), rtol=2 ** -7, atol=1e-5) and not got[0][:-k].any()
     for a, b in zip(got[1:], ref[1:]):
         assert torch.allclose(a.float(), b.float(), rtol=2 ** -6, atol=2 ** -8 * float(b.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=["bf16", "f16"])
+def test_gated_weights_of_the_widest_tiles(dev, seq, dtype):
+    """Weights large enough for 256 x 256 tiles in the weight gradients (512 of them, two for each CU) and few rows behind them, in two parts and in one: the bounds of
+    test_gated_gradients_round_once_at_every_size, a last row tile that is not whole."""
+    M, D, F = 200, 4096, 4090
+    x, wg, wu, bg, bu, dy = _gated_inputs(dev, M, D, F, dtype, True, seed=2)
+    o = osq.gated_linear(x, wg, wu, bg, bu, "silu", dy)
+    for rounded, low, high in ((False, 0.0, 1.05), (True, 1.1, 1.6)):
+        leaves = [t.detach().requires_grad_() for t in (x, wg, wu, bg, bu)]
+        grads = torch.autograd.grad(seq.gated_linear(*leaves, rounded_grads=rounded), leaves, dy)
+        ratio = {n: _norm_ratio(g, o[n]) for n, g in zip(("dx", "dw_gate", "dw_up", "db_gate", "db_up"), grads)}
+        print(dtype, ratio)
+        assert all((r <= high) for r in ratio.values()) and all(ratio[n] >= low for n in ("dx", "dw_gate", "dw_up")), ratio
+        assert max(ratio["db_gate"], ratio["db_up"]) <= 1.05                    # (sums of the unrounded values either way)

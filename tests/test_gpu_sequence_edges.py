@@ -355,3 +355,43 @@ def test_gated_weights_of_the_widest_tiles(dev, seq, dtype):
         print(dtype, ratio)
         assert all((r <= high) for r in ratio.values()) and all(ratio[n] >= low for n in ("dx", "dw_gate", "dw_up")), ratio
         assert max(ratio["db_gate"], ratio["db_up"]) <= 1.05                    # (sums of the unrounded values either way)
+
+
+def test_threads_at_once(dev, seq):
+    """Training passes of four threads, each on a stream of its own, have the bits of lone ones; an error in one of them is that thread's own."""
+    import threading
+    jobs = []
+    for k in range(4):
+        g = _gen(40 + k)
+        i, rst, dy, _ = _scan_inputs(dev, 130 + k, 2, 40 + 8 * k, 12 + k, 1, torch.float32, "dense", seed=k)
+        w, wg = torch.randn(40 + 8 * k, 4, generator=g).to(dev), torch.randn(24, 40 + 8 * k, generator=g).to(dev).to(torch.bfloat16)
+
+        def job(i=i, rst=rst, dy=dy, w=w, wg=wg):
+            li = {n: v.detach().requires_grad_() for n, v in i.items()}
+            y = _scan_call(seq, dict(li, x=seq.causal_conv(li["x"], w, reset=rst)), rst, True)
+            out = seq.gated_linear(y.to(torch.bfloat16), wg, wg)
+            return [out.detach()] + list(torch.autograd.grad(out.float().sum() + (y * dy).sum(), list(li.values())))
+        jobs.append(job)
+    want = [job() for job in jobs]
+    torch.cuda.synchronize(dev)
+    got, errors = [None] * 4, []
+
+    def run(k):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream(dev)):
+                for _ in range(5):
+                    got[k] = jobs[k]()
+                    with pytest.raises(ValueError, match="weight must be"):
+                        seq.causal_conv(torch.zeros(2, 1, 8 + k, device=dev), torch.zeros(3, 4, device=dev))
+                torch.cuda.current_stream(dev).synchronize()
+        except BaseException as e:      # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=run, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for a, b in zip(got, want):
+        for p, q in zip(a, b):
+            assert torch.equal(p, q)
